@@ -1,0 +1,138 @@
+// Element types, 16-byte row pieces and the 8-bit checkpoint format, shared by the kernels of
+// norm.hip (group norm), ckpt8.hip (checkpoint write / read) and wgrad8.hip (weight gradients).
+//
+// Checkpoint format.  A row of C values is cut into blocks of 32 consecutive channels.  A block
+// holds one byte s and a signed code per value, value = code * 2^(s - 127), where e = s - 127 is the
+// least integer >= -126 with max|x| <= 127 * 2^e and code = x / 2^e rounded to nearest, ties to
+// even: off by at most 2^(e-1) <= max|x| / 127.  A power of two as the scale keeps every step
+// exact: x / 2^e is an exponent shift, and code * 2^e has at most 7 significant bits and is a
+// value of bfloat16, of float and (inside its range) of half.  A block with an infinity or a NaN
+// has s = 255 and codes 0 and reads as NaN throughout.
+// Codes of a row take ld = 16 * ceil(C / 16) bytes (the tail is zero) so that every row can be read
+// in 16-byte pieces; scales take ceil(C / 32) bytes.
+#pragma once
+#include "gvae_common.h"
+
+namespace gvae {
+
+constexpr int kBlock8 = 32;
+inline int ckpt8_ld(int C) { return (C + 15) / 16 * 16; }
+inline int ckpt8_blocks(int C) { return (C + kBlock8 - 1) / kBlock8; }
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+// a 16-byte piece of a row, at the alignment of its element (the hardware takes any)
+template <class T>
+struct Piece {
+  static constexpr int V = 16 / (int)sizeof(T);
+  typedef T raw __attribute__((ext_vector_type(16 / sizeof(T))));
+  typedef raw mem __attribute__((aligned(sizeof(T))));
+};
+
+// nv (1..V) leading elements of the piece at p, zero behind them
+template <class T>
+__device__ __forceinline__ typename Piece<T>::raw load_piece(const T *p, int nv) {
+  constexpr int V = Piece<T>::V;
+  if (nv == V) return *reinterpret_cast<const typename Piece<T>::mem *>(p);
+  typename Piece<T>::raw r;
+#pragma unroll
+  for (int v = 0; v < V; ++v) r[v] = v < nv ? p[v] : (T)0.0f;
+  return r;
+}
+template <class T>
+__device__ __forceinline__ void store_piece(T *p, const float *f, int nv) {
+  constexpr int V = Piece<T>::V;
+  typename Piece<T>::raw r;
+#pragma unroll
+  for (int v = 0; v < V; ++v) r[v] = (T)f[v];
+  if (nv == V) {
+    *reinterpret_cast<typename Piece<T>::mem *>(p) = r;
+    return;
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    if (v < nv) p[v] = r[v];
+}
+
+__device__ __forceinline__ float pow2_field(uint32_t field) { return __uint_as_float(field << 23); }
+
+// max over the 2, 4 or 8 neighbouring lanes that share a block (lane groups aligned to their size)
+template <int W>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t m) {
+  static_assert(W == 1 || W == 2 || W == 4 || W == 8, "lanes of a block");
+  if (W >= 2) m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xf, 0xf, false));
+  if (W >= 4) m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xf, 0xf, false));
+  // (mirror within 8 lanes: by now each half of four holds one value)
+  if (W >= 8) m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xf, 0xf, false));
+  return m;
+}
+
+// The scale byte of a block from the largest bit pattern of |x| in it: with |x| = 1.M * 2^(E-127),
+// 127 * 2^e reaches it for e = E - 133 as long as 1.M <= 127/64, and for e = E - 132 always.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t absmax) {
+  if (absmax >= 0x7f800000u) return 255u;
+  const int s = (int)(absmax >> 23) - 6 + ((absmax & 0x7fffffu) > 0x7e0000u ? 1 : 0);
+  return (uint32_t)(s < 1 ? 1 : s);
+}
+
+// V values of a row's block, spread over W = 32 / V neighbouring lanes that all make this call:
+// codes to `codes` (ld bytes a row, nc of this lane's places inside it) and the block's byte.
+// Places behind the last channel are given as 0.
+template <int V>
+__device__ __forceinline__ void emit8(const float *f, int8_t *codes, int nc, uint8_t *scale, bool first) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int v = 0; v < V; ++v) m = max(m, __float_as_uint(f[v]) & 0x7fffffffu);
+  m = lanes_max<kBlock8 / V>(m);
+  const uint32_t s = scale_byte(m);
+  // (a largest value that rounds up to 2^128 is kept below it)
+  const float lim = s == 249u ? 63.0f : 127.0f;
+  const float inv = s == 255u ? 0.0f : pow2_field(254u - s);
+  uint32_t w[(V + 3) / 4];
+#pragma unroll
+  for (int q = 0; q < V / 4; ++q) {
+    uint32_t p = 0;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const float c = s == 255u ? 0.0f : rintf(f[4 * q + v] * inv);
+      p |= ((uint32_t)(int)fminf(fmaxf(c, -lim), lim) & 0xffu) << (8 * v);
+    }
+    w[q] = p;
+  }
+  if (nc >= V) {
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q) reinterpret_cast<uint32_t *>(codes)[q] = w[q];
+  }
+  if (first) *scale = (uint8_t)s;
+}
+
+// V codes at `codes` (aligned to V bytes) times their block's power of two
+template <int V>
+struct Codes {
+  uint32_t w[V / 4];
+};
+template <int V>
+__device__ __forceinline__ Codes<V> load_codes(const int8_t *codes) {
+  Codes<V> r;
+#pragma unroll
+  for (int q = 0; q < V / 4; ++q) r.w[q] = reinterpret_cast<const uint32_t *>(codes)[q];
+  return r;
+}
+template <int V>
+__device__ __forceinline__ void decode8(const Codes<V> &c, float p, float *f) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) f[v] = (float)(int8_t)(c.w[v >> 2] >> (8 * (v & 3))) * p;
+}
+
+#define GVAE_DTYPE_SWITCH(dtype, T, ...)                                  \
+  switch (dtype) {                                                       \
+    case GVAE_F32: { typedef float T; __VA_ARGS__; } break;              \
+    case GVAE_BF16: { typedef gvae::bf16_t T; __VA_ARGS__; } break;      \
+    default: { typedef gvae::f16_t T; __VA_ARGS__; } break;              \
+  }
+
+inline int dtype_bytes(int dtype) { return dtype == GVAE_F32 ? 4 : 2; }
+inline bool dtype_known(int dtype) { return dtype >= GVAE_F32 && dtype <= GVAE_F16; }
+
+}  // namespace gvae

@@ -1,0 +1,297 @@
+"""Group norm with an activation, 8-bit activation checkpoints and the gradients that read them.
+
+Operators on node features laid out (graphs, rows, channels), channels last, on the current HIP
+stream of the current device (libgvae_hip.so; there is no CPU fallback):
+
+  group_norm_act            forward, optionally leaving 8-bit checkpoints of its input and output
+  group_norm_act_backward   gradients, from the input or from its checkpoint
+  checkpoint8               an activation into an 8-bit checkpoint; Checkpoint8.read() brings it back
+  linear_wgrad8             weight and bias gradient of a linear layer from its input's checkpoint
+
+They are plain calls: nothing here is recorded by autograd.  `GraphVAE(norm="group")` builds its
+encoder from the same kernels, and its backward from the gradients here.
+"""
+from __future__ import annotations
+
+from ctypes import c_float, c_int, c_int64, c_void_p
+from typing import NamedTuple
+
+import torch
+
+from . import _hip
+
+_DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_ACT = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+BLOCK = 32
+
+_bound = None
+
+
+def _bind():
+    global _bound
+    if _bound is None:
+        L = _hip.lib()
+        L.gvae_ckpt8_write.argtypes = [c_void_p, c_int, c_int64, c_int, c_int64, c_void_p, c_void_p, c_void_p]
+        L.gvae_ckpt8_read.argtypes = [c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int, c_int64, c_void_p]
+        L.gvae_group_norm_ws_bytes.argtypes = [c_int] * 4
+        L.gvae_group_norm_ws_bytes.restype = c_int64
+        L.gvae_group_norm_fwd.argtypes = [c_void_p, c_int, c_int64, c_int64, c_void_p, c_int, c_int, c_int, c_int,
+                                          c_void_p, c_void_p, c_float, c_int] + [c_void_p] * 9
+        L.gvae_group_norm_bwd.argtypes = ([c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_int64]
+                                          + [c_void_p] * 3 + [c_int] * 4 + [c_void_p] * 4 + [c_int]
+                                          + [c_void_p] * 5)
+        L.gvae_linear_wgrad8_ws_bytes.argtypes = [c_int64, c_int, c_int]
+        L.gvae_linear_wgrad8_ws_bytes.restype = c_int64
+        L.gvae_linear_wgrad8.argtypes = [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int,
+                                         c_void_p, c_void_p, c_void_p, c_void_p]
+        _bound = L
+    return _bound
+
+
+def _act_code(act: str) -> int:
+    if act not in _ACT:
+        raise ValueError(f"act must be one of {sorted(_ACT)}, got {act!r}")
+    return _ACT[act]
+
+
+def _on_device(t: torch.Tensor, what: str) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise _hip.GvaeHipError(f"{what}: expected a device tensor (the HIP path has no CPU fallback)")
+    if t.device.index != torch._C._cuda_getDevice():
+        raise _hip.GvaeHipError(f"{what} on {t.device} but the current device is cuda:"
+                                f"{torch.cuda.current_device()}: wrap the call in torch.cuda.device(...)")
+    return t
+
+
+def _activation(t: torch.Tensor, what: str, shape=None, dtype=None) -> int:
+    """Checks an activation or gradient of any row and batch stride; returns its type code."""
+    _on_device(t, what)
+    code = _DTYPE.get(t.dtype)
+    if code is None or (dtype is not None and t.dtype != dtype):
+        raise _hip.GvaeHipError(f"{what}: expected {dtype or 'float32, bfloat16 or float16'}, got {t.dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise _hip.GvaeHipError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.numel() == 0:
+        raise _hip.GvaeHipError(f"{what}: no element in shape {tuple(t.shape)}")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise _hip.GvaeHipError(f"{what}: channels must be last and contiguous, got strides {t.stride()}")
+    return code
+
+
+def _rows_of(t: torch.Tensor, what: str) -> tuple[int, int]:
+    """(rows, elements between rows) of an activation seen as a matrix."""
+    C = t.shape[-1]
+    if t.is_contiguous():
+        return t.numel() // C, C
+    if t.dim() == 2 and (t.shape[0] == 1 or t.stride(0) >= C):
+        return t.shape[0], max(t.stride(0), C)
+    raise _hip.GvaeHipError(f"{what}: expected a contiguous tensor or a matrix of evenly spaced rows, got shape "
+                            f"{tuple(t.shape)} with strides {t.stride()}")
+
+
+def _graph_strides(t: torch.Tensor, what: str) -> tuple[int, int]:
+    """(batch stride, row stride) of (graphs, rows, channels); an axis of length 1 has none of its own."""
+    B, N, C = t.shape
+    row = t.stride(1) if N > 1 else C
+    batch = t.stride(0) if B > 1 else 0
+    if row < C:
+        raise _hip.GvaeHipError(f"{what}: rows overlap (strides {t.stride()})")
+    return batch, row
+
+
+class Checkpoint8:
+    """An activation kept in 8 bits: `codes` (..., 16*ceil(C/16)) int8 and `scales` (..., ceil(C/32))
+    uint8, value = code * 2^(scale - 127) with one scale per 32 consecutive channels of a row (each
+    value off by at most 1/127 of its block's largest).  `channels` is C; `dtype` what `read` returns."""
+
+    __slots__ = ("codes", "scales", "channels", "dtype")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, channels: int,
+                 dtype: torch.dtype = torch.bfloat16) -> None:
+        C = int(channels)
+        lead = tuple(codes.shape[:-1])
+        if (C < 1 or codes.dtype != torch.int8 or scales.dtype != torch.uint8
+                or tuple(codes.shape) != lead + ((C + 15) // 16 * 16,)
+                or tuple(scales.shape) != lead + ((C + 31) // 32,)):
+            raise _hip.GvaeHipError(f"Checkpoint8 of {C} channels: codes {tuple(codes.shape)} {codes.dtype}, scales "
+                                    f"{tuple(scales.shape)} {scales.dtype}")
+        if not (codes.is_contiguous() and scales.is_contiguous()) or codes.device != scales.device:
+            raise _hip.GvaeHipError("Checkpoint8: codes and scales must be contiguous and on one device")
+        if dtype not in _DTYPE:
+            raise _hip.GvaeHipError(f"Checkpoint8: cannot be read as {dtype}")
+        if codes.data_ptr() % 16:
+            raise _hip.GvaeHipError("Checkpoint8: codes must be 16-byte aligned")
+        self.codes, self.scales, self.channels, self.dtype = codes, scales, C, dtype
+
+    @property
+    def shape(self) -> tuple[int, ...]:
+        return tuple(self.codes.shape[:-1]) + (self.channels,)
+
+    def _check(self, what: str) -> "Checkpoint8":
+        _on_device(self.codes, what)
+        if self.codes.numel() == 0:
+            raise _hip.GvaeHipError(f"{what}: no element in shape {self.shape}")
+        return self
+
+    def read(self, dtype: torch.dtype | None = None) -> torch.Tensor:
+        """The values the checkpoint stands for, as `dtype` (default: the type that was written);
+        exact in bfloat16 and float32."""
+        dtype = self.dtype if dtype is None else dtype
+        if dtype not in _DTYPE:
+            raise _hip.GvaeHipError(f"Checkpoint8.read: cannot be read as {dtype}")
+        self._check("Checkpoint8.read")
+        out = torch.empty(self.shape, dtype=dtype, device=self.codes.device)
+        C = self.channels
+        _hip._check(_bind().gvae_ckpt8_read(self.codes.data_ptr(), self.scales.data_ptr(), out.numel() // C, C,
+                                            out.data_ptr(), _DTYPE[dtype], C, _hip._stream()))
+        return out
+
+
+def _empty8(shape, device, dtype) -> Checkpoint8:
+    C = shape[-1]
+    lead = tuple(shape[:-1])
+    return Checkpoint8(torch.empty(lead + ((C + 15) // 16 * 16,), dtype=torch.int8, device=device),
+                       torch.empty(lead + ((C + 31) // 32,), dtype=torch.uint8, device=device), C, dtype)
+
+
+def checkpoint8(x: torch.Tensor) -> Checkpoint8:
+    """8-bit checkpoint of x (..., C) float32 / bfloat16 / float16: contiguous, or a matrix with any
+    row stride.  A block of 32 channels that holds an infinity or a NaN reads back as NaN."""
+    code = _activation(x, "checkpoint8")
+    if x.dim() < 1:
+        raise _hip.GvaeHipError("checkpoint8: expected at least one axis")
+    rows, ld = _rows_of(x, "checkpoint8")
+    c = _empty8(x.shape, x.device, x.dtype)
+    _hip._check(_bind().gvae_ckpt8_write(x.data_ptr(), code, rows, x.shape[-1], ld, c.codes.data_ptr(),
+                                         c.scales.data_ptr(), _hip._stream()))
+    return c
+
+
+class GroupNormOut(NamedTuple):
+    y: torch.Tensor             # (graphs, rows, channels), x's type
+    mean: torch.Tensor          # (graphs, groups) float32
+    rstd: torch.Tensor          # (graphs, groups) float32
+    x8: Checkpoint8 | None      # checkpoint of x, if asked for
+    y8: Checkpoint8 | None      # checkpoint of y, if asked for
+
+
+def _norm_params(weight, bias, C: int, what: str):
+    for t in (weight, bias):
+        if t is not None:
+            _hip._dev(t, torch.float32)
+            if tuple(t.shape) != (C,):
+                raise _hip.GvaeHipError(f"{what}: weight and bias must have shape ({C},), got {tuple(t.shape)}")
+    return (weight.data_ptr() if weight is not None else None, bias.data_ptr() if bias is not None else None)
+
+
+def _live_rows(rows, B: int, what: str):
+    if rows is None:
+        return None
+    _hip._dev(rows, torch.int32)
+    if tuple(rows.shape) != (B,):
+        raise _hip.GvaeHipError(f"{what}: rows must have shape ({B},), got {tuple(rows.shape)}")
+    return rows.data_ptr()
+
+
+def _norm_sizes(x_shape, groups: int, what: str):
+    if len(x_shape) != 3:
+        raise _hip.GvaeHipError(f"{what}: expected (graphs, rows, channels), got shape {tuple(x_shape)}")
+    B, N, C = x_shape
+    if groups < 1 or C % groups:
+        raise ValueError(f"{what}: {C} channels do not divide into {groups} groups")
+    return B, N, C
+
+
+def group_norm_act(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, groups: int, *,
+                   act: str = "relu", eps: float = 1e-5, rows: torch.Tensor | None = None, keep_x: bool = False,
+                   keep_y: bool = False) -> GroupNormOut:
+    """act(group_norm(x) * weight + bias) over each graph's live rows and `groups` runs of consecutive
+    channels.
+
+    x: (graphs, rows, channels) float32 / bfloat16 / float16, channels contiguous, any row and batch
+    strides.  weight, bias: (channels,) float32 or None.  act: none | relu | silu | gelu (the erf form).
+    rows: live rows per graph (int32), None = all; rows behind them are not read and come out 0, a
+    graph without any has mean 0 and variance 0.  keep_x / keep_y: also return 8-bit checkpoints of x
+    (dead rows as 0) and of y, the same as `checkpoint8` of them."""
+    what = "group_norm_act"
+    B, N, C = _norm_sizes(x.shape, groups, what)
+    code, act_code = _activation(x, what), _act_code(act)
+    batch, row = _graph_strides(x, what)
+    w, b = _norm_params(weight, bias, C, what)
+    live = _live_rows(rows, B, what)
+    if not eps > 0.0:
+        raise ValueError(f"{what}: eps must be positive, got {eps}")
+    L, dev = _bind(), x.device
+    y = torch.empty((B, N, C), dtype=x.dtype, device=dev)
+    stats = torch.empty((2, B, groups), dtype=torch.float32, device=dev)
+    x8 = _empty8(x.shape, dev, x.dtype) if keep_x else None
+    y8 = _empty8(x.shape, dev, x.dtype) if keep_y else None
+    ws = torch.empty(L.gvae_group_norm_ws_bytes(B, N, C, groups), dtype=torch.uint8, device=dev)
+    mean, rstd = stats[0], stats[1]
+    _hip._check(L.gvae_group_norm_fwd(
+        x.data_ptr(), code, batch, row, live, B, N, C, groups, w, b, eps, act_code, y.data_ptr(), mean.data_ptr(),
+        rstd.data_ptr(), x8.codes.data_ptr() if keep_x else None, x8.scales.data_ptr() if keep_x else None,
+        y8.codes.data_ptr() if keep_y else None, y8.scales.data_ptr() if keep_y else None, ws.data_ptr(),
+        _hip._stream()))
+    return GroupNormOut(y, mean, rstd, x8, y8)
+
+
+def group_norm_act_backward(dy: torch.Tensor, x, weight: torch.Tensor | None, bias: torch.Tensor | None,
+                            mean: torch.Tensor, rstd: torch.Tensor, groups: int, *, act: str = "relu",
+                            rows: torch.Tensor | None = None):
+    """Gradients of `group_norm_act`: (dx, dweight, dbias), dx of dy's type, the others float32 (summed
+    over graphs and rows in a fixed order).  x: the forward's input, of dy's type, or its Checkpoint8;
+    mean, rstd: as the forward returned them; weight, bias, groups, act, rows: as given to it.  dy: like x
+    of any row and batch strides (an expanded gradient is read in place).  dx of dead rows is 0."""
+    what = "group_norm_act_backward"
+    kept = isinstance(x, Checkpoint8)
+    B, N, C = _norm_sizes(dy.shape, groups, what)
+    code, act_code = _activation(dy, what), _act_code(act)
+    if kept:
+        x._check(what)
+        if x.shape != (B, N, C):
+            raise _hip.GvaeHipError(f"{what}: checkpoint of shape {x.shape}, gradient {tuple(dy.shape)}")
+        xs, xb, xr, x8, x8s = None, 0, C, x.codes.data_ptr(), x.scales.data_ptr()
+    else:
+        _activation(x, what, dy.shape, dy.dtype)
+        xb, xr = _graph_strides(x, what)
+        xs, x8, x8s = x.data_ptr(), None, None
+    db_, dr_ = _graph_strides(dy, what)
+    w, b = _norm_params(weight, bias, C, what)
+    live = _live_rows(rows, B, what)
+    for t in (mean, rstd):
+        _hip._dev(t, torch.float32)
+        if tuple(t.shape) != (B, groups):
+            raise _hip.GvaeHipError(f"{what}: mean and rstd must have shape ({B}, {groups}), got {tuple(t.shape)}")
+    L, dev = _bind(), dy.device
+    dx = torch.empty((B, N, C), dtype=dy.dtype, device=dev)
+    grads = torch.empty((2, C), dtype=torch.float32, device=dev)
+    ws = torch.empty(L.gvae_group_norm_ws_bytes(B, N, C, groups), dtype=torch.uint8, device=dev)
+    dweight, dbias = grads[0], grads[1]
+    _hip._check(L.gvae_group_norm_bwd(
+        dy.data_ptr(), code, db_, dr_, xs, xb, xr, x8, x8s, live, B, N, C, groups, w, b, mean.data_ptr(),
+        rstd.data_ptr(), act_code, dx.data_ptr(), dweight.data_ptr(), dbias.data_ptr(), ws.data_ptr(),
+        _hip._stream()))
+    return dx, dweight, dbias
+
+
+def linear_wgrad8(dy: torch.Tensor, x8: Checkpoint8) -> tuple[torch.Tensor, torch.Tensor]:
+    """(dweight (O, I), dbias (O)) of a linear layer y = x W^T + b, in dy's type, from its output's
+    gradient dy (..., O) and the checkpoint of its input (..., I).  dy: contiguous, or a matrix with any
+    row stride.  Every product is exact, sums are float32 in a fixed order, rounded once."""
+    what = "linear_wgrad8"
+    if not isinstance(x8, Checkpoint8):
+        raise _hip.GvaeHipError(f"{what}: the input must be a Checkpoint8")
+    x8._check(what)
+    code = _activation(dy, what)
+    if dy.dim() < 2 or tuple(dy.shape[:-1]) != x8.shape[:-1]:
+        raise _hip.GvaeHipError(f"{what}: gradient {tuple(dy.shape)} and checkpoint {x8.shape} differ in their rows")
+    rows, ld = _rows_of(dy, what)
+    O, I = dy.shape[-1], x8.channels
+    L, dev = _bind(), dy.device
+    dw = torch.empty((O, I), dtype=dy.dtype, device=dev)
+    db = torch.empty((O,), dtype=dy.dtype, device=dev)
+    ws = torch.empty(L.gvae_linear_wgrad8_ws_bytes(rows, O, I), dtype=torch.uint8, device=dev)
+    _hip._check(L.gvae_linear_wgrad8(dy.data_ptr(), code, ld, x8.codes.data_ptr(), x8.scales.data_ptr(), rows, O, I,
+                                     dw.data_ptr(), db.data_ptr(), ws.data_ptr(), _hip._stream()))
+    return dw, db

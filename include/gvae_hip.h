@@ -366,6 +366,73 @@ int gvae_sample_decode(const gvae_dims *d, const float *d_params, const float *d
                        uint8_t *d_adj, uint8_t *d_exists, int32_t *d_count, void *d_ws,
                        void *stream);
 
+/* ===========================================================================
+ * Group norm with an activation and 8-bit activation checkpoints.  No counterpart in the
+ * reference, whose encoder normalises with BatchNorm (graphvae/models/model.py:71-76) and keeps
+ * every activation for the backward in fp32.
+ * =========================================================================== */
+
+/* Element types of the activations and their gradients. */
+#define GVAE_F32 0
+#define GVAE_BF16 1
+#define GVAE_F16 2
+
+#define GVAE_ACT_NONE 0
+#define GVAE_ACT_RELU 1
+#define GVAE_ACT_SILU 2
+#define GVAE_ACT_GELU 3   /* z/2 * (1 + erf(z / sqrt 2)) */
+
+/* An 8-bit checkpoint of a (rows, C) activation: per row, gvae_ckpt8_row_bytes(C) code bytes
+ * (16 * ceil(C/16), zero behind the C-th) and gvae_ckpt8_row_scales(C) = ceil(C/32) scale bytes.
+ * The value of channel c is code[c] * 2^(scale[c/32] - 127).  When written, a block's power of two
+ * is the least one (at least 2^-126) of which 127 reach the block's largest magnitude, and codes
+ * are rounded to nearest, ties to even; a block with an infinity or a NaN gets the scale byte 255
+ * and reads as NaN.  d_codes must be 16-byte aligned. */
+int gvae_ckpt8_row_bytes(int C);
+int gvae_ckpt8_row_scales(int C);
+/* d_x: (rows, C) with unit channel stride and row_stride elements between rows. */
+int gvae_ckpt8_write(const void *d_x, int dtype, int64_t rows, int C, int64_t row_stride, int8_t *d_codes,
+                     uint8_t *d_scales, void *stream);
+/* Exact in bf16 and fp32; in fp16 values outside its range become its largest, small ones are rounded. */
+int gvae_ckpt8_read(const int8_t *d_codes, const uint8_t *d_scales, int64_t rows, int C, void *d_x, int dtype,
+                    int64_t row_stride, void *stream);
+
+/* Bytes of scratch for either call below, whatever the element type. */
+int64_t gvae_group_norm_ws_bytes(int B, int N, int C, int G);
+
+/* y = act(w * (x - mean) / sqrt(var + eps) + b), mean and variance over a graph's live rows and the
+ * C/G consecutive channels of a group.
+ *   d_x       (B, N, C): unit channel stride, any row stride >= C and batch stride >= 0 (elements)
+ *   d_rows    live rows of each graph, clamped to [0, N]; NULL = N for all.  Rows of x behind them
+ *             are not read; their y is 0.  A graph without a live row has mean 0 and variance 0.
+ *   d_weight, d_bias   C floats each; NULL = ones / zeros
+ *   d_y       (B, N, C) contiguous;  d_mean, d_rstd  (B, G) floats
+ *   d_x8, d_y8 (with their scales; either may be NULL): checkpoints of x (0 in dead rows) and of y as
+ *             returned, B*N rows, equal to what gvae_ckpt8_write makes of them */
+int gvae_group_norm_fwd(const void *d_x, int dtype, int64_t batch_stride, int64_t row_stride, const int32_t *d_rows,
+                        int B, int N, int C, int G, const float *d_weight, const float *d_bias, float eps, int act,
+                        void *d_y, float *d_mean, float *d_rstd, int8_t *d_x8, uint8_t *d_x8_scales, int8_t *d_y8,
+                        uint8_t *d_y8_scales, void *d_ws, void *stream);
+
+/* Gradients of gvae_group_norm_fwd from the mean and rstd it returned and either the input (d_x) or
+ * its checkpoint (d_x8, d_x8_scales; the other NULL).  d_dx (B, N, C) contiguous, 0 in dead rows;
+ * d_dweight and d_dbias (C floats each, summed over graphs and rows in a fixed order) both or
+ * neither.  dy of dead rows is not read. */
+int gvae_group_norm_bwd(const void *d_dy, int dtype, int64_t dy_batch_stride, int64_t dy_row_stride, const void *d_x,
+                        int64_t batch_stride, int64_t row_stride, const int8_t *d_x8, const uint8_t *d_x8_scales,
+                        const int32_t *d_rows, int B, int N, int C, int G, const float *d_weight,
+                        const float *d_bias, const float *d_mean, const float *d_rstd, int act, void *d_dx,
+                        float *d_dweight, float *d_dbias, void *d_ws, void *stream);
+
+/* Weight and bias gradient of a linear layer whose input (rows, I) was kept as a checkpoint:
+ * d_dw (O, I) = dY^T x, d_db (O) = column sums of dY (may be NULL), both contiguous and of dY's type.
+ * Every product of a gradient and a checkpointed value enters the sums exactly; sums are fp32, in a
+ * fixed order.  d_ws: gvae_linear_wgrad8_ws_bytes(rows, O, I) bytes. */
+int64_t gvae_linear_wgrad8_ws_bytes(int64_t rows, int O, int I);
+int gvae_linear_wgrad8(const void *d_dy, int dtype, int64_t row_stride, const int8_t *d_codes,
+                       const uint8_t *d_scales, int64_t rows, int O, int I, void *d_dw, void *d_db, void *d_ws,
+                       void *stream);
+
 #ifdef __cplusplus
 }
 #endif
