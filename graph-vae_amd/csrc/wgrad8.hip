@@ -1,6 +1,20 @@
 // Weight and bias gradient of a linear layer y = x W^T + b from the 8-bit checkpoint of its input:
 //   dW[o,i] = sum_t dY[t,o] * code[t,i] * 2^(s[t,i/32] - 127),   db[o] = sum_t dY[t,o]
-// Rows are split over work-groups; the parts are summed in their order by a second launch.
+//
+// On the matrix cores in bf16 without a rounding of either factor: code * 2^e has 7 significant bits
+// and is a bf16 value as it stands; a gradient is cut into bf16 pieces that add up to it exactly, one
+// for bf16 (8 significant bits), two for half (11), three for float (24), each multiplied in turn.
+// Sums are fp32 (v_mfma_f32_32x32x16_bf16).
+//
+// Both factors lie with the summed axis outermost in memory, so a lane's eight consecutive rows of
+// one column are a column of the tile: tiles are staged row by row in LDS and read through
+// the transposing ds_read_b64_tr_b16 (a group of 16 lanes reads 4 rows x 16 columns and gets 4 rows
+// of one column each).  Those 4 rows are brought to different banks by XORing the 64-byte piece of a
+// row with its row number mod 4.
+//
+// A work-group owns a tile of dW and a range of rows; the parts are summed in their order by a second
+// launch.  Column sums of dY ride along: among the work-groups that share a dY tile, each adds up its
+// share of the row steps.
 #include "gvae_ckpt8.h"
 
 namespace gvae {
@@ -10,85 +24,272 @@ struct WgradArgs {
   const int8_t *codes;
   const uint8_t *scales;
   void *dw, *db;
-  float *part, *part_b;       // (splits, O, I) and (splits, O)
+  float *part, *part_b;       // (splits, O, I) and (splits * tx, O)
   int64_t rows, ldy;
-  int O, I, ld8, nb8, splits;
+  int O, I, ld8, nb8, splits, tx, ty;
   int64_t split_rows;
 };
 
-constexpr int kTile = 64, kDepth = 16;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-template <class T>
-__global__ __launch_bounds__(256) void wgrad8_kernel(WgradArgs a) {
-  __shared__ float sa[kDepth][kTile], sb[kDepth][kTile + 4];
-  const int i0 = blockIdx.x * kTile, o0 = blockIdx.y * kTile, tid = threadIdx.x;
-  const int tx = tid & 15, ty = tid >> 4;
-  const int64_t t0 = (int64_t)blockIdx.z * a.split_rows;
-  const int64_t t1 = t0 + a.split_rows < a.rows ? t0 + a.split_rows : a.rows;
-  float acc[4][4] = {}, bias[4] = {};
-  for (int64_t t = t0; t < t1; t += kDepth) {
-    for (int e = tid; e < kDepth * kTile; e += 256) {
-      const int k = e / kTile, c = e % kTile;
-      const bool row = t + k < t1;
-      sa[k][c] = row && o0 + c < a.O ? (float)((const T *)a.dy)[(t + k) * a.ldy + o0 + c] : 0.0f;
-      float x = 0.0f;
-      if (row && i0 + c < a.I)
-        x = (float)a.codes[(t + k) * a.ld8 + i0 + c] * pow2_field(a.scales[(t + k) * a.nb8 + (i0 + c) / kBlock8]);
-      sb[k][c] = x;
-    }
-    __syncthreads();
+template <class T> struct Pieces;
+template <> struct Pieces<bf16_t> { static constexpr int P = 1; };
+template <> struct Pieces<f16_t> { static constexpr int P = 2; };
+template <> struct Pieces<float> { static constexpr int P = 3; };
+
+// a finite value into P bf16 pieces that add up to it; what is not finite stays whole in the first
+template <int P>
+__device__ __forceinline__ void cut(float x, uint16_t *out) {
+  const uint32_t b = __float_as_uint(x);
+  const bool finite = (b & 0x7f800000u) != 0x7f800000u;
+  out[0] = (uint16_t)((b >> 16) | (x != x ? 0x40u : 0u));
+  float r = finite ? x - __uint_as_float(b & 0xffff0000u) : 0.0f;
 #pragma unroll
-    for (int k = 0; k < kDepth; ++k)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const float av = sa[k][ty * 4 + u];
-        bias[u] += av;
-#pragma unroll
-        for (int v = 0; v < 4; ++v) acc[u][v] = __fmaf_rn(av, sb[k][tx * 4 + v], acc[u][v]);
-      }
-    __syncthreads();
-  }
-  float *p = a.part + (int64_t)blockIdx.z * a.O * a.I;
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int o = o0 + ty * 4 + u;
-    if (o >= a.O) continue;
-#pragma unroll
-    for (int v = 0; v < 4; ++v)
-      if (i0 + tx * 4 + v < a.I) p[(int64_t)o * a.I + i0 + tx * 4 + v] = acc[u][v];
-    if (blockIdx.x == 0 && tx == 0) a.part_b[(int64_t)blockIdx.z * a.O + o] = bias[u];
+  for (int p = 1; p < P; ++p) {
+    const uint32_t c = __float_as_uint(r);
+    out[p] = (uint16_t)(c >> 16);
+    r -= __uint_as_float(c & 0xffff0000u);
   }
 }
 
+// byte offset of column c (a multiple of 8) of row k in a tile of `W` columns
+template <int W>
+__device__ __forceinline__ int tile_at(int k, int c) {
+  return k * (2 * W) + (((c >> 5) ^ (k & 3)) << 6) + 2 * (c & 31);
+}
+
+// FM x FN matrix-core tiles of 32 x 32 per wavefront, WM x WN wavefronts, KT rows per step
+template <class T, int FM, int FN, int WM, int WN, int KT>
+struct Wgrad {
+  static constexpr int P = Pieces<T>::P, V = Piece<T>::V;
+  static constexpr int TM = 32 * FM * WM, TN = 32 * FN * WN, NT = 64 * WM * WN;
+  static constexpr int kBytesA = KT * TM * 2, kBytesB = KT * TN * 2;
+  static constexpr int kStage = P * kBytesA + kBytesB;
+  static constexpr int NA = KT * TM / (V * NT), NB = KT * TN / (16 * NT);   // pieces of a thread per step
+  static_assert(NA * V * NT == KT * TM && NB * 16 * NT == KT * TN && NB >= 1, "tile and threads");
+};
+
+template <class T, int FM, int FN, int WM, int WN, int KT>
+__global__ __launch_bounds__(64 * WM * WN, 2) void wgrad8_kernel(WgradArgs a) {
+  using S = Wgrad<T, FM, FN, WM, WN, KT>;
+  constexpr int P = S::P, V = S::V, TM = S::TM, TN = S::TN, NT = S::NT;
+  extern __shared__ __align__(16) char lds[];
+  // consecutive work-groups go to the eight XCDs in turn: each XCD takes a run of the numbering below,
+  // in which the tiles of one row range are neighbours and share that range in the XCD's L2
+  const int total = gridDim.x, xcd = blockIdx.x & 7, q8 = total >> 3, r8 = total & 7;
+  const int id = xcd * q8 + (xcd < r8 ? xcd : r8) + ((int)blockIdx.x >> 3);
+  const int tiles = a.tx * a.ty, split = id / tiles, tile = id - split * tiles;
+  const int ix = tile % a.tx, i0 = ix * TN, o0 = (tile / a.tx) * TM;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
+  const int64_t t0 = (int64_t)split * a.split_rows;
+  const int64_t t1 = t0 + a.split_rows < a.rows ? t0 + a.split_rows : a.rows;
+  const int steps = (int)((t1 - t0 + KT - 1) / KT);
+
+  typename Piece<T>::raw ra[S::NA];
+  uint4 rb[S::NB];
+  uint32_t rs[S::NB];
+  float bias[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) bias[v] = 0.0f;
+
+  // a thread's piece: always the same columns, rows k = first + j * step
+  constexpr int CA = TM / V, CB = TN / 16;
+  const int ca = (tid % CA) * V, ka = tid / CA, cb = (tid % CB) * 16, kb = tid / CB;
+  const int nva = a.O - (o0 + ca) < V ? a.O - (o0 + ca) : V;
+  const bool onb = i0 + cb < a.ld8;
+  const T *dy = (const T *)a.dy + o0 + ca;
+  const int8_t *codes = a.codes + i0 + cb;
+  const uint8_t *scales = a.scales + (i0 + cb) / kBlock8;
+
+  auto load = [&](int step) {
+    const int64_t t = t0 + (int64_t)step * KT;
+#pragma unroll
+    for (int j = 0; j < S::NA; ++j) {
+      const int64_t row = t + ka + j * (NT / CA);
+      ra[j] = typename Piece<T>::raw{};
+      if (row < t1 && nva > 0) ra[j] = load_piece<T>(dy + row * a.ldy, nva);
+    }
+#pragma unroll
+    for (int j = 0; j < S::NB; ++j) {
+      const int64_t row = t + kb + j * (NT / CB);
+      rb[j] = make_uint4(0, 0, 0, 0);
+      rs[j] = 0;
+      if (row < t1 && onb) {
+        rb[j] = *reinterpret_cast<const uint4 *>(codes + row * a.ld8);
+        rs[j] = scales[row * a.nb8];
+      }
+    }
+  };
+  auto stage = [&](int step, char *buf) {
+#pragma unroll
+    for (int j = 0; j < S::NA; ++j) {
+      const int k = ka + j * (NT / CA);
+      uint16_t out[V][3];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if constexpr (P == 1) out[v][0] = __builtin_bit_cast(uint16_t, (T)ra[j][v]);
+        else cut<P>((float)ra[j][v], out[v]);
+      }
+      if (step % a.tx == ix)
+#pragma unroll
+        for (int v = 0; v < V; ++v) bias[v] += (float)ra[j][v];
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        uint32_t w[V / 2];
+#pragma unroll
+        for (int v = 0; v < V / 2; ++v) w[v] = out[2 * v][p] | ((uint32_t)out[2 * v + 1][p] << 16);
+        char *dst = buf + p * S::kBytesA + tile_at<TM>(k, ca & ~7) + 2 * (ca & 7);
+        if (V == 8) *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[V / 2 - 2], w[V / 2 - 1]);
+        else *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
+      }
+    }
+    char *bb = buf + P * S::kBytesA;
+#pragma unroll
+    for (int j = 0; j < S::NB; ++j) {
+      const int k = kb + j * (NT / CB);
+      const float p = pow2_field(rs[j]);
+      const uint32_t src[4] = {rb[j].x, rb[j].y, rb[j].z, rb[j].w};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t w[4];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          // (exact in bf16: the upper half of the float is all of it)
+          const uint32_t c = src[2 * h + (v >> 1)] >> (16 * (v & 1));
+          const uint32_t lo = __float_as_uint((float)(int8_t)c * p), hi = __float_as_uint((float)(int8_t)(c >> 8) * p);
+          w[v] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+        }
+        *reinterpret_cast<uint4 *>(bb + tile_at<TN>(k, cb + 8 * h)) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  };
+
+  f32x16 acc[FM][FN];
+#pragma unroll
+  for (int m = 0; m < FM; ++m)
+#pragma unroll
+    for (int n = 0; n < FN; ++n)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) acc[m][n][q] = 0.0f;
+
+  // transposed read: this lane's row within a group of four, its 16 columns and 4 of them
+  const int kr = 8 * (lane >> 5) + ((lane >> 2) & 3), sw = (lane >> 2) & 3;
+  const int off = 2 * (16 * ((lane >> 4) & 1) + 4 * (lane & 3));
+  typedef __attribute__((address_space(3))) s16x4 *lds_ptr;
+  auto frag = [&](char *base, int rowbytes, int k0, int blk) -> bf16x8 {
+    char *p = base + (k0 + kr) * rowbytes + ((blk ^ sw) << 6) + off;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 4 * rowbytes));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  auto compute = [&](char *buf) {
+#pragma unroll
+    for (int k0 = 0; k0 < KT; k0 += 16) {
+      bf16x8 bf[FN];
+#pragma unroll
+      for (int n = 0; n < FN; ++n) bf[n] = frag(buf + P * S::kBytesA, 2 * TN, k0, wn * FN + n);
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int m = 0; m < FM; ++m) {
+          const bf16x8 af = frag(buf + p * S::kBytesA, 2 * TM, k0, wm * FM + m);
+#pragma unroll
+          for (int n = 0; n < FN; ++n)
+            acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af, bf[n], acc[m][n], 0, 0, 0);
+        }
+    }
+  };
+
+  load(0);
+  stage(0, lds);
+  __syncthreads();
+  for (int s = 0; s < steps; ++s) {
+    char *cur = lds + (s & 1) * S::kStage, *nxt = lds + ((s & 1) ^ 1) * S::kStage;
+    const bool more = s + 1 < steps;
+    if (more) load(s + 1);
+    compute(cur);
+    if (more) stage(s + 1, nxt);
+    __syncthreads();
+  }
+
+  const bool whole = a.splits == 1;
+  float *part = a.part + (int64_t)split * a.O * a.I;
+#pragma unroll
+  for (int m = 0; m < FM; ++m)
+#pragma unroll
+    for (int n = 0; n < FN; ++n) {
+      const int i = i0 + (wn * FN + n) * 32 + (lane & 31);
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        const int o = o0 + (wm * FM + m) * 32 + (q & 3) + 8 * (q >> 2) + 4 * (lane >> 5);
+        if (o < a.O && i < a.I) {
+          if (whole) ((T *)a.dw)[(int64_t)o * a.I + i] = (T)acc[m][n][q];
+          else part[(int64_t)o * a.I + i] = acc[m][n][q];
+        }
+      }
+    }
+  // column sums over this work-group's share of the steps: its row lanes in order
+  if (!a.db) return;
+  float *sb = reinterpret_cast<float *>(lds);   // (all reads of the tiles are behind the last barrier)
+#pragma unroll
+  for (int v = 0; v < V; ++v) sb[ka * TM + ca + v] = bias[v];
+  __syncthreads();
+  for (int c = tid; c < TM; c += NT) {
+    float s = 0.0f;
+    for (int k = 0; k < NT / CA; ++k) s += sb[k * TM + c];
+    if (o0 + c < a.O) a.part_b[((int64_t)split * a.tx + ix) * a.O + o0 + c] = s;
+  }
+}
+
+// The parts of dW (if there is more than one) and of db, in their order
 template <class T>
 __global__ __launch_bounds__(256) void wgrad8_sum_kernel(WgradArgs a) {
-  const int64_t n = (int64_t)a.O * a.I, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t n = a.splits > 1 ? (int64_t)a.O * a.I : 0, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (e < n) {
     float s = 0.0f;
     for (int k = 0; k < a.splits; ++k) s += a.part[k * n + e];
     ((T *)a.dw)[e] = (T)s;
   } else if (e < n + a.O && a.db) {
     float s = 0.0f;
-    for (int k = 0; k < a.splits; ++k) s += a.part_b[(int64_t)k * a.O + (e - n)];
+    for (int k = 0; k < a.splits * a.tx; ++k) s += a.part_b[(int64_t)k * a.O + (e - n)];
     ((T *)a.db)[e - n] = (T)s;
   }
 }
 
 struct WgradShape {
-  int tx, ty, splits;
+  int tm, tn, tx, ty, splits;
   int64_t split_rows;
 };
+// A tile of 256 x 256 if both sides fill at least one and there is work for every CU, else 128 x 128;
+// rows are split until there is a work-group for each CU (two of the small ones), no
+// range shorter than 128 rows.
 static WgradShape wgrad_shape(int64_t rows, int O, int I) {
   WgradShape s;
-  s.tx = ceil_div(I, kTile);
-  s.ty = ceil_div(O, kTile);
-  const int64_t tiles = (int64_t)s.tx * s.ty;
-  int64_t want = tiles >= 1024 ? 1 : 1024 / tiles;
+  const bool big = O >= 256 && I >= 256 && rows >= 1024;
+  s.tm = s.tn = big ? 256 : 128;
+  s.tx = ceil_div(I, s.tn);
+  s.ty = ceil_div(O, s.tm);
+  const int64_t tiles = (int64_t)s.tx * s.ty, fill = big ? 256 : 512;
+  int64_t want = tiles >= fill ? 1 : fill / tiles;
   const int64_t most = (rows + 127) / 128;
   if (want > most) want = most;
-  s.split_rows = ((rows + want - 1) / want + kDepth - 1) / kDepth * kDepth;
+  s.split_rows = ((rows + want - 1) / want + 63) / 64 * 64;
   s.splits = (int)((rows + s.split_rows - 1) / s.split_rows);
   return s;
+}
+
+template <class T, int FM, int FN, int WM, int WN, int KT>
+static int wgrad_launch(const WgradArgs &a, hipStream_t s) {
+  using S = Wgrad<T, FM, FN, WM, WN, KT>;
+  const size_t lds = 2 * S::kStage;
+  static_assert(2 * S::kStage <= (int)kMaxDynLds && S::NT * S::V * 4 <= 2 * S::kStage, "LDS");
+  auto kernel = wgrad8_kernel<T, FM, FN, WM, WN, KT>;
+  hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  GVAE_REQUIRE(e == hipSuccess, GVAE_ELAUNCH, "linear_wgrad8: %s", hipGetErrorString(e));
+  hipLaunchKernelGGL(kernel, dim3((unsigned)((int64_t)a.tx * a.ty * a.splits)), dim3(S::NT), lds, s, a);
+  return GVAE_OK;
 }
 
 }  // namespace gvae
@@ -99,7 +300,8 @@ extern "C" {
 
 int64_t gvae_linear_wgrad8_ws_bytes(int64_t rows, int O, int I) {
   if (rows <= 0 || O <= 0 || I <= 0) return 0;
-  return 4 * (int64_t)wgrad_shape(rows, O, I).splits * ((int64_t)O * I + O);
+  const WgradShape s = wgrad_shape(rows, O, I);
+  return 4 * (int64_t)s.splits * ((s.splits > 1 ? (int64_t)O * I : 0) + (int64_t)s.tx * O);
 }
 
 int gvae_linear_wgrad8(const void *d_dy, int dtype, int64_t row_stride, const int8_t *d_codes, const uint8_t *d_scales,
@@ -109,21 +311,26 @@ int gvae_linear_wgrad8(const void *d_dy, int dtype, int64_t row_stride, const in
   GVAE_REQUIRE(rows > 0 && O > 0 && I > 0 && row_stride >= O, GVAE_EINVAL,
                "linear_wgrad8: bad sizes (rows=%lld out=%d in=%d stride=%lld)", (long long)rows, O, I,
                (long long)row_stride);
-  GVAE_REQUIRE((int64_t)O * I < (1LL << 38) && O <= (1 << 20) && I <= (1 << 20), GVAE_ELIMIT,
-               "linear_wgrad8: %d x %d weights", O, I);
   const WgradShape sh = wgrad_shape(rows, O, I);
+  GVAE_REQUIRE(O <= (1 << 20) && I <= (1 << 20) && (int64_t)sh.tx * sh.ty * sh.splits < (1LL << 31) &&
+                   sh.split_rows < (1LL << 36) && (int64_t)O * I < (1LL << 38), GVAE_ELIMIT,
+               "linear_wgrad8: %lld rows, %d x %d weights", (long long)rows, O, I);
   WgradArgs a;
   a.dy = d_dy; a.codes = d_codes; a.scales = d_scales; a.dw = d_dw; a.db = d_db;
   a.rows = rows; a.ldy = row_stride; a.O = O; a.I = I; a.ld8 = ckpt8_ld(I); a.nb8 = ckpt8_blocks(I);
-  a.splits = sh.splits; a.split_rows = sh.split_rows;
-  a.part = (float *)d_ws;
-  a.part_b = a.part + (int64_t)sh.splits * O * I;
+  a.splits = sh.splits; a.split_rows = sh.split_rows; a.tx = sh.tx; a.ty = sh.ty;
+  a.part_b = (float *)d_ws;
+  a.part = a.part_b + (int64_t)sh.splits * sh.tx * O;
   hipStream_t s = (hipStream_t)stream;
-  const int64_t n = (int64_t)O * I + O;
+  int rc = GVAE_OK;
   GVAE_DTYPE_SWITCH(dtype, T, {
-    hipLaunchKernelGGL((wgrad8_kernel<T>), dim3(sh.tx, sh.ty, sh.splits), dim3(256), 0, s, a);
-    hipLaunchKernelGGL((wgrad8_sum_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a);
+    constexpr int kDeep = Pieces<T>::P == 1 ? 64 : 32;
+    rc = sh.tm == 256 ? wgrad_launch<T, 4, 2, 2, 4, kDeep>(a, s) : wgrad_launch<T, 2, 2, 2, 2, kDeep>(a, s);
+    const int64_t n = (sh.splits > 1 ? (int64_t)O * I : 0) + (d_db ? O : 0);
+    if (rc == GVAE_OK && n > 0)
+      hipLaunchKernelGGL((wgrad8_sum_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a);
   });
+  if (rc) return rc;
   return check_launch("linear_wgrad8");
 }
 
