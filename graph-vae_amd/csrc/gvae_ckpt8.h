@@ -40,6 +40,17 @@ __device__ __forceinline__ typename Piece<T>::raw load_piece(const T *p, int nv)
   for (int v = 0; v < V; ++v) r[v] = v < nv ? p[v] : (T)0.0f;
   return r;
 }
+// A piece held over several passes of a kernel: between two passes the compiler must not keep its
+// values converted to float (twice the registers for 16-bit types) instead of converting again.
+template <class T>
+__device__ __forceinline__ void keep_raw(typename Piece<T>::raw &r) {
+  if (sizeof(T) == 4) return;
+  typedef uint32_t words __attribute__((ext_vector_type(4)));
+  words w = __builtin_bit_cast(words, r);
+  asm volatile("" : "+v"(w));
+  r = __builtin_bit_cast(typename Piece<T>::raw, w);
+}
+
 template <class T>
 __device__ __forceinline__ void store_piece(T *p, const float *f, int nv) {
   constexpr int V = Piece<T>::V;

@@ -1,0 +1,314 @@
+// Group norm over each graph's live rows, channels last, with an activation: what the forward
+// (norm_fwd.hip) and the backward (norm_bwd.hip) share.
+//
+//   graph b, group q of C/G channels, live rows i < rows[b], m = rows[b] * C/G:
+//   mean = sum x / m,  var = sum (x - mean)^2 / m,  r = 1 / sqrt(var + eps)
+//   h = (x - mean) r,  z = h w_c + b_c,  y = act(z);  rows behind the last live one: y = 0
+//   dz = dy act'(z);  dw_c = sum dz h,  db_c = sum dz  (over graphs and rows)
+//   dx = r (w dz - (A1 + h A2)),  A1 = sum_group w dz / m,  A2 = sum_group w dz h / m
+//
+// z is formed by a subtraction, two products and a sum, each rounded (no contraction), in the
+// forward and in the backward alike: the branch of a ReLU is the same in both.
+//
+// All of it is bound by memory.  Two forms each:
+//   resident   a work-group holds a graph's live rows of a run of groups (a slab) in registers: one
+//              read, the sums through LDS, one write.  The slab is as narrow as fills the chip, but
+//              no row segment is under 64 bytes.
+//   split      a group too long for that is summed in chunks of rows by as many work-groups, joined
+//              by one wavefront per group, and read again to be written.
+#pragma once
+#include "gvae_ckpt8.h"
+
+#include <cmath>
+
+namespace gvae {
+
+constexpr int kThreads = 256;
+constexpr int kBatch = 8;     // rows of a thread in registers at a time (split form)
+
+struct NormArgs {
+  const void *x;              // input, or null if the codes are given (backward)
+  const int8_t *codes;
+  const uint8_t *scales;
+  const void *dy;
+  void *out;                  // y or dx, contiguous
+  const float *w, *b;
+  float *mean, *rstd;         // (B, G)
+  const int32_t *rows;
+  int8_t *x8, *y8;
+  uint8_t *x8s, *y8s;
+  float *part1, *part2;       // split: (B * chunks, C), mean and M2 or the two sums of the backward;
+                              // resident backward: (graph lanes, C), the two sums
+  float *A;                   // (B, G, 2)
+  int64_t xb, xr, dyb, dyr;   // strides of x and dy in elements
+  float eps;
+  int act;
+  int B, N, C, G, cpg;
+  int lanes;                  // pieces per row (split: in one column tile, resident: in a slab)
+  int rp;                     // rows side by side in a work-group
+  int chunk_rows, chunks;     // split
+  int slab, nslab;            // resident: channels of a slab
+  int graph_step;             // resident backward: graphs walked in steps of this
+  int join;                   // resident: lanes (a power of two) that add up one group
+  int ld8, nb8;
+};
+
+__device__ __forceinline__ int live_rows(const NormArgs &a, int b) {
+  if (!a.rows) return a.N;
+  const int r = a.rows[b];
+  return r < 0 ? 0 : (r > a.N ? a.N : r);
+}
+
+// 1 / (1 + exp(-z)) from the hardware's exp2 and reciprocal (one unit in the last place each): the
+// argument's rounding makes it |z| u relative, under the rounding of z that it is computed from.
+__device__ __forceinline__ float sigmoid_fast(float z) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
+}
+// Phi(z) = (1 + erf(z / sqrt 2)) / 2 and *e = exp(-z^2 / 2), by formula 7.1.26 of Abramowitz and
+// Stegun (Hastings): 1 - erf(x) = (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 + p x), |error| <= 1.5e-7
+__device__ __forceinline__ float normal_cdf(float z, float *e) {
+  const float x = fabsf(z) * 0.70710678118654752f;
+  const float t = __builtin_amdgcn_rcpf(__fmaf_rn(0.3275911f, x, 1.0f));
+  float p = __fmaf_rn(1.061405429f, t, -1.453152027f);
+  p = __fmaf_rn(p, t, 1.421413741f);
+  p = __fmaf_rn(p, t, -0.284496736f);
+  p = __fmaf_rn(p, t, 0.254829592f);
+  *e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
+  const float tail = 0.5f * p * t * *e;                  // 1 - Phi(|z|)
+  return z < 0.0f ? tail : 1.0f - tail;
+}
+template <int ACT>
+__device__ __forceinline__ float act_value(float z) {
+  if (ACT == GVAE_ACT_RELU) return z < 0.0f ? 0.0f : z;   // (keeps a NaN)
+  if (ACT == GVAE_ACT_SILU) return z * sigmoid_fast(z);
+  if (ACT == GVAE_ACT_GELU) {
+    float e;
+    return z * normal_cdf(z, &e);
+  }
+  return z;
+}
+template <int ACT>
+__device__ __forceinline__ float act_slope(float z) {
+  if (ACT == GVAE_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+  if (ACT == GVAE_ACT_SILU) {
+    const float s = sigmoid_fast(z);
+    return s * __fmaf_rn(z, 1.0f - s, 1.0f);
+  }
+  if (ACT == GVAE_ACT_GELU) {
+    float e;
+    const float c = normal_cdf(z, &e);
+    return __fmaf_rn(z * 0.39894228040143268f, e, c);
+  }
+  return 1.0f;
+}
+// the same for a piece, with the activation chosen at run time (uniform over the launch)
+template <int V>
+__device__ __forceinline__ void act_values(int act, float *z) {
+  switch (act) {
+    case GVAE_ACT_RELU:
+#pragma unroll
+      for (int v = 0; v < V; ++v) z[v] = act_value<GVAE_ACT_RELU>(z[v]);
+      break;
+    case GVAE_ACT_SILU:
+#pragma unroll
+      for (int v = 0; v < V; ++v) z[v] = act_value<GVAE_ACT_SILU>(z[v]);
+      break;
+    case GVAE_ACT_GELU:
+#pragma unroll
+      for (int v = 0; v < V; ++v) z[v] = act_value<GVAE_ACT_GELU>(z[v]);
+      break;
+    default: break;
+  }
+}
+template <int V>
+__device__ __forceinline__ void act_slopes(int act, float *z) {
+  switch (act) {
+    case GVAE_ACT_RELU:
+#pragma unroll
+      for (int v = 0; v < V; ++v) z[v] = act_slope<GVAE_ACT_RELU>(z[v]);
+      break;
+    case GVAE_ACT_SILU:
+#pragma unroll
+      for (int v = 0; v < V; ++v) z[v] = act_slope<GVAE_ACT_SILU>(z[v]);
+      break;
+    case GVAE_ACT_GELU:
+#pragma unroll
+      for (int v = 0; v < V; ++v) z[v] = act_slope<GVAE_ACT_GELU>(z[v]);
+      break;
+    default:
+#pragma unroll
+      for (int v = 0; v < V; ++v) z[v] = 1.0f;
+      break;
+  }
+}
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+
+// the same over a work-group of NT threads (every thread gets the sum)
+template <int NT>
+__device__ __forceinline__ float group_sum(float v, float *sh) {
+  v = wave_sum(v);
+  if (NT == 64) return v;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0.0f;
+#pragma unroll
+  for (int k = 0; k < NT / 64; ++k) v += sh[k];
+  return v;
+}
+
+// V values of x at row i of graph b, from the tensor or from the checkpoint
+template <class T, bool KEPT>
+__device__ __forceinline__ void load_x(const NormArgs &a, int b, int i, int c0, int nv, float *f) {
+  constexpr int V = Piece<T>::V;
+  if (KEPT) {
+    const int64_t row = (int64_t)b * a.N + i;
+    decode8<V>(load_codes<V>(a.codes + row * a.ld8 + c0), pow2_field(a.scales[row * a.nb8 + c0 / kBlock8]), f);
+  } else {
+    const typename Piece<T>::raw r = load_piece<T>((const T *)a.x + b * a.xb + (int64_t)i * a.xr + c0, nv);
+#pragma unroll
+    for (int v = 0; v < V; ++v) f[v] = (float)r[v];
+  }
+}
+
+// what the channels of a piece are scaled and shifted by
+template <int V>
+struct Scale {
+  float mean[V], rstd[V], w[V], b[V];
+  __device__ Scale(const NormArgs &a, int g, int c0, int nv) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const bool in = v < nv;
+      const int c = in ? c0 + v : 0;
+      const int64_t q = (int64_t)g * a.G + c / a.cpg;
+      mean[v] = in ? a.mean[q] : 0.0f;
+      rstd[v] = in ? a.rstd[q] : 0.0f;
+      w[v] = in && a.w ? a.w[c] : (in ? 1.0f : 0.0f);
+      b[v] = in && a.b ? a.b[c] : 0.0f;
+    }
+  }
+};
+
+// ---- split form: where a thread of a chunk work-group stands
+template <int V>
+struct Place {
+  int b, chunk, c0, nv, r, row_end;   // first channel, channels of the piece, first row lane
+  bool on;
+  __device__ Place(const NormArgs &a, bool live_only) {
+    b = blockIdx.x / a.chunks;
+    chunk = blockIdx.x - b * a.chunks;
+    const int col = threadIdx.x % a.lanes;
+    r = threadIdx.x / a.lanes;
+    c0 = (blockIdx.y * a.lanes + col) * V;
+    nv = a.C - c0 < V ? a.C - c0 : V;
+    on = r < a.rp;
+    const int stop = live_only ? live_rows(a, b) : a.N;
+    row_end = (chunk + 1) * a.chunk_rows < stop ? (chunk + 1) * a.chunk_rows : stop;
+  }
+};
+
+// ---- resident form: sums over the groups of a slab.  Every thread has left E entries of its piece in
+// LDS (thread order, which is row-major: rp rows of row_entries); a group is ge neighbouring entries of
+// each row.  `join` lanes add up a group, in a fixed order.
+template <int NS, int LEN>
+__device__ __forceinline__ void join_groups(const float (*ent)[LEN], int row_entries, int ge, int ng, int rp, int join,
+                                            int threads, float (*out)[LEN]) {
+  const int lane = threadIdx.x & (join - 1);
+  const int dr = join / ge, dq = join - dr * ge;
+  for (int g = threadIdx.x / join; g < ng; g += threads / join) {
+    float s[NS];
+#pragma unroll
+    for (int k = 0; k < NS; ++k) s[k] = 0.0f;
+    int r = lane / ge, q = lane - r * ge;
+    while (r < rp) {
+      const int e = r * row_entries + g * ge + q;
+#pragma unroll
+      for (int k = 0; k < NS; ++k) s[k] += ent[k][e];
+      r += dr;
+      q += dq;
+      if (q >= ge) { q -= ge; ++r; }
+    }
+    for (int off = join >> 1; off > 0; off >>= 1)
+#pragma unroll
+      for (int k = 0; k < NS; ++k) s[k] += __shfl_xor(s[k], off, 64);
+    if (lane == 0)
+#pragma unroll
+      for (int k = 0; k < NS; ++k) out[k][g] = s[k];
+  }
+}
+
+// Column tiles, row lanes and row chunks of the split form: a row is cut into tiles of at most 256
+// pieces; the rows of a graph are cut so that about 2048 work-groups (eight per CU) share the
+// batch, each with at least eight rows per row lane.
+struct SplitShape {
+  int lanes, tiles, rp, chunk_rows, chunks;
+};
+inline SplitShape split_shape(int B, int N, int C, int V, bool whole_blocks) {
+  SplitShape s;
+  int pieces = ceil_div(C, V);
+  if (whole_blocks) pieces = ceil_div(C, kBlock8) * (kBlock8 / V);
+  s.lanes = pieces < kThreads ? pieces : kThreads;
+  s.tiles = ceil_div(pieces, s.lanes);
+  s.rp = kThreads / s.lanes;
+  const int64_t have = (int64_t)B * s.tiles;
+  const int want = (int)(have >= 2048 ? 1 : (2048 + have - 1) / have);
+  int rows = ceil_div(N, want), least = kBatch * s.rp;
+  if (rows < least) rows = least;
+  s.chunk_rows = ceil_div(rows, s.rp) * s.rp;
+  s.chunks = ceil_div(N, s.chunk_rows);
+  return s;
+}
+
+// Slab of the resident form.  `align`: channels a slab has to start at a multiple of (32 where
+// checkpoints are written, the piece where one is read); `most`: pieces a work-group can hold;
+// `threads`: the widest row of pieces.  false: no slab of whole groups fits, or the batch would leave
+// most of the chip idle that the split form fills.
+struct ResidentShape {
+  int slab, nslab, lanes, pieces;
+};
+inline bool resident_shape(int B, int N, int C, int cpg, int V, int align, int64_t most, int threads,
+                           ResidentShape *s) {
+  int64_t unit = cpg;
+  while (unit % align && unit < C) unit += cpg;
+  if (unit > C) unit = C;
+  auto lanes_of = [&](int64_t slab) { return (int)(((slab + align - 1) / align * align + V - 1) / V); };
+  // as many slabs as make 1024 work-groups, none with a row segment under 64 bytes (4 pieces)
+  const int64_t want = B >= 1024 ? 1 : (1024 + B - 1) / B;
+  int64_t units = ((C + unit - 1) / unit + want - 1) / want;
+  const int64_t least = (4 * V + unit - 1) / unit;
+  if (units < least) units = least;
+  for (;; --units) {
+    int64_t slab = units * unit;
+    if (slab > C) slab = C;
+    const int lanes = lanes_of(slab);
+    if (lanes <= threads && (int64_t)N * lanes <= most) {
+      s->slab = (int)slab; s->lanes = lanes;
+      s->nslab = ceil_div(C, (int)slab);
+      s->pieces = N * lanes;
+      // a few long graphs: the split form's chunks fill the chip, these slabs would not
+      return (int64_t)B * s->nslab >= 128 || s->pieces <= 2048;
+    }
+    if (units <= least || units <= 1) return false;
+  }
+}
+// lanes that add up one of `groups` groups with `threads` threads
+inline int join_lanes(int groups, int threads) {
+  int j = 64;
+  while (j > 1 && (int64_t)j * groups > threads) j >>= 1;
+  return j;
+}
+
+inline int64_t norm_ws_floats(int B, int C, int G) {
+  // the most partial rows any element type and form leads to (split: 2048 work-groups or one per
+  // graph; resident: at most one per graph), and A1, A2
+  return 2 * ((int64_t)2048 + B) * C + 2 * (int64_t)B * G;
+}
+
+int norm_check(const char *who, int dtype, int B, int N, int C, int G, int act, int64_t ld);
+
+}  // namespace gvae

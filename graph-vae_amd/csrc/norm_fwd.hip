@@ -1,0 +1,366 @@
+// Group norm with an activation: forward (gvae_norm.h has the mathematics and the two forms).
+//
+// Split form: what a chunk leaves is one (mean, M2) pair per channel, combined as n, mean, M2 with
+// M2 = M2a + M2b + d^2 na nb / n, so no square of an uncentred value is ever summed.
+#include "gvae_norm.h"
+
+namespace gvae {
+
+// --------------------------------------------------------------------------- resident form
+// One graph and one slab per work-group; K pieces a thread, kept as they were loaded.  Two passes over
+// the registers (mean, then centred squares).  IN: a piece lies inside one group (one entry per
+// thread in LDS), else every channel has its own.
+template <class T, bool IN, int NT, int K>
+__global__ __launch_bounds__(NT) void norm_resident_kernel(NormArgs a) {
+  constexpr int V = Piece<T>::V, E = IN ? 1 : V;
+  __shared__ float ent[1][NT * E], grp[2][NT * E];
+  const int b = blockIdx.x / a.nslab, s0 = (blockIdx.x - b * a.nslab) * a.slab;
+  const int s1 = s0 + a.slab < a.C ? s0 + a.slab : a.C;
+  const int col = threadIdx.x % a.lanes, r0 = threadIdx.x / a.lanes;
+  const int c0 = s0 + col * V, nv = s1 - c0 < V ? s1 - c0 : V;
+  const bool on = r0 < a.rp && nv > 0;
+  const int live = live_rows(a, b), ng = (s1 - s0) / a.cpg, g0 = s0 / a.cpg;
+  const T *x = (const T *)a.x + b * a.xb + c0;
+  typename Piece<T>::raw k[K];
+#pragma unroll
+  for (int u = 0; u < K; ++u) {
+    const int i = r0 + u * a.rp;
+    k[u] = typename Piece<T>::raw{};
+    if (on && i < live) k[u] = load_piece<T>(x + (int64_t)i * a.xr, nv);
+  }
+  // this thread's entry e of group entries starts at the piece's own group
+  const int mine = (threadIdx.x < a.rp * a.lanes) ? (int)threadIdx.x * E : -1;
+  const int ge = IN ? a.cpg / V : a.cpg;
+  const float inv = 1.0f / ((float)(live > 0 ? live : 1) * (float)a.cpg);
+  float mean[E], rstd[E];
+  {
+    float s[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) s[e] = 0.0f;
+#pragma unroll
+    for (int u = 0; u < K; ++u)
+#pragma unroll
+      for (int v = 0; v < V; ++v) s[IN ? 0 : v] += (float)k[u][v];
+    if (mine >= 0)
+#pragma unroll
+      for (int e = 0; e < E; ++e) ent[0][mine + e] = s[e];
+  }
+#pragma unroll
+  for (int u = 0; u < K; ++u) keep_raw<T>(k[u]);
+  __syncthreads();
+  join_groups<1, NT * E>(ent, a.lanes * E, ge, ng, a.rp, a.join, NT, grp);
+  __syncthreads();
+  auto group_of = [&](int e) {
+    const int c = c0 + e < s1 ? c0 + e : s1 - 1;
+    return (c - s0) / a.cpg;
+  };
+#pragma unroll
+  for (int e = 0; e < E; ++e) mean[e] = grp[0][group_of(e)] * inv;
+  {
+    float s[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) s[e] = 0.0f;
+#pragma unroll
+    for (int u = 0; u < K; ++u)
+      if (on && r0 + u * a.rp < live)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float d = v < nv ? (float)k[u][v] - mean[IN ? 0 : v] : 0.0f;
+          s[IN ? 0 : v] = __fmaf_rn(d, d, s[IN ? 0 : v]);
+        }
+    if (mine >= 0)
+#pragma unroll
+      for (int e = 0; e < E; ++e) ent[0][mine + e] = s[e];
+  }
+#pragma unroll
+  for (int u = 0; u < K; ++u) keep_raw<T>(k[u]);
+  __syncthreads();
+  join_groups<1, NT * E>(ent, a.lanes * E, ge, ng, a.rp, a.join, NT, grp + 1);
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < E; ++e) rstd[e] = 1.0f / sqrtf(grp[1][group_of(e)] * inv + a.eps);
+  for (int g = threadIdx.x; g < ng; g += NT) {
+    const int64_t q = (int64_t)b * a.G + g0 + g;
+    a.mean[q] = grp[0][g] * inv;
+    a.rstd[q] = 1.0f / sqrtf(grp[1][g] * inv + a.eps);
+  }
+  if (r0 >= a.rp) return;
+  float w[V], bias[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    w[v] = v < nv ? (a.w ? a.w[c0 + v] : 1.0f) : 0.0f;
+    bias[v] = v < nv && a.b ? a.b[c0 + v] : 0.0f;
+  }
+#pragma unroll
+  for (int u = 0; u < K; ++u) {
+    const int i = r0 + u * a.rp;
+    if (i >= a.N) break;
+    float xf[V], y[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      xf[v] = (float)k[u][v];
+      y[v] = (xf[v] - mean[IN ? 0 : v]) * rstd[IN ? 0 : v] * w[v] + bias[v];
+    }
+    act_values<V>(a.act, y);
+#pragma unroll
+    for (int v = 0; v < V; ++v) y[v] = i < live && v < nv ? (float)(T)y[v] : 0.0f;
+    const int64_t row = (int64_t)b * a.N + i;
+    if (nv > 0) store_piece<T>((T *)a.out + row * a.C + c0, y, nv);
+    // (the lanes of a block share a row: with checkpoints kept, `lanes` is a whole number of blocks)
+    const int nc = a.ld8 - c0;
+    const bool first = c0 % kBlock8 == 0 && nv > 0;
+    if (a.x8) emit8<V>(xf, a.x8 + row * a.ld8 + c0, nc, a.x8s + row * a.nb8 + c0 / kBlock8, first);
+    if (a.y8) emit8<V>(y, a.y8 + row * a.ld8 + c0, nc, a.y8s + row * a.nb8 + c0 / kBlock8, first);
+  }
+}
+
+// --------------------------------------------------------------------------- split form
+// (n, mean, M2) of every channel over a chunk's live rows
+template <class T>
+__global__ __launch_bounds__(kThreads) void norm_stats_kernel(NormArgs a) {
+  constexpr int V = Piece<T>::V;
+  __shared__ float sh_mean[kThreads * V], sh_m2[kThreads * V];
+  __shared__ int sh_n[kThreads];
+  const Place<V> p(a, true);
+  const int row0 = p.chunk * a.chunk_rows;
+  float mean[V], m2[V];
+  int n = 0;
+#pragma unroll
+  for (int v = 0; v < V; ++v) mean[v] = m2[v] = 0.0f;
+  if (p.on && p.nv > 0) {
+    const T *x = (const T *)a.x + p.b * a.xb + p.c0;
+    for (int i = row0 + p.r; i < p.row_end; i += kBatch * a.rp) {
+      typename Piece<T>::raw k[kBatch];
+      int cnt = 0;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+        if (i + u * a.rp < p.row_end) {
+          k[u] = load_piece<T>(x + (int64_t)(i + u * a.rp) * a.xr, p.nv);
+          ++cnt;
+        }
+      const float inv = 1.0f / (float)cnt;
+      const float share = (float)cnt / (float)(n + cnt), cross = (float)n * share;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float s = 0.0f;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) if (u < cnt) s += (float)k[u][v];
+        const float mb = s * inv;
+        float q = 0.0f;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) if (u < cnt) {
+          const float d = (float)k[u][v] - mb;
+          q = __fmaf_rn(d, d, q);
+        }
+        const float d = mb - mean[v];
+        mean[v] = __fmaf_rn(d, share, mean[v]);
+        m2[v] += __fmaf_rn(d * d, cross, q);
+      }
+      n += cnt;
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    sh_mean[threadIdx.x * V + v] = mean[v];
+    sh_m2[threadIdx.x * V + v] = m2[v];
+  }
+  sh_n[threadIdx.x] = n;
+  __syncthreads();
+  // the row lanes of a channel, in their order
+  const int wide = a.lanes * V;
+  for (int c = threadIdx.x; c < wide; c += kThreads) {
+    const int gc = blockIdx.y * wide + c;
+    if (gc >= a.C) continue;
+    const int col = c / V;
+    float tot = 0.0f, s = 0.0f;
+    for (int r = 0; r < a.rp; ++r) {
+      const float nr = (float)sh_n[r * a.lanes + col];
+      tot += nr;
+      s = __fmaf_rn(nr, sh_mean[r * wide + c], s);
+    }
+    const float mu = tot > 0.0f ? s / tot : 0.0f;
+    float q = 0.0f;
+    for (int r = 0; r < a.rp; ++r) {
+      const float d = sh_mean[r * wide + c] - mu;
+      q += sh_m2[r * wide + c] + (float)sh_n[r * a.lanes + col] * d * d;
+    }
+    const int64_t o = (int64_t)blockIdx.x * a.C + gc;
+    a.part1[o] = mu;
+    a.part2[o] = q;
+  }
+}
+
+// mean and 1/sqrt(var + eps) of a group from its chunks' channels, a work-group per group
+template <int NT>
+__global__ __launch_bounds__(NT) void norm_stats_join_kernel(NormArgs a) {
+  __shared__ float sh[NT / 64];
+  const int64_t q = blockIdx.x;
+  const int b = (int)(q / a.G), g = (int)(q - (int64_t)b * a.G);
+  const int live = live_rows(a, b), total = a.chunks * a.cpg;
+  auto rows_of = [&](int k) {
+    const int n = live - k * a.chunk_rows;
+    return (float)(n < 0 ? 0 : (n > a.chunk_rows ? a.chunk_rows : n));
+  };
+  const int64_t base = (int64_t)b * a.chunks * a.C + g * a.cpg;
+  float s = 0.0f;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < total; e += NT) {
+    const int k = e / a.cpg, c = e - k * a.cpg;
+    s = __fmaf_rn(rows_of(k), a.part1[base + (int64_t)k * a.C + c], s);
+  }
+  s = group_sum<NT>(s, sh);
+  const float m = (float)live * (float)a.cpg;
+  const float mu = live > 0 ? s / m : 0.0f;
+  float v = 0.0f;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < total; e += NT) {
+    const int k = e / a.cpg, c = e - k * a.cpg;
+    const float d = a.part1[base + (int64_t)k * a.C + c] - mu;
+    v += __fmaf_rn(rows_of(k) * d, d, a.part2[base + (int64_t)k * a.C + c]);
+  }
+  v = group_sum<NT>(v, sh);
+  if (threadIdx.x == 0) {
+    a.mean[q] = mu;
+    a.rstd[q] = 1.0f / sqrtf((live > 0 ? v / m : 0.0f) + a.eps);
+  }
+}
+
+template <class T, int ACT>
+__global__ __launch_bounds__(kThreads) void norm_apply_kernel(NormArgs a) {
+  constexpr int V = Piece<T>::V;
+  const Place<V> p(a, false);
+  if (!p.on) return;
+  const int live = live_rows(a, p.b);
+  const Scale<V> k(a, p.b, p.c0, p.nv);
+  const T *x = (const T *)a.x + p.b * a.xb + p.c0;
+  for (int i = p.chunk * a.chunk_rows + p.r; i < p.row_end; i += a.rp) {
+    float xf[V], y[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) xf[v] = y[v] = 0.0f;
+    if (i < live && p.nv > 0) {
+      const typename Piece<T>::raw r = load_piece<T>(x + (int64_t)i * a.xr, p.nv);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (v < p.nv) {
+          xf[v] = (float)r[v];
+          y[v] = (float)(T)act_value<ACT>((xf[v] - k.mean[v]) * k.rstd[v] * k.w[v] + k.b[v]);
+        }
+      }
+    }
+    const int64_t row = (int64_t)p.b * a.N + i;
+    if (p.nv > 0) store_piece<T>((T *)a.out + row * a.C + p.c0, y, p.nv);
+    // (the lanes of a block share a row: with checkpoints kept, `lanes` is a whole number of blocks)
+    const int nc = a.ld8 - p.c0;
+    const bool first = p.c0 % kBlock8 == 0 && p.nv > 0;
+    if (a.x8) emit8<V>(xf, a.x8 + row * a.ld8 + p.c0, nc, a.x8s + row * a.nb8 + p.c0 / kBlock8, first);
+    if (a.y8) emit8<V>(y, a.y8 + row * a.ld8 + p.c0, nc, a.y8s + row * a.nb8 + p.c0 / kBlock8, first);
+  }
+}
+
+
+template <class T, bool IN>
+static void resident_launch(NormArgs &a, const ResidentShape &rs, hipStream_t s) {
+  const dim3 grid((unsigned)((int64_t)a.B * a.nslab));
+  const int groups = a.slab / a.cpg;
+#define RUN(NT, K)                                                                        \
+  do {                                                                                    \
+    a.rp = NT / a.lanes;                                                                  \
+    a.join = join_lanes(groups, NT);                                                      \
+    if ((int64_t)a.rp * K >= a.N) {                                                       \
+      hipLaunchKernelGGL((norm_resident_kernel<T, IN, NT, K>), grid, dim3(NT), 0, s, a);  \
+      return;                                                                             \
+    }                                                                                     \
+  } while (0)
+  if (a.lanes <= 64) RUN(64, 4);
+  if (a.lanes <= 256) {
+    RUN(256, 2);
+    RUN(256, 4);
+    RUN(256, 8);
+  }
+  RUN(1024, 4);
+  RUN(1024, 8);
+  RUN(1024, 16);
+#undef RUN
+}
+
+// whether NT threads with K pieces each hold N rows of `lanes` pieces, for the largest form
+static bool resident_fits(int N, int lanes) { return lanes <= 1024 && (int64_t)(1024 / lanes) * 16 >= N; }
+
+}  // namespace gvae
+
+using namespace gvae;
+
+extern "C" {
+
+int64_t gvae_group_norm_ws_bytes(int B, int N, int C, int G) {
+  if (B <= 0 || N <= 0 || C <= 0 || G <= 0) return 0;
+  return norm_ws_floats(B, C, G) * 4;
+}
+
+}  // extern "C"
+
+int gvae::norm_check(const char *who, int dtype, int B, int N, int C, int G, int act, int64_t ld) {
+  GVAE_REQUIRE(dtype_known(dtype), GVAE_EINVAL, "%s: unknown element type %d", who, dtype);
+  GVAE_REQUIRE(B > 0 && N > 0 && C > 0 && G > 0 && C % G == 0, GVAE_EINVAL,
+               "%s: bad sizes (graphs=%d rows=%d channels=%d groups=%d)", who, B, N, C, G);
+  GVAE_REQUIRE(act >= GVAE_ACT_NONE && act <= GVAE_ACT_GELU, GVAE_EINVAL, "%s: unknown activation %d", who, act);
+  GVAE_REQUIRE(ld >= C, GVAE_EINVAL, "%s: rows overlap (stride %lld for %d channels)", who, (long long)ld, C);
+  GVAE_REQUIRE((int64_t)B * G < (1LL << 31) && (int64_t)N * (C / G) < (1LL << 31) && C <= 65535 * 32 &&
+                   (int64_t)B + 2048 < (1LL << 31), GVAE_ELIMIT,
+               "%s: too many groups or values per group (graphs=%d rows=%d channels=%d groups=%d)", who, B, N, C, G);
+  return GVAE_OK;
+}
+
+
+extern "C" {
+
+int gvae_group_norm_fwd(const void *d_x, int dtype, int64_t batch_stride, int64_t row_stride, const int32_t *d_rows,
+                        int B, int N, int C, int G, const float *d_weight, const float *d_bias, float eps, int act,
+                        void *d_y, float *d_mean, float *d_rstd, int8_t *d_x8, uint8_t *d_x8_scales, int8_t *d_y8,
+                        uint8_t *d_y8_scales, void *d_ws, void *stream) {
+  GVAE_REQUIRE(d_x && d_y && d_mean && d_rstd && d_ws, GVAE_EINVAL, "group_norm_fwd: null pointer");
+  GVAE_REQUIRE(!d_x8 == !d_x8_scales && !d_y8 == !d_y8_scales, GVAE_EINVAL,
+               "group_norm_fwd: a checkpoint needs both its codes and its scales");
+  GVAE_REQUIRE(eps > 0.0f && std::isfinite(eps), GVAE_EINVAL, "group_norm_fwd: eps must be positive");
+  if (int rc = norm_check("group_norm_fwd", dtype, B, N, C, G, act, row_stride)) return rc;
+  GVAE_REQUIRE(batch_stride >= 0, GVAE_EINVAL, "group_norm_fwd: negative stride");
+  hipStream_t s = (hipStream_t)stream;
+  NormArgs a{};
+  a.x = d_x; a.xb = batch_stride; a.xr = row_stride; a.rows = d_rows;
+  a.w = d_weight; a.b = d_bias; a.eps = eps; a.out = d_y; a.mean = d_mean; a.rstd = d_rstd;
+  a.x8 = d_x8; a.x8s = d_x8_scales; a.y8 = d_y8; a.y8s = d_y8_scales;
+  a.B = B; a.N = N; a.C = C; a.G = G; a.cpg = C / G;
+  a.ld8 = ckpt8_ld(C); a.nb8 = ckpt8_blocks(C);
+  a.act = act;
+  const int V = 16 / dtype_bytes(dtype);
+  const bool keep = d_x8 || d_y8;
+  ResidentShape rs;
+  if (resident_shape(B, N, C, a.cpg, V, keep ? kBlock8 : 1, 16384, 1024, &rs) && resident_fits(N, rs.lanes)) {
+    a.slab = rs.slab; a.nslab = rs.nslab; a.lanes = rs.lanes;
+    GVAE_DTYPE_SWITCH(dtype, T, {
+      if (a.cpg % V == 0) resident_launch<T, true>(a, rs, s);
+      else resident_launch<T, false>(a, rs, s);
+    });
+    return check_launch("group_norm_fwd");
+  }
+  const SplitShape sh = split_shape(B, N, C, V, keep);
+  a.lanes = sh.lanes; a.rp = sh.rp; a.chunk_rows = sh.chunk_rows; a.chunks = sh.chunks;
+  a.part1 = (float *)d_ws;
+  a.part2 = a.part1 + (int64_t)B * sh.chunks * C;
+  const dim3 grid((unsigned)(B * sh.chunks), sh.tiles), joins((unsigned)((int64_t)B * G));
+  GVAE_DTYPE_SWITCH(dtype, T, {
+    hipLaunchKernelGGL((norm_stats_kernel<T>), grid, dim3(kThreads), 0, s, a);
+    if ((int64_t)sh.chunks * a.cpg <= 256) hipLaunchKernelGGL((norm_stats_join_kernel<64>), joins, dim3(64), 0, s, a);
+    else hipLaunchKernelGGL((norm_stats_join_kernel<512>), joins, dim3(512), 0, s, a);
+    switch (act) {
+      case GVAE_ACT_NONE: hipLaunchKernelGGL((norm_apply_kernel<T, GVAE_ACT_NONE>), grid, dim3(kThreads), 0, s, a); break;
+      case GVAE_ACT_RELU: hipLaunchKernelGGL((norm_apply_kernel<T, GVAE_ACT_RELU>), grid, dim3(kThreads), 0, s, a); break;
+      case GVAE_ACT_SILU: hipLaunchKernelGGL((norm_apply_kernel<T, GVAE_ACT_SILU>), grid, dim3(kThreads), 0, s, a); break;
+      default: hipLaunchKernelGGL((norm_apply_kernel<T, GVAE_ACT_GELU>), grid, dim3(kThreads), 0, s, a); break;
+    }
+  });
+  return check_launch("group_norm_fwd");
+}
+
+}  // extern "C"
+
