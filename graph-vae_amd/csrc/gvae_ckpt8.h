@@ -19,6 +19,13 @@ constexpr int kBlock8 = 32;
 inline int ckpt8_ld(int C) { return (C + 15) / 16 * 16; }
 inline int ckpt8_blocks(int C) { return (C + kBlock8 - 1) / kBlock8; }
 
+// Consecutive work-groups are handed to the eight XCDs in turn.  This numbers them so that each XCD takes a
+// run of neighbours, which then share what they read (and lines that they write parts of) in its L2.
+__device__ __forceinline__ int xcd_run(unsigned id, unsigned total) {
+  const unsigned xcd = id & 7, q = total >> 3, r = total & 7;
+  return (int)(xcd * q + (xcd < r ? xcd : r) + (id >> 3));
+}
+
 typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
 

@@ -24,7 +24,8 @@
 namespace gvae {
 
 constexpr int kThreads = 256;
-constexpr int kBatch = 8;     // rows of a thread in registers at a time (split form)
+constexpr int kBatch = 8;     // rows of a thread in registers at a time (statistics of the split form)
+constexpr int kLeast = 4;     // rows of a thread in a chunk, at least
 
 struct NormArgs {
   const void *x;              // input, or null if the codes are given (backward)
@@ -162,20 +163,6 @@ __device__ __forceinline__ float group_sum(float v, float *sh) {
   return v;
 }
 
-// V values of x at row i of graph b, from the tensor or from the checkpoint
-template <class T, bool KEPT>
-__device__ __forceinline__ void load_x(const NormArgs &a, int b, int i, int c0, int nv, float *f) {
-  constexpr int V = Piece<T>::V;
-  if (KEPT) {
-    const int64_t row = (int64_t)b * a.N + i;
-    decode8<V>(load_codes<V>(a.codes + row * a.ld8 + c0), pow2_field(a.scales[row * a.nb8 + c0 / kBlock8]), f);
-  } else {
-    const typename Piece<T>::raw r = load_piece<T>((const T *)a.x + b * a.xb + (int64_t)i * a.xr + c0, nv);
-#pragma unroll
-    for (int v = 0; v < V; ++v) f[v] = (float)r[v];
-  }
-}
-
 // what the channels of a piece are scaled and shifted by
 template <int V>
 struct Scale {
@@ -199,9 +186,10 @@ template <int V>
 struct Place {
   int b, chunk, c0, nv, r, row_end;   // first channel, channels of the piece, first row lane
   bool on;
-  __device__ Place(const NormArgs &a, bool live_only) {
-    b = blockIdx.x / a.chunks;
-    chunk = blockIdx.x - b * a.chunks;
+  __device__ Place(const NormArgs &a, bool live_only, bool backwards) {
+    const int id = backwards ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x;
+    b = id / a.chunks;
+    chunk = id - b * a.chunks;
     const int col = threadIdx.x % a.lanes;
     r = threadIdx.x / a.lanes;
     c0 = (blockIdx.y * a.lanes + col) * V;
@@ -215,9 +203,31 @@ struct Place {
 // ---- resident form: sums over the groups of a slab.  Every thread has left E entries of its piece in
 // LDS (thread order, which is row-major: rp rows of row_entries); a group is ge neighbouring entries of
 // each row.  `join` lanes add up a group, in a fixed order.
-template <int NS, int LEN>
-__device__ __forceinline__ void join_groups(const float (*ent)[LEN], int row_entries, int ge, int ng, int rp, int join,
-                                            int threads, float (*out)[LEN]) {
+// Sums over the row lanes of a work-group: NS tables of rp rows of `wide` columns in LDS, the sum of a
+// column by as many lanes (a power of two, at most 64) as there are threads for, in a fixed order;
+// done(column, sums) once per column.
+template <int NS, int NT, int LEN, class F>
+__device__ __forceinline__ void column_sums(const float (*tab)[LEN], int wide, int rp, F done) {
+  int lanes = 1;
+  while (lanes < 64 && 2 * lanes * wide <= NT && lanes < rp) lanes *= 2;
+  const int lane = threadIdx.x & (lanes - 1);
+  for (int c = threadIdx.x / lanes; c < wide; c += NT / lanes) {
+    float s[NS];
+#pragma unroll
+    for (int k = 0; k < NS; ++k) s[k] = 0.0f;
+    for (int r = lane; r < rp; r += lanes)
+#pragma unroll
+      for (int k = 0; k < NS; ++k) s[k] += tab[k][r * wide + c];
+    for (int off = lanes >> 1; off > 0; off >>= 1)
+#pragma unroll
+      for (int k = 0; k < NS; ++k) s[k] += __shfl_xor(s[k], off, 64);
+    if (lane == 0) done(c, s);
+  }
+}
+
+template <int NS, int LA, int LB>
+__device__ __forceinline__ void join_groups(const float (*ent)[LA], int row_entries, int ge, int ng, int rp, int join,
+                                            int threads, float (*out)[LB]) {
   const int lane = threadIdx.x & (join - 1);
   const int dr = join / ge, dq = join - dr * ge;
   for (int g = threadIdx.x / join; g < ng; g += threads / join) {
@@ -244,7 +254,7 @@ __device__ __forceinline__ void join_groups(const float (*ent)[LEN], int row_ent
 
 // Column tiles, row lanes and row chunks of the split form: a row is cut into tiles of at most 256
 // pieces; the rows of a graph are cut so that about 2048 work-groups (eight per CU) share the
-// batch, each with at least eight rows per row lane.
+// batch, each with at least kLeast rows per row lane.
 struct SplitShape {
   int lanes, tiles, rp, chunk_rows, chunks;
 };
@@ -257,7 +267,7 @@ inline SplitShape split_shape(int B, int N, int C, int V, bool whole_blocks) {
   s.rp = kThreads / s.lanes;
   const int64_t have = (int64_t)B * s.tiles;
   const int want = (int)(have >= 2048 ? 1 : (2048 + have - 1) / have);
-  int rows = ceil_div(N, want), least = kBatch * s.rp;
+  int rows = ceil_div(N, want), least = kLeast * s.rp;
   if (rows < least) rows = least;
   s.chunk_rows = ceil_div(rows, s.rp) * s.rp;
   s.chunks = ceil_div(N, s.chunk_rows);
@@ -265,35 +275,33 @@ inline SplitShape split_shape(int B, int N, int C, int V, bool whole_blocks) {
 }
 
 // Slab of the resident form.  `align`: channels a slab has to start at a multiple of (32 where
-// checkpoints are written, the piece where one is read); `most`: pieces a work-group can hold;
-// `threads`: the widest row of pieces.  false: no slab of whole groups fits, or the batch would leave
-// most of the chip idle that the split form fills.
+// checkpoints are written, the piece where one is read); `threads` and `held`: the largest
+// work-group and the pieces a thread holds in it.  The slab is the widest of at most 4096 pieces (four such
+// work-groups share a CU: one's loads run beside another's sums) that leaves 1024 work-groups, but no
+// row segment is under 64 bytes; a longer one only if that narrowest one does not fit.  false: no
+// slab of whole groups fits, or the batch would leave most of the chip idle that the split form fills.
 struct ResidentShape {
-  int slab, nslab, lanes, pieces;
+  int slab, nslab, lanes;
 };
-inline bool resident_shape(int B, int N, int C, int cpg, int V, int align, int64_t most, int threads,
-                           ResidentShape *s) {
+inline bool resident_shape(int B, int N, int C, int cpg, int V, int align, int threads, int held, ResidentShape *s) {
   int64_t unit = cpg;
   while (unit % align && unit < C) unit += cpg;
   if (unit > C) unit = C;
   auto lanes_of = [&](int64_t slab) { return (int)(((slab + align - 1) / align * align + V - 1) / V); };
-  // as many slabs as make 1024 work-groups, none with a row segment under 64 bytes (4 pieces)
   const int64_t want = B >= 1024 ? 1 : (1024 + B - 1) / B;
   int64_t units = ((C + unit - 1) / unit + want - 1) / want;
   const int64_t least = (4 * V + unit - 1) / unit;
   if (units < least) units = least;
   for (;; --units) {
-    int64_t slab = units * unit;
-    if (slab > C) slab = C;
+    const int64_t slab = units * unit < C ? units * unit : C;
     const int lanes = lanes_of(slab);
-    if (lanes <= threads && (int64_t)N * lanes <= most) {
-      s->slab = (int)slab; s->lanes = lanes;
-      s->nslab = ceil_div(C, (int)slab);
-      s->pieces = N * lanes;
-      // a few long graphs: the split form's chunks fill the chip, these slabs would not
-      return (int64_t)B * s->nslab >= 128 || s->pieces <= 2048;
+    const bool fits = lanes <= threads && (int64_t)(threads / lanes) * held >= N;
+    const bool last = units <= least || units <= 1;
+    if (fits && (last || (int64_t)N * lanes <= 4096)) {
+      s->slab = (int)slab; s->lanes = lanes; s->nslab = ceil_div(C, (int)slab);
+      return (int64_t)B * s->nslab >= 128 || (int64_t)N * lanes <= 2048;
     }
-    if (units <= least || units <= 1) return false;
+    if (last) return false;
   }
 }
 // lanes that add up one of `groups` groups with `threads` threads
@@ -303,10 +311,30 @@ inline int join_lanes(int groups, int threads) {
   return j;
 }
 
-inline int64_t norm_ws_floats(int B, int C, int G) {
-  // the most partial rows any element type and form leads to (split: 2048 work-groups or one per
-  // graph; resident: at most one per graph), and A1, A2
-  return 2 * ((int64_t)2048 + B) * C + 2 * (int64_t)B * G;
+// which form a call takes, and the workspace it needs (floats): resident forward none; resident backward
+// a row of partial sums per graph lane; split the chunks' partial rows and A1, A2
+struct NormPlan {
+  bool resident;
+  ResidentShape rs;
+  SplitShape sp;
+  int graph_step;
+  int64_t floats;
+};
+inline NormPlan norm_plan(bool backward, int dtype, int B, int N, int C, int G, bool checkpoints) {
+  NormPlan p{};
+  const int V = dtype == GVAE_F32 ? 4 : 8, cpg = C / G;
+  p.resident = backward ? resident_shape(B, N, C, cpg, V, checkpoints ? V : 1, 512, 8, &p.rs)
+                        : resident_shape(B, N, C, cpg, V, checkpoints ? kBlock8 : 1, 1024, 16, &p.rs);
+  if (p.resident) {
+    // about 1024 work-groups walk the graphs of the backward
+    p.graph_step = p.rs.nslab >= 1024 ? 1 : 1024 / p.rs.nslab;
+    if (p.graph_step > B) p.graph_step = B;
+    p.floats = backward ? 2 * (int64_t)p.graph_step * C : 0;
+    return p;
+  }
+  p.sp = split_shape(B, N, C, V, !backward && checkpoints);
+  p.floats = 2 * (int64_t)B * p.sp.chunks * C + (backward ? 2 * (int64_t)B * G : 0);
+  return p;
 }
 
 int norm_check(const char *who, int dtype, int B, int N, int C, int G, int act, int64_t ld);

@@ -36,8 +36,8 @@ struct XPiece<T, true> {
 template <class T, bool KEPT, bool IN, int NT, int K>
 __global__ __launch_bounds__(NT) void norm_bwd_resident_kernel(NormArgs a) {
   constexpr int V = Piece<T>::V, E = IN ? 1 : V;
-  __shared__ float ent[2][NT * E], grp[2][NT * E];
-  const int lane_b = blockIdx.x / a.nslab, s0 = (blockIdx.x - lane_b * a.nslab) * a.slab;
+  __shared__ float ent[2][NT * V], grp[2][NT * E];
+  const int id = xcd_run(blockIdx.x, gridDim.x), lane_b = id / a.nslab, s0 = (id - lane_b * a.nslab) * a.slab;
   const int s1 = s0 + a.slab < a.C ? s0 + a.slab : a.C;
   const int col = threadIdx.x % a.lanes, r0 = threadIdx.x / a.lanes;
   const int c0 = s0 + col * V, nv = s1 - c0 < V ? s1 - c0 : V;
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(NT) void norm_bwd_resident_kernel(NormArgs a) {
       x[u].keep();
     }
     __syncthreads();
-    join_groups<2, NT * E>(ent, a.lanes * E, ge, ng, a.rp, a.join, NT, grp);
+    join_groups<2, NT * V, NT * E>(ent, a.lanes * E, ge, ng, a.rp, a.join, NT, grp);
     __syncthreads();
     const float inv = 1.0f / ((float)(live > 0 ? live : 1) * (float)a.cpg);
     float a1[E], a2[E];
@@ -150,75 +150,115 @@ __global__ __launch_bounds__(NT) void norm_bwd_resident_kernel(NormArgs a) {
       store_piece<T>((T *)a.out + ((int64_t)b * a.N + i) * a.C + c0, dx, nv);
     }
   }
-  // the row lanes of a channel, in their order, one channel of every piece at a time
+  // this work-group's row of partial sums
+  __syncthreads();
+  if (mine >= 0)
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    __syncthreads();
-    ent[0][threadIdx.x] = t1[v];
-    ent[1][threadIdx.x] = t2[v];
-    __syncthreads();
-    if (threadIdx.x < a.lanes && v < nv) {
-      float u1 = 0.0f, u2 = 0.0f;
-      for (int r = 0; r < a.rp; ++r) {
-        u1 += ent[0][r * a.lanes + threadIdx.x];
-        u2 += ent[1][r * a.lanes + threadIdx.x];
-      }
-      a.part1[(int64_t)lane_b * a.C + c0 + v] = u1;
-      a.part2[(int64_t)lane_b * a.C + c0 + v] = u2;
+    for (int v = 0; v < V; ++v) {
+      ent[0][threadIdx.x * V + v] = t1[v];
+      ent[1][threadIdx.x * V + v] = t2[v];
     }
-  }
+  __syncthreads();
+  column_sums<2, NT>(ent, a.lanes * V, a.rp, [&](int c, const float *s) {
+    if (s0 + c < s1) {
+      a.part1[(int64_t)lane_b * a.C + s0 + c] = s[0];
+      a.part2[(int64_t)lane_b * a.C + s0 + c] = s[1];
+    }
+  });
 }
 
 // --------------------------------------------------------------------------- split form
+constexpr int kAhead = 4;   // rows of a thread requested at a time
 template <class T, int ACT, bool KEPT>
 __global__ __launch_bounds__(kThreads) void norm_bwd_sums_kernel(NormArgs a) {
   constexpr int V = Piece<T>::V;
-  __shared__ float sh1[kThreads * V], sh2[kThreads * V];
-  const Place<V> p(a, true);
+  __shared__ float sh[2][kThreads * V];
+  const Place<V> p(a, true, false);
   float s1[V], s2[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) s1[v] = s2[v] = 0.0f;
   if (p.on && p.nv > 0) {
     const Scale<V> k(a, p.b, p.c0, p.nv);
     const T *dy = (const T *)a.dy + p.b * a.dyb + p.c0;
-    for (int i = p.chunk * a.chunk_rows + p.r; i < p.row_end; i += a.rp) {
-      const typename Piece<T>::raw g = load_piece<T>(dy + (int64_t)i * a.dyr, p.nv);
-      float x[V];
-      load_x<T, KEPT>(a, p.b, i, p.c0, p.nv, x);
+    for (int i0 = p.chunk * a.chunk_rows + p.r; i0 < p.row_end; i0 += kAhead * a.rp) {
+      typename Piece<T>::raw g[kAhead];
+      XPiece<T, KEPT> x[kAhead];
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float h = (x[v] - k.mean[v]) * k.rstd[v];
-        const float dz = (float)g[v] * act_slope<ACT>(h * k.w[v] + k.b[v]);
-        s1[v] += dz;
-        s2[v] = __fmaf_rn(dz, h, s2[v]);
+      for (int u = 0; u < kAhead; ++u) {
+        const int i = i0 + u * a.rp;
+        if (i >= p.row_end) break;
+        g[u] = load_piece<T>(dy + (int64_t)i * a.dyr, p.nv);
+        x[u].load(a, p.b, i, p.c0, p.nv);
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (i0 + u * a.rp >= p.row_end) break;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float h = (x[u].at(v) - k.mean[v]) * k.rstd[v];
+          const float dz = v < p.nv ? (float)g[u][v] * act_slope<ACT>(h * k.w[v] + k.b[v]) : 0.0f;
+          s1[v] += dz;
+          s2[v] += v < p.nv ? dz * h : 0.0f;
+        }
       }
     }
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    sh1[threadIdx.x * V + v] = s1[v];
-    sh2[threadIdx.x * V + v] = s2[v];
+    sh[0][threadIdx.x * V + v] = s1[v];
+    sh[1][threadIdx.x * V + v] = s2[v];
   }
   __syncthreads();
   const int wide = a.lanes * V;
-  for (int c = threadIdx.x; c < wide; c += kThreads) {
+  column_sums<2, kThreads>(sh, wide, a.rp, [&](int c, const float *s) {
     const int gc = blockIdx.y * wide + c;
-    if (gc >= a.C) continue;
-    float t1 = 0.0f, t2 = 0.0f;
-    for (int r = 0; r < a.rp; ++r) {
-      t1 += sh1[r * wide + c];
-      t2 += sh2[r * wide + c];
-    }
-    a.part1[(int64_t)blockIdx.x * a.C + gc] = t1;
-    a.part2[(int64_t)blockIdx.x * a.C + gc] = t2;
-  }
+    if (gc >= a.C) return;
+    a.part1[(int64_t)blockIdx.x * a.C + gc] = s[0];
+    a.part2[(int64_t)blockIdx.x * a.C + gc] = s[1];
+  });
 }
 
-// A1 and A2 of a group, a work-group per group
+// A row of 16 channels of dw or db: the partial rows summed by NT / 16 row lanes, in their order
 template <int NT>
-__global__ __launch_bounds__(NT) void norm_bwd_join_kernel(NormArgs a) {
-  __shared__ float sh[NT / 64];
-  const int64_t q = blockIdx.x;
+__device__ __forceinline__ void param_sums(const float *__restrict__ p, int64_t n, int C, int c,
+                                           float *__restrict__ out, float (*sh)[17]) {
+  const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4;
+  constexpr int L = NT / 16;
+  c += cl;
+  float s[8] = {};
+  if (c < C) {
+    int64_t r = rl;
+    for (; r + 7 * L < n; r += 8 * L)
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s[u] += p[(r + u * L) * C + c];
+    for (; r < n; r += L) s[0] += p[r * C + c];
+  }
+  sh[rl][cl] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+  __syncthreads();
+  if (rl == 0 && c < C) {
+    float t = 0.0f;
+    for (int k = 0; k < L; ++k) t += sh[k][cl];
+    out[c] = t;
+  }
+}
+__global__ __launch_bounds__(1024) void norm_bwd_params_kernel(NormArgs a, int64_t n, float *dw, float *db) {
+  __shared__ float sh[64][17];
+  param_sums<1024>(blockIdx.y ? a.part2 : a.part1, n, a.C, blockIdx.x * 16, blockIdx.y ? dw : db, sh);
+}
+
+// A1 and A2 of a group, a work-group per group, and behind the B * G groups the sums for dw and db
+// (both read the partial rows, neither waits for the other)
+template <int NT>
+__global__ __launch_bounds__(NT) void norm_bwd_join_kernel(NormArgs a, float *dw, float *db) {
+  __shared__ float sh[NT / 16][17];
+  const int64_t q = blockIdx.x, groups = (int64_t)a.B * a.G;
+  if (q >= groups) {
+    const int k = (int)(q - groups), tiles = (a.C + 15) / 16;
+    const bool second = k >= tiles;
+    param_sums<NT>(second ? a.part2 : a.part1, (int64_t)a.B * a.chunks, a.C, (second ? k - tiles : k) * 16,
+                   second ? dw : db, sh);
+    return;
+  }
   const int b = (int)(q / a.G), g = (int)(q - (int64_t)b * a.G);
   const int64_t base = (int64_t)b * a.chunks * a.C + g * a.cpg;
   float s1 = 0.0f, s2 = 0.0f;
@@ -229,8 +269,8 @@ __global__ __launch_bounds__(NT) void norm_bwd_join_kernel(NormArgs a) {
     s1 = __fmaf_rn(w, a.part1[base + (int64_t)k * a.C + c], s1);
     s2 = __fmaf_rn(w, a.part2[base + (int64_t)k * a.C + c], s2);
   }
-  s1 = group_sum<NT>(s1, sh);
-  s2 = group_sum<NT>(s2, sh);
+  s1 = group_sum<NT>(s1, &sh[0][0]);
+  s2 = group_sum<NT>(s2, &sh[0][0]);
   if (threadIdx.x == 0) {
     const int live = live_rows(a, b);
     const float m = (float)(live > 0 ? live : 1) * (float)a.cpg;
@@ -239,36 +279,11 @@ __global__ __launch_bounds__(NT) void norm_bwd_join_kernel(NormArgs a) {
   }
 }
 
-// dw and db: the partial rows summed, 16 channels x 64 row lanes per work-group
-__global__ __launch_bounds__(1024) void norm_bwd_params_kernel(const float *__restrict__ part1,
-                                                               const float *__restrict__ part2, int64_t n,
-                                                               int C, float *__restrict__ db,
-                                                               float *__restrict__ dw) {
-  __shared__ float sh[64][17];
-  const float *p = blockIdx.y ? part2 : part1;
-  float *out = blockIdx.y ? dw : db;
-  const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4, c = blockIdx.x * 16 + cl;
-  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (c < C) {
-    int64_t r = rl;
-    for (; r + 192 < n; r += 256)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) s[u] += p[(r + 64 * u) * C + c];
-    for (; r < n; r += 64) s[0] += p[r * C + c];
-  }
-  sh[rl][cl] = (s[0] + s[1]) + (s[2] + s[3]);
-  __syncthreads();
-  if (rl == 0 && c < C) {
-    float t = 0.0f;
-    for (int k = 0; k < 64; ++k) t += sh[k][cl];
-    out[c] = t;
-  }
-}
-
+// (walked from the last graph to the first: what the sums read last may still be in the caches)
 template <class T, int ACT, bool KEPT>
 __global__ __launch_bounds__(kThreads) void norm_bwd_apply_kernel(NormArgs a) {
   constexpr int V = Piece<T>::V;
-  const Place<V> p(a, false);
+  const Place<V> p(a, false, true);
   if (!p.on || p.nv <= 0) return;
   const int live = live_rows(a, p.b);
   const Scale<V> k(a, p.b, p.c0, p.nv);
@@ -280,33 +295,38 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_apply_kernel(NormArgs a) {
     a2[v] = a.A[2 * q + 1];
   }
   const T *dy = (const T *)a.dy + p.b * a.dyb + p.c0;
-  for (int i = p.chunk * a.chunk_rows + p.r; i < p.row_end; i += a.rp) {
-    float dx[V];
+  for (int i0 = p.chunk * a.chunk_rows + p.r; i0 < p.row_end; i0 += kAhead * a.rp) {
+    typename Piece<T>::raw g[kAhead];
+    XPiece<T, KEPT> x[kAhead];
 #pragma unroll
-    for (int v = 0; v < V; ++v) dx[v] = 0.0f;
-    if (i < live) {
-      const typename Piece<T>::raw g = load_piece<T>(dy + (int64_t)i * a.dyr, p.nv);
-      float x[V];
-      load_x<T, KEPT>(a, p.b, i, p.c0, p.nv, x);
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = i0 + u * a.rp;
+      if (i >= p.row_end || i >= live) break;
+      g[u] = load_piece<T>(dy + (int64_t)i * a.dyr, p.nv);
+      x[u].load(a, p.b, i, p.c0, p.nv);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = i0 + u * a.rp;
+      if (i >= p.row_end) break;
+      float dx[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const float h = (x[v] - k.mean[v]) * k.rstd[v];
-        const float dz = (float)g[v] * act_slope<ACT>(h * k.w[v] + k.b[v]);
-        dx[v] = k.rstd[v] * (dz * k.w[v] - __fmaf_rn(h, a2[v], a1[v]));
+        const float h = (x[u].at(v) - k.mean[v]) * k.rstd[v];
+        const float dz = (float)g[u][v] * act_slope<ACT>(h * k.w[v] + k.b[v]);
+        dx[v] = i < live ? k.rstd[v] * (dz * k.w[v] - __fmaf_rn(h, a2[v], a1[v])) : 0.0f;
       }
+      store_piece<T>((T *)a.out + ((int64_t)p.b * a.N + i) * a.C + p.c0, dx, p.nv);
     }
-    store_piece<T>((T *)a.out + ((int64_t)p.b * a.N + i) * a.C + p.c0, dx, p.nv);
   }
 }
-
 
 }  // namespace gvae
 
 using namespace gvae;
 
 static void params_launch(const NormArgs &a, int64_t rows, float *dw, float *db, hipStream_t s) {
-  hipLaunchKernelGGL(norm_bwd_params_kernel, dim3(ceil_div(a.C, 16), 2), dim3(1024), 0, s, a.part1, a.part2, rows, a.C,
-                     db, dw);
+  hipLaunchKernelGGL(norm_bwd_params_kernel, dim3(ceil_div(a.C, 16), 2), dim3(1024), 0, s, a, rows, dw, db);
 }
 
 template <class T, bool KEPT, bool IN>
@@ -331,16 +351,16 @@ static void resident_launch(NormArgs &a, hipStream_t s) {
   RUN(512, 8);
 #undef RUN
 }
-static bool resident_fits(int N, int lanes) { return lanes <= 512 && (int64_t)(512 / lanes) * 8 >= N; }
-
 template <class T, int ACT, bool KEPT>
 static void norm_bwd_launch(const NormArgs &a, const SplitShape &sh, float *dw, float *db, hipStream_t s) {
-  const dim3 grid((unsigned)(a.B * sh.chunks), sh.tiles), joins((unsigned)((int64_t)a.B * a.G));
+  const dim3 grid((unsigned)(a.B * sh.chunks), sh.tiles);
+  const dim3 joins((unsigned)((int64_t)a.B * a.G + (dw ? 2 * ceil_div(a.C, 16) : 0)));
   hipLaunchKernelGGL((norm_bwd_sums_kernel<T, ACT, KEPT>), grid, dim3(kThreads), 0, s, a);
-  if ((int64_t)sh.chunks * a.cpg <= 256) hipLaunchKernelGGL((norm_bwd_join_kernel<64>), joins, dim3(64), 0, s, a);
-  else hipLaunchKernelGGL((norm_bwd_join_kernel<512>), joins, dim3(512), 0, s, a);
+  if ((int64_t)sh.chunks * a.cpg <= 256 && (int64_t)a.B * sh.chunks <= 64)
+    hipLaunchKernelGGL((norm_bwd_join_kernel<64>), joins, dim3(64), 0, s, a, dw, db);
+  else
+    hipLaunchKernelGGL((norm_bwd_join_kernel<512>), joins, dim3(512), 0, s, a, dw, db);
   hipLaunchKernelGGL((norm_bwd_apply_kernel<T, ACT, KEPT>), grid, dim3(kThreads), 0, s, a);
-  if (dw) params_launch(a, (int64_t)a.B * sh.chunks, dw, db, s);
 }
 template <class T, bool KEPT>
 static void norm_bwd_act(const NormArgs &a, const SplitShape &sh, int act, float *dw, float *db, hipStream_t s) {
@@ -359,7 +379,7 @@ int gvae_group_norm_bwd(const void *d_dy, int dtype, int64_t dy_batch_stride, in
                         const int32_t *d_rows, int B, int N, int C, int G, const float *d_weight,
                         const float *d_bias, const float *d_mean, const float *d_rstd, int act, void *d_dx,
                         float *d_dweight, float *d_dbias, void *d_ws, void *stream) {
-  GVAE_REQUIRE(d_dy && d_dx && d_mean && d_rstd && d_ws, GVAE_EINVAL, "group_norm_bwd: null pointer");
+  GVAE_REQUIRE(d_dy && d_dx && d_mean && d_rstd, GVAE_EINVAL, "group_norm_bwd: null pointer");
   GVAE_REQUIRE(!d_dweight == !d_dbias, GVAE_EINVAL, "group_norm_bwd: weight and bias gradients come together");
   GVAE_REQUIRE(!d_x == (d_x8 && d_x8_scales) && !d_x8 == !d_x8_scales, GVAE_EINVAL,
                "group_norm_bwd: give either the input or its checkpoint (codes and scales)");
@@ -376,12 +396,11 @@ int gvae_group_norm_bwd(const void *d_dy, int dtype, int64_t dy_batch_stride, in
   a.act = act;
   hipStream_t s = (hipStream_t)stream;
   const int V = 16 / dtype_bytes(dtype);
-  ResidentShape rs;
-  if (resident_shape(B, N, C, a.cpg, V, d_x8 ? V : 1, 4096, 512, &rs) && resident_fits(N, rs.lanes)) {
-    a.slab = rs.slab; a.nslab = rs.nslab; a.lanes = rs.lanes;
-    // about 1024 work-groups, each with a row of partial sums; a single row is the result
-    a.graph_step = rs.nslab >= 1024 ? 1 : 1024 / rs.nslab;
-    if (a.graph_step > B) a.graph_step = B;
+  const NormPlan plan = norm_plan(true, dtype, B, N, C, G, d_x8 != nullptr);
+  GVAE_REQUIRE(d_ws, GVAE_EINVAL, "group_norm_bwd: null pointer");
+  if (plan.resident) {
+    a.slab = plan.rs.slab; a.nslab = plan.rs.nslab; a.lanes = plan.rs.lanes; a.graph_step = plan.graph_step;
+    // (a single row of sums is the result)
     const bool direct = a.graph_step == 1 && d_dweight;
     a.part1 = direct ? d_dbias : (float *)d_ws;
     a.part2 = direct ? d_dweight : a.part1 + (int64_t)a.graph_step * C;
@@ -395,7 +414,7 @@ int gvae_group_norm_bwd(const void *d_dy, int dtype, int64_t dy_batch_stride, in
     if (d_dweight && !direct) params_launch(a, a.graph_step, d_dweight, d_dbias, s);
     return check_launch("group_norm_bwd");
   }
-  const SplitShape sh = split_shape(B, N, C, V, false);
+  const SplitShape &sh = plan.sp;
   a.lanes = sh.lanes; a.rp = sh.rp; a.chunk_rows = sh.chunk_rows; a.chunks = sh.chunks;
   a.part1 = (float *)d_ws;
   a.part2 = a.part1 + (int64_t)B * sh.chunks * C;

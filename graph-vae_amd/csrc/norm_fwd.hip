@@ -14,7 +14,7 @@ template <class T, bool IN, int NT, int K>
 __global__ __launch_bounds__(NT) void norm_resident_kernel(NormArgs a) {
   constexpr int V = Piece<T>::V, E = IN ? 1 : V;
   __shared__ float ent[1][NT * E], grp[2][NT * E];
-  const int b = blockIdx.x / a.nslab, s0 = (blockIdx.x - b * a.nslab) * a.slab;
+  const int id = xcd_run(blockIdx.x, gridDim.x), b = id / a.nslab, s0 = (id - b * a.nslab) * a.slab;
   const int s1 = s0 + a.slab < a.C ? s0 + a.slab : a.C;
   const int col = threadIdx.x % a.lanes, r0 = threadIdx.x / a.lanes;
   const int c0 = s0 + col * V, nv = s1 - c0 < V ? s1 - c0 : V;
@@ -48,7 +48,7 @@ __global__ __launch_bounds__(NT) void norm_resident_kernel(NormArgs a) {
 #pragma unroll
   for (int u = 0; u < K; ++u) keep_raw<T>(k[u]);
   __syncthreads();
-  join_groups<1, NT * E>(ent, a.lanes * E, ge, ng, a.rp, a.join, NT, grp);
+  join_groups<1, NT * E, NT * E>(ent, a.lanes * E, ge, ng, a.rp, a.join, NT, grp);
   __syncthreads();
   auto group_of = [&](int e) {
     const int c = c0 + e < s1 ? c0 + e : s1 - 1;
@@ -75,7 +75,7 @@ __global__ __launch_bounds__(NT) void norm_resident_kernel(NormArgs a) {
 #pragma unroll
   for (int u = 0; u < K; ++u) keep_raw<T>(k[u]);
   __syncthreads();
-  join_groups<1, NT * E>(ent, a.lanes * E, ge, ng, a.rp, a.join, NT, grp + 1);
+  join_groups<1, NT * E, NT * E>(ent, a.lanes * E, ge, ng, a.rp, a.join, NT, grp + 1);
   __syncthreads();
 #pragma unroll
   for (int e = 0; e < E; ++e) rstd[e] = 1.0f / sqrtf(grp[1][group_of(e)] * inv + a.eps);
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(kThreads) void norm_stats_kernel(NormArgs a) {
   constexpr int V = Piece<T>::V;
   __shared__ float sh_mean[kThreads * V], sh_m2[kThreads * V];
   __shared__ int sh_n[kThreads];
-  const Place<V> p(a, true);
+  const Place<V> p(a, true, false);
   const int row0 = p.chunk * a.chunk_rows;
   float mean[V], m2[V];
   int n = 0;
@@ -225,41 +225,49 @@ __global__ __launch_bounds__(NT) void norm_stats_join_kernel(NormArgs a) {
   }
 }
 
+// Rows of a thread are requested kAhead at a time.  The graphs are walked from the last to the first: what
+// the statistics read last may still be in the caches.
+constexpr int kAhead = 4;
 template <class T, int ACT>
 __global__ __launch_bounds__(kThreads) void norm_apply_kernel(NormArgs a) {
   constexpr int V = Piece<T>::V;
-  const Place<V> p(a, false);
+  const Place<V> p(a, false, true);
   if (!p.on) return;
   const int live = live_rows(a, p.b);
   const Scale<V> k(a, p.b, p.c0, p.nv);
   const T *x = (const T *)a.x + p.b * a.xb + p.c0;
-  for (int i = p.chunk * a.chunk_rows + p.r; i < p.row_end; i += a.rp) {
-    float xf[V], y[V];
+  for (int i0 = p.chunk * a.chunk_rows + p.r; i0 < p.row_end; i0 += kAhead * a.rp) {
+    typename Piece<T>::raw r[kAhead];
 #pragma unroll
-    for (int v = 0; v < V; ++v) xf[v] = y[v] = 0.0f;
-    if (i < live && p.nv > 0) {
-      const typename Piece<T>::raw r = load_piece<T>(x + (int64_t)i * a.xr, p.nv);
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = i0 + u * a.rp;
+      r[u] = typename Piece<T>::raw{};
+      if (i < p.row_end && i < live && p.nv > 0) r[u] = load_piece<T>(x + (int64_t)i * a.xr, p.nv);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = i0 + u * a.rp;
+      if (i >= p.row_end) break;
+      float xf[V], y[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        if (v < p.nv) {
-          xf[v] = (float)r[v];
-          y[v] = (float)(T)act_value<ACT>((xf[v] - k.mean[v]) * k.rstd[v] * k.w[v] + k.b[v]);
-        }
+        xf[v] = (float)r[u][v];
+        y[v] = i < live && v < p.nv
+                   ? (float)(T)act_value<ACT>((xf[v] - k.mean[v]) * k.rstd[v] * k.w[v] + k.b[v]) : 0.0f;
       }
+      const int64_t row = (int64_t)p.b * a.N + i;
+      if (p.nv > 0) store_piece<T>((T *)a.out + row * a.C + p.c0, y, p.nv);
+      // (the lanes of a block share a row: with checkpoints kept, `lanes` is a whole number of blocks)
+      const int nc = a.ld8 - p.c0;
+      const bool first = p.c0 % kBlock8 == 0 && p.nv > 0;
+      if (a.x8) emit8<V>(xf, a.x8 + row * a.ld8 + p.c0, nc, a.x8s + row * a.nb8 + p.c0 / kBlock8, first);
+      if (a.y8) emit8<V>(y, a.y8 + row * a.ld8 + p.c0, nc, a.y8s + row * a.nb8 + p.c0 / kBlock8, first);
     }
-    const int64_t row = (int64_t)p.b * a.N + i;
-    if (p.nv > 0) store_piece<T>((T *)a.out + row * a.C + p.c0, y, p.nv);
-    // (the lanes of a block share a row: with checkpoints kept, `lanes` is a whole number of blocks)
-    const int nc = a.ld8 - p.c0;
-    const bool first = p.c0 % kBlock8 == 0 && p.nv > 0;
-    if (a.x8) emit8<V>(xf, a.x8 + row * a.ld8 + p.c0, nc, a.x8s + row * a.nb8 + p.c0 / kBlock8, first);
-    if (a.y8) emit8<V>(y, a.y8 + row * a.ld8 + p.c0, nc, a.y8s + row * a.nb8 + p.c0 / kBlock8, first);
   }
 }
 
-
 template <class T, bool IN>
-static void resident_launch(NormArgs &a, const ResidentShape &rs, hipStream_t s) {
+static void resident_launch(NormArgs &a, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)a.B * a.nslab));
   const int groups = a.slab / a.cpg;
 #define RUN(NT, K)                                                                        \
@@ -276,15 +284,12 @@ static void resident_launch(NormArgs &a, const ResidentShape &rs, hipStream_t s)
     RUN(256, 2);
     RUN(256, 4);
     RUN(256, 8);
+    RUN(256, 16);
   }
-  RUN(1024, 4);
   RUN(1024, 8);
   RUN(1024, 16);
 #undef RUN
 }
-
-// whether NT threads with K pieces each hold N rows of `lanes` pieces, for the largest form
-static bool resident_fits(int N, int lanes) { return lanes <= 1024 && (int64_t)(1024 / lanes) * 16 >= N; }
 
 }  // namespace gvae
 
@@ -292,9 +297,9 @@ using namespace gvae;
 
 extern "C" {
 
-int64_t gvae_group_norm_ws_bytes(int B, int N, int C, int G) {
-  if (B <= 0 || N <= 0 || C <= 0 || G <= 0) return 0;
-  return norm_ws_floats(B, C, G) * 4;
+int64_t gvae_group_norm_ws_bytes(int backward, int dtype, int B, int N, int C, int G, int checkpoints) {
+  if (!dtype_known(dtype) || B <= 0 || N <= 0 || C <= 0 || G <= 0 || C % G) return 0;
+  return 4 * norm_plan(backward != 0, dtype, B, N, C, G, checkpoints != 0).floats;
 }
 
 }  // extern "C"
@@ -318,7 +323,7 @@ int gvae_group_norm_fwd(const void *d_x, int dtype, int64_t batch_stride, int64_
                         int B, int N, int C, int G, const float *d_weight, const float *d_bias, float eps, int act,
                         void *d_y, float *d_mean, float *d_rstd, int8_t *d_x8, uint8_t *d_x8_scales, int8_t *d_y8,
                         uint8_t *d_y8_scales, void *d_ws, void *stream) {
-  GVAE_REQUIRE(d_x && d_y && d_mean && d_rstd && d_ws, GVAE_EINVAL, "group_norm_fwd: null pointer");
+  GVAE_REQUIRE(d_x && d_y && d_mean && d_rstd, GVAE_EINVAL, "group_norm_fwd: null pointer");
   GVAE_REQUIRE(!d_x8 == !d_x8_scales && !d_y8 == !d_y8_scales, GVAE_EINVAL,
                "group_norm_fwd: a checkpoint needs both its codes and its scales");
   GVAE_REQUIRE(eps > 0.0f && std::isfinite(eps), GVAE_EINVAL, "group_norm_fwd: eps must be positive");
@@ -333,17 +338,18 @@ int gvae_group_norm_fwd(const void *d_x, int dtype, int64_t batch_stride, int64_
   a.ld8 = ckpt8_ld(C); a.nb8 = ckpt8_blocks(C);
   a.act = act;
   const int V = 16 / dtype_bytes(dtype);
-  const bool keep = d_x8 || d_y8;
-  ResidentShape rs;
-  if (resident_shape(B, N, C, a.cpg, V, keep ? kBlock8 : 1, 16384, 1024, &rs) && resident_fits(N, rs.lanes)) {
+  const NormPlan plan = norm_plan(false, dtype, B, N, C, G, d_x8 || d_y8);
+  GVAE_REQUIRE(d_ws || !plan.floats, GVAE_EINVAL, "group_norm_fwd: null pointer");
+  if (plan.resident) {
+    const ResidentShape &rs = plan.rs;
     a.slab = rs.slab; a.nslab = rs.nslab; a.lanes = rs.lanes;
     GVAE_DTYPE_SWITCH(dtype, T, {
-      if (a.cpg % V == 0) resident_launch<T, true>(a, rs, s);
-      else resident_launch<T, false>(a, rs, s);
+      if (a.cpg % V == 0) resident_launch<T, true>(a, s);
+      else resident_launch<T, false>(a, s);
     });
     return check_launch("group_norm_fwd");
   }
-  const SplitShape sh = split_shape(B, N, C, V, keep);
+  const SplitShape &sh = plan.sp;
   a.lanes = sh.lanes; a.rp = sh.rp; a.chunk_rows = sh.chunk_rows; a.chunks = sh.chunks;
   a.part1 = (float *)d_ws;
   a.part2 = a.part1 + (int64_t)B * sh.chunks * C;

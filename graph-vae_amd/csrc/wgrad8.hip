@@ -10,7 +10,7 @@
 // one column are a column of the tile: tiles are staged row by row in LDS and read through
 // the transposing ds_read_b64_tr_b16 (a group of 16 lanes reads 4 rows x 16 columns and gets 4 rows
 // of one column each).  Those 4 rows are brought to different banks by XORing the 64-byte piece of a
-// row with its row number mod 4.
+// row with bits of its row number.
 //
 // A work-group owns a tile of dW and a range of rows; the parts are summed in their order by a second
 // launch.  Column sums of dY ride along: among the work-groups that share a dY tile, each adds up its
@@ -54,10 +54,17 @@ __device__ __forceinline__ void cut(float x, uint16_t *out) {
   }
 }
 
-// byte offset of column c (a multiple of 8) of row k in a tile of `W` columns
+// What the 64-byte piece of a row is XORed with in a tile of W columns: four rows that are read together
+// then lie in different banks (256 bytes of them; two rows of 64 columns fill those already).
+template <int W>
+__device__ __forceinline__ int swizzle(int k) {
+  static_assert(W == 64 || W % 128 == 0, "pieces of a row");
+  return W == 64 ? (k >> 1) & 1 : k & 3;
+}
+// byte offset of column c (a multiple of 8) of row k
 template <int W>
 __device__ __forceinline__ int tile_at(int k, int c) {
-  return k * (2 * W) + (((c >> 5) ^ (k & 3)) << 6) + 2 * (c & 31);
+  return k * (2 * W) + (((c >> 5) ^ swizzle<W>(k)) << 6) + 2 * (c & 31);
 }
 
 // FM x FN matrix-core tiles of 32 x 32 per wavefront, WM x WN wavefronts, KT rows per step
@@ -76,10 +83,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad8_kernel(WgradArgs a) {
   using S = Wgrad<T, FM, FN, WM, WN, KT>;
   constexpr int P = S::P, V = S::V, TM = S::TM, TN = S::TN, NT = S::NT;
   extern __shared__ __align__(16) char lds[];
-  // consecutive work-groups go to the eight XCDs in turn: each XCD takes a run of the numbering below,
-  // in which the tiles of one row range are neighbours and share that range in the XCD's L2
-  const int total = gridDim.x, xcd = blockIdx.x & 7, q8 = total >> 3, r8 = total & 7;
-  const int id = xcd * q8 + (xcd < r8 ? xcd : r8) + ((int)blockIdx.x >> 3);
+  // (the tiles of one row range are neighbours: they share that range in an XCD's L2)
+  const int id = xcd_run(blockIdx.x, gridDim.x);
   const int tiles = a.tx * a.ty, split = id / tiles, tile = id - split * tiles;
   const int ix = tile % a.tx, i0 = ix * TN, o0 = (tile / a.tx) * TM;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
@@ -175,10 +180,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad8_kernel(WgradArgs a) {
       for (int q = 0; q < 16; ++q) acc[m][n][q] = 0.0f;
 
   // transposed read: this lane's row within a group of four, its 16 columns and 4 of them
-  const int kr = 8 * (lane >> 5) + ((lane >> 2) & 3), sw = (lane >> 2) & 3;
+  const int kr = 8 * (lane >> 5) + ((lane >> 2) & 3), swa = swizzle<TM>(kr), swb = swizzle<TN>(kr);
   const int off = 2 * (16 * ((lane >> 4) & 1) + 4 * (lane & 3));
   typedef __attribute__((address_space(3))) s16x4 *lds_ptr;
-  auto frag = [&](char *base, int rowbytes, int k0, int blk) -> bf16x8 {
+  auto frag = [&](char *base, int rowbytes, int k0, int blk, int sw) -> bf16x8 {
     char *p = base + (k0 + kr) * rowbytes + ((blk ^ sw) << 6) + off;
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p);
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 4 * rowbytes));
@@ -189,12 +194,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad8_kernel(WgradArgs a) {
     for (int k0 = 0; k0 < KT; k0 += 16) {
       bf16x8 bf[FN];
 #pragma unroll
-      for (int n = 0; n < FN; ++n) bf[n] = frag(buf + P * S::kBytesA, 2 * TN, k0, wn * FN + n);
+      for (int n = 0; n < FN; ++n) bf[n] = frag(buf + P * S::kBytesA, 2 * TN, k0, wn * FN + n, swb);
 #pragma unroll
       for (int p = 0; p < P; ++p)
 #pragma unroll
         for (int m = 0; m < FM; ++m) {
-          const bf16x8 af = frag(buf + p * S::kBytesA, 2 * TM, k0, wm * FM + m);
+          const bf16x8 af = frag(buf + p * S::kBytesA, 2 * TM, k0, wm * FM + m, swa);
 #pragma unroll
           for (int n = 0; n < FN; ++n)
             acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af, bf[n], acc[m][n], 0, 0, 0);
@@ -243,42 +248,75 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad8_kernel(WgradArgs a) {
   }
 }
 
-// The parts of dW (if there is more than one) and of db, in their order
-template <class T>
-__global__ __launch_bounds__(256) void wgrad8_sum_kernel(WgradArgs a) {
-  const int64_t n = a.splits > 1 ? (int64_t)a.O * a.I : 0, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e < n) {
-    float s = 0.0f;
-    for (int k = 0; k < a.splits; ++k) s += a.part[k * n + e];
-    ((T *)a.dw)[e] = (T)s;
-  } else if (e < n + a.O && a.db) {
-    float s = 0.0f;
-    for (int k = 0; k < a.splits * a.tx; ++k) s += a.part_b[(int64_t)k * a.O + (e - n)];
-    ((T *)a.db)[e - n] = (T)s;
+// The parts of dW (if there is more than one) and of db, in a fixed order: a work-group's 256 threads are
+// PL lanes to a value's parts times lanes of VW neighbouring values.  The first `wide_groups`
+// work-groups sum dW, the others db.
+template <class T, int VW, int PL>
+__global__ __launch_bounds__(256) void wgrad8_sum_kernel(WgradArgs a, unsigned wide_groups) {
+  typedef float vec __attribute__((ext_vector_type(VW)));
+  constexpr int L = 256 / PL;
+  __shared__ vec sh[PL][L];
+  const int lane = threadIdx.x % L, part = threadIdx.x / L;
+  if (blockIdx.x < wide_groups) {
+    const int64_t n = (int64_t)a.O * a.I, e = ((int64_t)blockIdx.x * L + lane) * VW;
+    vec s[4] = {};
+    if (e < n) {
+      int k = part;
+      for (; k + 3 * PL < a.splits; k += 4 * PL)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) s[u] += *reinterpret_cast<const vec *>(a.part + (k + PL * u) * n + e);
+      for (; k < a.splits; k += PL) s[0] += *reinterpret_cast<const vec *>(a.part + k * n + e);
+    }
+    s[0] = (s[0] + s[1]) + (s[2] + s[3]);
+    if (PL > 1) {
+      sh[part][lane] = s[0];
+      __syncthreads();
+      if (part != 0) return;
+#pragma unroll
+      for (int k = 1; k < PL; ++k) s[0] += sh[k][lane];
+    }
+    if (e >= n) return;
+    T *out = (T *)a.dw + e;
+#pragma unroll
+    for (int v = 0; v < VW; ++v) out[v] = (T)s[0][v];
+    return;
+  }
+  const int o = (blockIdx.x - wide_groups) * 16 + (threadIdx.x & 15), p0 = threadIdx.x >> 4, parts = a.splits * a.tx;
+  float s = 0.0f;
+  if (o < a.O)
+    for (int k = p0; k < parts; k += 16) s += a.part_b[(int64_t)k * a.O + o];
+  float *f = reinterpret_cast<float *>(sh);
+  f[threadIdx.x] = s;
+  __syncthreads();
+  if (p0 == 0 && o < a.O) {
+    for (int k = 1; k < 16; ++k) s += f[16 * k + threadIdx.x];
+    ((T *)a.db)[o] = (T)s;
   }
 }
 
 struct WgradShape {
-  int tm, tn, tx, ty, splits;
+  int tm, tx, ty, splits;
   int64_t split_rows;
 };
-// A tile of 256 x 256 if both sides fill at least one and there is work for every CU, else 128 x 128;
-// rows are split until there is a work-group for each CU (two of the small ones), no
-// range shorter than 128 rows.
+// A tile of 256 x 256 where both sides fill one and the rows are many, else of 128 x 128; of 64 x 64
+// where the larger ones would leave most of the chip without a work-group.  Rows are split until
+// there is a work-group for each CU (two of the smaller ones), no range shorter than 128 rows.
 static WgradShape wgrad_shape(int64_t rows, int O, int I) {
   WgradShape s;
-  const bool big = O >= 256 && I >= 256 && rows >= 1024;
-  s.tm = s.tn = big ? 256 : 128;
-  s.tx = ceil_div(I, s.tn);
-  s.ty = ceil_div(O, s.tm);
-  const int64_t tiles = (int64_t)s.tx * s.ty, fill = big ? 256 : 512;
-  int64_t want = tiles >= fill ? 1 : fill / tiles;
   const int64_t most = (rows + 127) / 128;
+  s.tm = 128;
+  if (O >= 256 && I >= 256 && rows >= 1024) s.tm = 256;
+  else if ((int64_t)ceil_div(I, 128) * ceil_div(O, 128) * most < 256) s.tm = 64;
+  s.tx = ceil_div(I, s.tm);
+  s.ty = ceil_div(O, s.tm);
+  const int64_t tiles = (int64_t)s.tx * s.ty, fill = s.tm == 256 ? 256 : 512;
+  int64_t want = tiles >= fill ? 1 : fill / tiles;
   if (want > most) want = most;
   s.split_rows = ((rows + want - 1) / want + 63) / 64 * 64;
   s.splits = (int)((rows + s.split_rows - 1) / s.split_rows);
   return s;
 }
+static int64_t wgrad_bias_floats(const WgradShape &s, int O) { return ((int64_t)s.splits * s.tx * O + 3) / 4 * 4; }
 
 template <class T, int FM, int FN, int WM, int WN, int KT>
 static int wgrad_launch(const WgradArgs &a, hipStream_t s) {
@@ -292,6 +330,21 @@ static int wgrad_launch(const WgradArgs &a, hipStream_t s) {
   return GVAE_OK;
 }
 
+// many parts: 16 lanes to a value's parts (4 where rows of dW are not whole vectors); few: one
+template <class T>
+static void sum_launch(const WgradArgs &a, hipStream_t s) {
+  const int64_t n = a.splits > 1 ? (int64_t)a.O * a.I : 0;
+  const unsigned bias_groups = a.db ? ceil_div(a.O, 16) : 0;
+  auto run = [&](auto kernel, int values) {
+    const unsigned wide = (unsigned)((n + values - 1) / values);
+    if (wide + bias_groups > 0) hipLaunchKernelGGL(kernel, dim3(wide + bias_groups), dim3(256), 0, s, a, wide);
+  };
+  if (n % 4 == 0 && a.splits <= 8) run(wgrad8_sum_kernel<T, 4, 1>, 1024);
+  else if (n % 4 == 0) run(wgrad8_sum_kernel<T, 4, 16>, 64);
+  else if (a.splits <= 8) run(wgrad8_sum_kernel<T, 1, 1>, 256);
+  else run(wgrad8_sum_kernel<T, 1, 4>, 64);
+}
+
 }  // namespace gvae
 
 using namespace gvae;
@@ -301,7 +354,7 @@ extern "C" {
 int64_t gvae_linear_wgrad8_ws_bytes(int64_t rows, int O, int I) {
   if (rows <= 0 || O <= 0 || I <= 0) return 0;
   const WgradShape s = wgrad_shape(rows, O, I);
-  return 4 * (int64_t)s.splits * ((s.splits > 1 ? (int64_t)O * I : 0) + (int64_t)s.tx * O);
+  return 4 * (wgrad_bias_floats(s, O) + (s.splits > 1 ? (int64_t)s.splits * O * I : 0));
 }
 
 int gvae_linear_wgrad8(const void *d_dy, int dtype, int64_t row_stride, const int8_t *d_codes, const uint8_t *d_scales,
@@ -313,22 +366,21 @@ int gvae_linear_wgrad8(const void *d_dy, int dtype, int64_t row_stride, const in
                (long long)row_stride);
   const WgradShape sh = wgrad_shape(rows, O, I);
   GVAE_REQUIRE(O <= (1 << 20) && I <= (1 << 20) && (int64_t)sh.tx * sh.ty * sh.splits < (1LL << 31) &&
-                   sh.split_rows < (1LL << 36) && (int64_t)O * I < (1LL << 38), GVAE_ELIMIT,
+                   sh.split_rows < (1LL << 36) && (int64_t)O * I < (1LL << 36), GVAE_ELIMIT,
                "linear_wgrad8: %lld rows, %d x %d weights", (long long)rows, O, I);
   WgradArgs a;
   a.dy = d_dy; a.codes = d_codes; a.scales = d_scales; a.dw = d_dw; a.db = d_db;
   a.rows = rows; a.ldy = row_stride; a.O = O; a.I = I; a.ld8 = ckpt8_ld(I); a.nb8 = ckpt8_blocks(I);
   a.splits = sh.splits; a.split_rows = sh.split_rows; a.tx = sh.tx; a.ty = sh.ty;
   a.part_b = (float *)d_ws;
-  a.part = a.part_b + (int64_t)sh.splits * sh.tx * O;
+  a.part = a.part_b + wgrad_bias_floats(sh, O);
   hipStream_t s = (hipStream_t)stream;
   int rc = GVAE_OK;
   GVAE_DTYPE_SWITCH(dtype, T, {
     constexpr int kDeep = Pieces<T>::P == 1 ? 64 : 32;
-    rc = sh.tm == 256 ? wgrad_launch<T, 4, 2, 2, 4, kDeep>(a, s) : wgrad_launch<T, 2, 2, 2, 2, kDeep>(a, s);
-    const int64_t n = (sh.splits > 1 ? (int64_t)O * I : 0) + (d_db ? O : 0);
-    if (rc == GVAE_OK && n > 0)
-      hipLaunchKernelGGL((wgrad8_sum_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a);
+    rc = sh.tm == 256 ? wgrad_launch<T, 4, 2, 2, 4, kDeep>(a, s)
+         : sh.tm == 128 ? wgrad_launch<T, 2, 2, 2, 2, kDeep>(a, s) : wgrad_launch<T, 1, 1, 2, 2, 64>(a, s);
+    if (rc == GVAE_OK) sum_launch<T>(a, s);
   });
   if (rc) return rc;
   return check_launch("linear_wgrad8");

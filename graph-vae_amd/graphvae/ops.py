@@ -33,7 +33,7 @@ def _bind():
         L = _hip.lib()
         L.gvae_ckpt8_write.argtypes = [c_void_p, c_int, c_int64, c_int, c_int64, c_void_p, c_void_p, c_void_p]
         L.gvae_ckpt8_read.argtypes = [c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int, c_int64, c_void_p]
-        L.gvae_group_norm_ws_bytes.argtypes = [c_int] * 4
+        L.gvae_group_norm_ws_bytes.argtypes = [c_int] * 7
         L.gvae_group_norm_ws_bytes.restype = c_int64
         L.gvae_group_norm_fwd.argtypes = [c_void_p, c_int, c_int64, c_int64, c_void_p, c_int, c_int, c_int, c_int,
                                           c_void_p, c_void_p, c_float, c_int] + [c_void_p] * 9
@@ -99,12 +99,21 @@ def _graph_strides(t: torch.Tensor, what: str) -> tuple[int, int]:
     return batch, row
 
 
+_NONE = (None, None)
+
+
+def _workspace(n: int, device):
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
 class Checkpoint8:
     """An activation kept in 8 bits: `codes` (..., 16*ceil(C/16)) int8 and `scales` (..., ceil(C/32))
     uint8, value = code * 2^(scale - 127) with one scale per 32 consecutive channels of a row (each
-    value off by at most 1/127 of its block's largest).  `channels` is C; `dtype` what `read` returns."""
+    value off by at most 1/127 of its block's largest).  `channels` is C; `dtype` what `read` returns.
 
-    __slots__ = ("codes", "scales", "channels", "dtype")
+    Checkpoint8(codes, scales, channels, dtype) wraps existing tensors, which it keeps."""
+
+    __slots__ = ("_codes", "_scales", "_buf", "_at", "shape", "dtype", "device")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, channels: int,
                  dtype: torch.dtype = torch.bfloat16) -> None:
@@ -121,37 +130,66 @@ class Checkpoint8:
             raise _hip.GvaeHipError(f"Checkpoint8: cannot be read as {dtype}")
         if codes.data_ptr() % 16:
             raise _hip.GvaeHipError("Checkpoint8: codes must be 16-byte aligned")
-        self.codes, self.scales, self.channels, self.dtype = codes, scales, C, dtype
+        self._codes, self._scales, self._buf = codes, scales, None
+        self._at = (codes.data_ptr(), scales.data_ptr())
+        self.shape, self.dtype, self.device = lead + (C,), dtype, codes.device
+
+    @classmethod
+    def _new(cls, shape: tuple, device, dtype: torch.dtype) -> "Checkpoint8":
+        """Room for a checkpoint: one allocation, the codes first."""
+        self = object.__new__(cls)
+        C = shape[-1]
+        rows = 1
+        for n in shape[:-1]:
+            rows *= n
+        n_codes = rows * ((C + 15) // 16 * 16)
+        self._buf = torch.empty(n_codes + rows * ((C + 31) // 32), dtype=torch.uint8, device=device)
+        base = self._buf.data_ptr()
+        self._codes = self._scales = None
+        self._at = (base, base + n_codes)
+        self.shape, self.dtype, self.device = tuple(shape), dtype, device
+        return self
+
+    def __reduce__(self):
+        # (copies and pickles hold their own memory)
+        return Checkpoint8, (self.codes, self.scales, self.channels, self.dtype)
 
     @property
-    def shape(self) -> tuple[int, ...]:
-        return tuple(self.codes.shape[:-1]) + (self.channels,)
+    def channels(self) -> int:
+        return self.shape[-1]
 
-    def _check(self, what: str) -> "Checkpoint8":
-        _on_device(self.codes, what)
-        if self.codes.numel() == 0:
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            self._codes = self._buf[:self._at[1] - self._at[0]].view(torch.int8).view(
+                self.shape[:-1] + ((self.shape[-1] + 15) // 16 * 16,))
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._scales = self._buf[self._at[1] - self._at[0]:].view(
+                self.shape[:-1] + ((self.shape[-1] + 31) // 32,))
+        return self._scales
+
+    def _check(self, what: str) -> None:
+        _on_device(self._buf if self._codes is None else self._codes, what)
+        if 0 in self.shape:
             raise _hip.GvaeHipError(f"{what}: no element in shape {self.shape}")
-        return self
 
     def read(self, dtype: torch.dtype | None = None) -> torch.Tensor:
         """The values the checkpoint stands for, as `dtype` (default: the type that was written);
         exact in bfloat16 and float32."""
         dtype = self.dtype if dtype is None else dtype
-        if dtype not in _DTYPE:
+        code = _DTYPE.get(dtype)
+        if code is None:
             raise _hip.GvaeHipError(f"Checkpoint8.read: cannot be read as {dtype}")
         self._check("Checkpoint8.read")
-        out = torch.empty(self.shape, dtype=dtype, device=self.codes.device)
-        C = self.channels
-        _hip._check(_bind().gvae_ckpt8_read(self.codes.data_ptr(), self.scales.data_ptr(), out.numel() // C, C,
-                                            out.data_ptr(), _DTYPE[dtype], C, _hip._stream()))
+        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        C = self.shape[-1]
+        _hip._check(_bind().gvae_ckpt8_read(self._at[0], self._at[1], out.numel() // C, C, out.data_ptr(), code, C,
+                                            _hip._stream()))
         return out
-
-
-def _empty8(shape, device, dtype) -> Checkpoint8:
-    C = shape[-1]
-    lead = tuple(shape[:-1])
-    return Checkpoint8(torch.empty(lead + ((C + 15) // 16 * 16,), dtype=torch.int8, device=device),
-                       torch.empty(lead + ((C + 31) // 32,), dtype=torch.uint8, device=device), C, dtype)
 
 
 def checkpoint8(x: torch.Tensor) -> Checkpoint8:
@@ -161,9 +199,8 @@ def checkpoint8(x: torch.Tensor) -> Checkpoint8:
     if x.dim() < 1:
         raise _hip.GvaeHipError("checkpoint8: expected at least one axis")
     rows, ld = _rows_of(x, "checkpoint8")
-    c = _empty8(x.shape, x.device, x.dtype)
-    _hip._check(_bind().gvae_ckpt8_write(x.data_ptr(), code, rows, x.shape[-1], ld, c.codes.data_ptr(),
-                                         c.scales.data_ptr(), _hip._stream()))
+    c = Checkpoint8._new(x.shape, x.device, x.dtype)
+    _hip._check(_bind().gvae_ckpt8_write(x.data_ptr(), code, rows, x.shape[-1], ld, *c._at, _hip._stream()))
     return c
 
 
@@ -223,16 +260,14 @@ def group_norm_act(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Ten
         raise ValueError(f"{what}: eps must be positive, got {eps}")
     L, dev = _bind(), x.device
     y = torch.empty((B, N, C), dtype=x.dtype, device=dev)
-    stats = torch.empty((2, B, groups), dtype=torch.float32, device=dev)
-    x8 = _empty8(x.shape, dev, x.dtype) if keep_x else None
-    y8 = _empty8(x.shape, dev, x.dtype) if keep_y else None
-    ws = torch.empty(L.gvae_group_norm_ws_bytes(B, N, C, groups), dtype=torch.uint8, device=dev)
-    mean, rstd = stats[0], stats[1]
+    mean, rstd = torch.empty((2, B, groups), dtype=torch.float32, device=dev).unbind(0)
+    x8 = Checkpoint8._new((B, N, C), dev, x.dtype) if keep_x else None
+    y8 = Checkpoint8._new((B, N, C), dev, x.dtype) if keep_y else None
+    ws = _workspace(L.gvae_group_norm_ws_bytes(0, code, B, N, C, groups, keep_x or keep_y), dev)
     _hip._check(L.gvae_group_norm_fwd(
         x.data_ptr(), code, batch, row, live, B, N, C, groups, w, b, eps, act_code, y.data_ptr(), mean.data_ptr(),
-        rstd.data_ptr(), x8.codes.data_ptr() if keep_x else None, x8.scales.data_ptr() if keep_x else None,
-        y8.codes.data_ptr() if keep_y else None, y8.scales.data_ptr() if keep_y else None, ws.data_ptr(),
-        _hip._stream()))
+        rstd.data_ptr(), *(x8._at if keep_x else _NONE), *(y8._at if keep_y else _NONE),
+        None if ws is None else ws.data_ptr(), _hip._stream()))
     return GroupNormOut(y, mean, rstd, x8, y8)
 
 
@@ -251,7 +286,7 @@ def group_norm_act_backward(dy: torch.Tensor, x, weight: torch.Tensor | None, bi
         x._check(what)
         if x.shape != (B, N, C):
             raise _hip.GvaeHipError(f"{what}: checkpoint of shape {x.shape}, gradient {tuple(dy.shape)}")
-        xs, xb, xr, x8, x8s = None, 0, C, x.codes.data_ptr(), x.scales.data_ptr()
+        xs, xb, xr, x8, x8s = None, 0, C, x._at[0], x._at[1]
     else:
         _activation(x, what, dy.shape, dy.dtype)
         xb, xr = _graph_strides(x, what)
@@ -265,9 +300,8 @@ def group_norm_act_backward(dy: torch.Tensor, x, weight: torch.Tensor | None, bi
             raise _hip.GvaeHipError(f"{what}: mean and rstd must have shape ({B}, {groups}), got {tuple(t.shape)}")
     L, dev = _bind(), dy.device
     dx = torch.empty((B, N, C), dtype=dy.dtype, device=dev)
-    grads = torch.empty((2, C), dtype=torch.float32, device=dev)
-    ws = torch.empty(L.gvae_group_norm_ws_bytes(B, N, C, groups), dtype=torch.uint8, device=dev)
-    dweight, dbias = grads[0], grads[1]
+    dweight, dbias = torch.empty((2, C), dtype=torch.float32, device=dev).unbind(0)
+    ws = _workspace(L.gvae_group_norm_ws_bytes(1, code, B, N, C, groups, kept), dev)
     _hip._check(L.gvae_group_norm_bwd(
         dy.data_ptr(), code, db_, dr_, xs, xb, xr, x8, x8s, live, B, N, C, groups, w, b, mean.data_ptr(),
         rstd.data_ptr(), act_code, dx.data_ptr(), dweight.data_ptr(), dbias.data_ptr(), ws.data_ptr(),
@@ -291,7 +325,7 @@ def linear_wgrad8(dy: torch.Tensor, x8: Checkpoint8) -> tuple[torch.Tensor, torc
     L, dev = _bind(), dy.device
     dw = torch.empty((O, I), dtype=dy.dtype, device=dev)
     db = torch.empty((O,), dtype=dy.dtype, device=dev)
-    ws = torch.empty(L.gvae_linear_wgrad8_ws_bytes(rows, O, I), dtype=torch.uint8, device=dev)
-    _hip._check(L.gvae_linear_wgrad8(dy.data_ptr(), code, ld, x8.codes.data_ptr(), x8.scales.data_ptr(), rows, O, I,
-                                     dw.data_ptr(), db.data_ptr(), ws.data_ptr(), _hip._stream()))
+    ws = _workspace(L.gvae_linear_wgrad8_ws_bytes(rows, O, I), dev)
+    _hip._check(L.gvae_linear_wgrad8(dy.data_ptr(), code, ld, *x8._at, rows, O, I, dw.data_ptr(), db.data_ptr(),
+                                     ws.data_ptr(), _hip._stream()))
     return dw, db

@@ -397,8 +397,9 @@ int gvae_ckpt8_write(const void *d_x, int dtype, int64_t rows, int C, int64_t ro
 int gvae_ckpt8_read(const int8_t *d_codes, const uint8_t *d_scales, int64_t rows, int C, void *d_x, int dtype,
                     int64_t row_stride, void *stream);
 
-/* Bytes of scratch for either call below, whatever the element type. */
-int64_t gvae_group_norm_ws_bytes(int B, int N, int C, int G);
+/* Bytes of scratch that a call below needs for these sizes (backward: 0 gvae_group_norm_fwd, 1
+ * gvae_group_norm_bwd; checkpoints: whether it writes any / reads one); 0 = d_ws may be NULL. */
+int64_t gvae_group_norm_ws_bytes(int backward, int dtype, int B, int N, int C, int G, int checkpoints);
 
 /* y = act(w * (x - mean) / sqrt(var + eps) + b), mean and variance over a graph's live rows and the
  * C/G consecutive channels of a group.

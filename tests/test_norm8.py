@@ -80,7 +80,7 @@ def _norm_fwd(L, x=16, dtype=0, bs=8, rs=8, B=1, N=1, C=8, G=2, act=1, eps=1e-5,
                                  y8, y8s, ws, None)
 
 
-@pytest.mark.parametrize("bad", [dict(x=None), dict(y=None), dict(ws=None), dict(mean=None), dict(dtype=3),
+@pytest.mark.parametrize("bad", [dict(x=None), dict(y=None), dict(ws=None, N=100000), dict(mean=None), dict(dtype=3),
                                  dict(dtype=-1), dict(B=0), dict(N=0), dict(C=0), dict(G=0), dict(G=3), dict(act=4),
                                  dict(act=-1), dict(rs=7), dict(bs=-8), dict(eps=0.0), dict(eps=float("nan")),
                                  dict(eps=float("inf")), dict(x8=16), dict(x8s=16), dict(y8=16), dict(y8s=16)])
@@ -128,7 +128,7 @@ def test_checkpoint_and_wgrad_refusals():
         assert L.gvae_linear_wgrad8(*a, None) == -1, a
         assert b"linear_wgrad8" in L.gvae_last_error()
     assert L.gvae_linear_wgrad8(16, 0, 1 << 21, 16, 16, 4, 1 << 21, 8, 16, 16, 16, None) == -3
-    for n in (L.gvae_group_norm_ws_bytes(0, 1, 1, 1), L.gvae_linear_wgrad8_ws_bytes(0, 1, 1)):
+    for n in (L.gvae_group_norm_ws_bytes(1, 0, 0, 1, 1, 1, 0), L.gvae_group_norm_ws_bytes(0, 0, 1, 1, 3, 2, 0), L.gvae_linear_wgrad8_ws_bytes(0, 1, 1)):
         assert n == 0
 
 
@@ -733,3 +733,69 @@ def test_results_repeat_bit_for_bit():
         first = _layer(ops, *args)
         for _ in range(3):
             assert all(torch.equal(p, q) for p, q in zip(first, _layer(ops, *args)))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1024, 256, 256), (1500, 300, 260), (3001, 515, 387), (70000, 40, 30),
+                                   (20000, 128, 128), (4100, 257, 1000)])
+def test_wgrad_large_tiles_and_many_parts(dtype, shape):
+    """Sizes that take the larger tiles, several of them, and many row ranges: against 64 bits, and
+    small integers exactly."""
+    from graphvae import ops
+    M, O, I = shape
+    g = torch.Generator(device="cuda").manual_seed(M + O)
+    codes = torch.randint(-127, 128, (M, -(-I // 16) * 16), generator=g, device="cuda", dtype=torch.int8)
+    codes[:, I:] = 0
+    c = ops.Checkpoint8(codes, torch.full((M, -(-I // 32)), 127, dtype=torch.uint8, device="cuda"), I)
+    x = codes[:, :I].double()
+    dy = torch.randint(-1, 2, (M, O), generator=g, device="cuda").to(dtype)
+    dw, db = ops.linear_wgrad8(dy, c)
+    want = dy.double().t() @ x
+    assert float(want.abs().max()) < 2 ** 24
+    assert torch.equal(dw, want.float().to(dtype)) and torch.equal(db, dy.double().sum(0).float().to(dtype))
+    scales = torch.randint(120, 130, (M, -(-I // 32)), generator=g, device="cuda", dtype=torch.uint8)
+    c = ops.Checkpoint8(codes, scales, I)
+    x = x * torch.exp2(scales.double() - 127).repeat_interleave(32, 1)[:, :I]
+    dy = torch.randn(M, O, generator=g, device="cuda").to(dtype)
+    dw, db = ops.linear_wgrad8(dy, c)
+    want, mag = dy.double().t() @ x, dy.double().abs().t() @ x.abs()
+    bound = 1.01 * (M + 8) * U32 * mag
+    near = (dw.double() - want).abs() <= half_step(dtype) * want.abs() + bound + subnormal(dtype)
+    # (half ends at 65504, and 65520 or more is an infinity in it, at no finite distance: of the sums over
+    # 70000 rows some are; within `bound` of that border either answer is right)
+    beyond = (want.abs() + bound >= 65520.0) & (dtype == torch.float16)
+    assert near[~beyond].all()
+    sure = beyond & (want.abs() - bound >= 65520.0)
+    assert torch.equal(dw[sure], want.to(dtype)[sure]) and (dw[beyond].abs() >= 65504.0 - 2 * bound[beyond]).all()
+    sb = dy.double().sum(0)
+    assert ((db.double() - sb).abs() <= half_step(dtype) * sb.abs() + 1.01 * (M + 8) * U32 * dy.double().abs().sum(0)
+            + subnormal(dtype)).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(200, 400, 64, 4), (40, 1000, 96, 6), (2, 70000, 32, 4), (1200, 9, 40, 8),
+                                   (1100, 3, 5, 5), (9, 4000, 45, 9), (130, 600, 33, 1)])
+def test_group_norm_forms(dtype, shape):
+    """Sizes around the resident and the split form's borders, forward and backward, from the tensor and
+    from its checkpoint."""
+    from graphvae import ops
+    B, N, C, G = shape
+    x, w, b, rows, dy = make_x(B, N, C, dtype, C)
+    live = torch.arange(N)[None, :, None] < rows[:, None, None]
+    x = torch.where(live, x, torch.zeros_like(x))
+    r = ops.group_norm_act(x.cuda(), w.cuda(), b.cuda(), G, act="silu", rows=rows.cuda(), keep_x=True, keep_y=True)
+    y, mean, rstd, tol, dmean, drel = norm_ref(x, w, b, G, "silu", 1e-5, rows)
+    assert ((r.y.cpu().double() - y).abs() <= half_step(dtype) * y.abs() + 1.01 * tol + subnormal(dtype)).all()
+    assert ((r.mean.cpu().double() - mean).abs() <= dmean + 2 * U32 * mean.abs()).all()
+    assert ((r.rstd.cpu().double() / rstd - 1).abs() <= drel + 4 * U32).all()
+    for got, src in ((r.x8, x.cuda()), (r.y8, r.y)):
+        c = ops.checkpoint8(src)
+        assert torch.equal(c.codes, got.codes) and torch.equal(c.scales, got.scales)
+    for arg, used in ((x.cuda(), x), (r.x8, r.x8.read(torch.float32).cpu())):
+        got = ops.group_norm_act_backward(dy.cuda(), arg, w.cuda(), b.cuda(), r.mean, r.rstd, G, act="silu",
+                                          rows=rows.cuda())
+        dx, dw, db, edx, edw, edb = bwd_ref(dy, used, w, b, r.mean.cpu(), r.rstd.cpu(), G, "silu", rows)
+        assert ((got[0].cpu().double() - dx).abs() <= half_step(dtype) * dx.abs() + 1.01 * edx + subnormal(dtype)).all()
+        assert ((got[1].cpu().double() - dw).abs() <= 2 * edw).all() and ((got[2].cpu().double() - db).abs() <= 2 * edb).all()
