@@ -419,6 +419,104 @@ int launch_colsum(const float *M, int rows, int cols, int64_t ld, float *out, in
   return check_launch("colsum");
 }
 
+// partial column sums of a range of rows: 64 columns x 4 row lanes per work-group
+__global__ __launch_bounds__(256) void colsum_rows_kernel(const float *__restrict__ M, int64_t rows, int cols,
+                                                          int64_t part_rows, float *__restrict__ part) {
+  __shared__ float sh[4][64];
+  const int cl = threadIdx.x & 63, rl = threadIdx.x >> 6, c = blockIdx.x * 64 + cl;
+  const int64_t r0 = (int64_t)blockIdx.y * part_rows, r1 = r0 + part_rows < rows ? r0 + part_rows : rows;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  if (c < cols) {
+    int64_t r = r0 + rl;
+    for (; r + 12 < r1; r += 16)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s[u] += M[(r + 4 * u) * cols + c];
+    for (; r < r1; r += 4) s[0] += M[r * cols + c];
+  }
+  sh[rl][cl] = (s[0] + s[1]) + (s[2] + s[3]);
+  __syncthreads();
+  if (rl == 0 && c < cols)
+    part[(int64_t)blockIdx.y * cols + c] = (sh[0][cl] + sh[1][cl]) + (sh[2][cl] + sh[3][cl]);
+}
+
+int launch_colsum_rows(const float *M, int64_t rows, int cols, float *part, int parts, float *out,
+                       hipStream_t s) {
+  const int64_t part_rows = (rows + parts - 1) / parts < 16 ? 16 : (rows + parts - 1) / parts;
+  const int n = (int)((rows + part_rows - 1) / part_rows);
+  hipLaunchKernelGGL(colsum_rows_kernel, dim3(ceil_div(cols, 64), n), dim3(256), 0, s, M, rows, cols, part_rows,
+                     part);
+  return launch_colsum(part, n, cols, cols, out, 0, s);
+}
+
+// ---------------------------------------------------------------------------
+// Pieces of the forward for an encoder whose layers are launches of their own (group norm).
+// ---------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void gcn_adjacency_kernel(const float *__restrict__ adj,
+                                                            const int32_t *__restrict__ n_x,
+                                                            const int32_t *__restrict__ Rarr, int N,
+                                                            float *__restrict__ Ahat) {
+  __shared__ double dinv[1024];
+  const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int nx = n_x[g], R = Rarr[g];
+  const float *A = adj + (int64_t)g * N * N;
+  for (int i = tid >> 6; i < N; i += 4) {       // a wavefront per row
+    int cnt = 0;
+    if (i < R)
+      for (int j = lane; j < R; j += 64) cnt += (j != i && A[(int64_t)i * N + j] != 0.0f) ? 1 : 0;
+    for (int off = 32; off > 0; off >>= 1) cnt += __shfl_xor(cnt, off, 64);
+    if (lane == 0) dinv[i] = (i < nx) ? 1.0 / sqrt(1.0 + (double)cnt) : 0.0;
+  }
+  __syncthreads();
+  float *O = Ahat + (int64_t)g * N * N;
+  for (int e = tid; e < N * N; e += 256) {
+    const int i = e / N, k = e - i * N;
+    const bool edge = i < nx && k < nx && (i == k || (i < R && k < R && A[e] != 0.0f));
+    O[e] = edge ? (float)(dinv[i] * dinv[k]) : 0.0f;
+  }
+}
+
+int launch_gcn_adjacency(const float *adj, const int32_t *n_x, const int32_t *R, int B, int N,
+                         float *Ahat, hipStream_t s) {
+  GVAE_REQUIRE(N <= 1024, GVAE_ELIMIT, "gcn_adjacency: N=%d", N);
+  hipLaunchKernelGGL(gcn_adjacency_kernel, dim3(B), dim3(256), 0, s, adj, n_x, R, N, Ahat);
+  return check_launch("gcn_adjacency");
+}
+
+__global__ __launch_bounds__(256) void pool_fwd_kernel(const float *__restrict__ act,
+                                                       const int32_t *__restrict__ n_x,
+                                                       const int32_t *__restrict__ Rarr, int N, int H,
+                                                       float *__restrict__ gvec) {
+  __shared__ double sh[4][64];
+  const int cl = threadIdx.x & 63, rl = threadIdx.x >> 6, c = blockIdx.x * 64 + cl, g = blockIdx.y;
+  const int nx = n_x[g];
+  double s = 0.0;
+  if (c < H)
+    for (int i = rl; i < nx; i += 4) s += act[((int64_t)g * N + i) * H + c];
+  sh[rl][cl] = s;
+  __syncthreads();
+  if (rl == 0 && c < H)
+    gvec[(int64_t)g * H + c] = (float)(((sh[0][cl] + sh[1][cl]) + (sh[2][cl] + sh[3][cl])) / (double)Rarr[g]);
+}
+
+int launch_pool_fwd(const float *Hact, const int32_t *n_x, const int32_t *R, int B, int N, int H,
+                    float *gvec, hipStream_t s) {
+  hipLaunchKernelGGL(pool_fwd_kernel, dim3(ceil_div(H, 64), B), dim3(256), 0, s, Hact, n_x, R, N, H, gvec);
+  return check_launch("pool_fwd");
+}
+
+__global__ void reparam_fwd_kernel(const float *__restrict__ mu, const float *__restrict__ lvraw,
+                                   const float *__restrict__ eps, int n, float *__restrict__ z) {
+  const int e = blockIdx.x * blockDim.x + threadIdx.x;
+  if (e >= n) return;
+  z[e] = mu[e] + eps[e] * expf(0.5f * fminf(fmaxf(lvraw[e], -4.0f), 4.0f));
+}
+
+int launch_reparam_fwd(const float *mu, const float *lvraw, const float *eps, int B, int Z, float *z,
+                       hipStream_t s) {
+  hipLaunchKernelGGL(reparam_fwd_kernel, dim3(ceil_div(B * Z, 256)), dim3(256), 0, s, mu, lvraw, eps, B * Z, z);
+  return check_launch("reparam_fwd");
+}
+
 __global__ __launch_bounds__(256) void pool_bwd_kernel(const float *__restrict__ dgvec,
                                                        const int32_t *__restrict__ n_x,
                                                        const int32_t *__restrict__ Rarr, int N, int H,

@@ -112,6 +112,20 @@ struct ColsumGroup {
   }
 };
 int launch_colsum_group(const ColsumGroup &g, hipStream_t s);
+// the same for matrices of many rows: at most `parts` partial rows in `part` (parts x cols floats), then
+// their sum; fixed order
+int launch_colsum_rows(const float *M, int64_t rows, int cols, float *part, int parts, float *out,
+                       hipStream_t s);
+// D^-1/2 (A + I) D^-1/2 over a graph's n_x live rows (edges among its R real nodes), zero elsewhere:
+// the dense form of GCNConv's normalisation (graphvae/models/model.py:72,75)
+int launch_gcn_adjacency(const float *adj, const int32_t *n_x, const int32_t *R, int B, int N,
+                         float *Ahat, hipStream_t s);
+// gvec = sum of a graph's live rows / R (model.py:297), and z = mu + eps * exp(logvar / 2), logvar clamped
+// (model.py:298-300), for encoders whose layers run as launches of their own
+int launch_pool_fwd(const float *Hact, const int32_t *n_x, const int32_t *R, int B, int N, int H,
+                    float *gvec, hipStream_t s);
+int launch_reparam_fwd(const float *mu, const float *lvraw, const float *eps, int B, int Z, float *z,
+                       hipStream_t s);
 int launch_pool_bwd(const float *dgvec, const int32_t *n_x, const int32_t *R, int B, int N, int H,
                     float *dH, hipStream_t s);
 // dmu, dlvraw from dz and the KL term (coefficient c_kl / B per graph)

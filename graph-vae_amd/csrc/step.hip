@@ -7,6 +7,8 @@
 // (loss weighting, clipping, Adam).
 #include "gvae_dense.h"
 
+#include <cmath>
+
 namespace gvae {
 
 static inline int64_t align4(int64_t n) { return (n + 3) & ~(int64_t)3; }
@@ -39,6 +41,13 @@ struct Workspace {
   float *dgam_p, *dbet_p, *dbias_p;
   // the per-graph backward keeps both layers' results until the batch-wide sums that follow it
   float *dH0_2, *dgam_p2, *dbet_p2, *dbias_p2;
+  // group norm: three activations in transit, what the forward keeps for the backward (fp32 or 8-bit
+  // checkpoints), statistics, scratch of the operators
+  float *T0, *T1, *T2, *rstd1, *rstd2;
+  int8_t *Y1q, *H1q, *Y2q;
+  uint8_t *Y1s, *H1s, *Y2s;
+  void *op_ws;
+  float *colsum_part;
   float *splitk;
   int64_t splitk_floats;
   int32_t *status;
@@ -54,21 +63,21 @@ struct Workspace {
 
 static const int kMaxSplits = 64;
 
-static Workspace carve(const gvae_dims *d, int B, char *base) {
+constexpr int kColsumParts = 128;
+
+// `gn`: the encoder normalises by groups.  Everything the matching, the losses and the heads use
+// comes first and lies alike for either norm (gvae_step_forward_match_loss need not know which).
+static Workspace carve(const gvae_dims *d, int B, char *base, const gvae_gn_opts *gn = nullptr) {
   const int64_t F = d->F, H = d->H, Z = d->Z, N = d->N, U = N * (N - 1) / 2;
-  (void)F;
   Workspace w{};
   int64_t off = 0;
-  auto take = [&](int64_t nfloat) {
-    float *p = reinterpret_cast<float *>(base + off);
-    off += (nfloat * 4 + 255) & ~(int64_t)255;
+  auto take_bytes = [&](int64_t bytes) {
+    char *p = base + off;
+    off += (bytes + 255) & ~(int64_t)255;
     return p;
   };
+  auto take = [&](int64_t nfloat) { return reinterpret_cast<float *>(take_bytes(nfloat * 4)); };
   const int64_t BNH = (int64_t)B * N * H, BNN = (int64_t)B * N * N, BH = (int64_t)B * H;
-  w.Ahat = take(BNN); w.H0a = take(BNH); w.Y1 = take(BNH); w.H1 = take(BNH);
-  w.H0b = take(BNH); w.Y2 = take(BNH); w.H2 = take(BNH);
-  w.mean1 = take(BH); w.invstd1 = take(BH); w.varu1 = take(BH);
-  w.mean2 = take(BH); w.invstd2 = take(BH); w.varu2 = take(BH);
   w.gvec = take(BH); w.mu = take((int64_t)B * Z); w.lvraw = take((int64_t)B * Z);
   w.z = take((int64_t)B * Z); w.he = take(BH); w.hn = take(BH);
   w.vec = take((int64_t)B * U); w.node = take((int64_t)B * N);
@@ -77,9 +86,6 @@ static Workspace carve(const gvae_dims *d, int B, char *base) {
   w.dvec = take((int64_t)B * U); w.dnode = take((int64_t)B * N);
   w.dhe = take(BH); w.dhn = take(BH); w.dz = take((int64_t)B * Z);
   w.dmu = take((int64_t)B * Z); w.dlv = take((int64_t)B * Z); w.dgvec = take(BH);
-  w.dAct = take(BNH); w.dY = take(BNH); w.dH0 = take(BNH);
-  w.dgam_p = take(BH); w.dbet_p = take(BH); w.dbias_p = take(BH);
-  w.dH0_2 = take(BNH); w.dgam_p2 = take(BH); w.dbet_p2 = take(BH); w.dbias_p2 = take(BH);
   // split-K partials: splits <= ceil(512 / tiles) and tiles >= M*N/4096, so
   // splits*M*N <= 512*4096 + M*N for every GEMM that is split
   int64_t mn = U * H;
@@ -93,6 +99,38 @@ static Workspace carve(const gvae_dims *d, int B, char *base) {
   w.pw_i = take(B);
   w.perm_fwd = reinterpret_cast<int64_t *>(take(2 * (int64_t)B * N));
   w.mpm_ws = reinterpret_cast<char *>(take((gvae_mpm_stream_ws_bytes(B, (int)N) + 3) / 4));
+  w.Ahat = take(BNN);
+  if (!gn) {
+    w.H0a = take(BNH); w.Y1 = take(BNH); w.H1 = take(BNH);
+    w.H0b = take(BNH); w.Y2 = take(BNH); w.H2 = take(BNH);
+    w.mean1 = take(BH); w.invstd1 = take(BH); w.varu1 = take(BH);
+    w.mean2 = take(BH); w.invstd2 = take(BH); w.varu2 = take(BH);
+    // (dAct + dY and dH0 .. dH0_2 also hold the forward's fp64 activations: contiguous runs)
+    w.dAct = take(BNH); w.dY = take(BNH); w.dH0 = take(BNH);
+    w.dgam_p = take(BH); w.dbet_p = take(BH); w.dbias_p = take(BH);
+    w.dH0_2 = take(BNH); w.dgam_p2 = take(BH); w.dbet_p2 = take(BH); w.dbias_p2 = take(BH);
+    w.bytes = off;
+    return w;
+  }
+  const int64_t BN = (int64_t)B * N, G = gn->groups;
+  w.T0 = take(BNH); w.T1 = take(BNH); w.T2 = take(BNH);
+  if (gn->act_bits == 8) {
+    const int64_t ld = gvae_ckpt8_row_bytes((int)H), nb = gvae_ckpt8_row_scales((int)H);
+    w.Y1q = (int8_t *)take_bytes(BN * ld); w.Y1s = (uint8_t *)take_bytes(BN * nb);
+    w.H1q = (int8_t *)take_bytes(BN * ld); w.H1s = (uint8_t *)take_bytes(BN * nb);
+    w.Y2q = (int8_t *)take_bytes(BN * ld); w.Y2s = (uint8_t *)take_bytes(BN * nb);
+  } else {
+    w.Y1 = take(BNH); w.H1 = take(BNH); w.Y2 = take(BNH);
+  }
+  w.mean1 = take(B * G); w.rstd1 = take(B * G); w.mean2 = take(B * G); w.rstd2 = take(B * G);
+  int64_t op = 0;
+  for (int k = 0; k < 4; ++k) {
+    const int64_t n = gvae_group_norm_ws_bytes(k & 1, GVAE_F32, B, (int)N, (int)H, gn->groups, k >> 1);
+    op = n > op ? n : op;
+  }
+  const int64_t wg = gvae_linear_wgrad8_ws_bytes(BN, (int)H, (int)H);
+  w.op_ws = take_bytes(op > wg ? op : wg);
+  w.colsum_part = take((int64_t)kColsumParts * H);
   w.bytes = off;
   return w;
 }
@@ -163,9 +201,11 @@ static int linear_bwd_weight(const float *dC, const float *A, int64_t lda, float
                              int K, float *splitk, hipStream_t s) {
   return launch_gemm(desc_linear_bwd_weight(dC, A, lda, dW, M, N, K, splitk), s);
 }
-// Y[b] (N x H) = Ahat[b] (N x N) * X[b] (N x H)
-static int aggregate(const float *Ahat, const float *X, float *Y, int B, int N, int H, hipStream_t s) {
+// Y[b] (N x H) = Ahat[b] (N x N) * X[b] (N x H) [+ bias]
+static int aggregate(const float *Ahat, const float *X, float *Y, int B, int N, int H, hipStream_t s,
+                     const float *bias = nullptr) {
   GemmDesc g;
+  g.bias = bias;
   g.A = Ahat; g.a_rs = N; g.a_cs = 1; g.a_bs = (int64_t)N * N;
   g.B = X; g.b_rs = H; g.b_cs = 1; g.b_bs = (int64_t)N * H;
   g.C = Y; g.c_rs = H; g.c_bs = (int64_t)N * H;
@@ -539,6 +579,75 @@ int gvae_step_forward_match_loss(const gvae_dims *d, const float *d_adj, const i
   return check_launch("step_forward_match_loss");
 }
 
+// Gradients of the losses down to the decoder's hidden layers (masked by their ReLUs), with the second
+// decoder layers' weight gradients.
+static int backward_decoder(const gvae_dims *d, const Workspace &w, const Params &P, const int64_t *off,
+                            const float *d_adj, const int32_t *d_R, const float *d_pos_weight, int loss_variant,
+                            float c_rec, const float *d_up, int B, float *d_grads, hipStream_t s) {
+  const int H = d->H, N = d->N, U = N * (N - 1) / 2;
+  auto G = [&](int i) { return d_grads + off[i]; };
+  if (loss_variant == GVAE_LOSS_INDIVIDUAL_RHO)
+    TRY(launch_loss_bwd_indiv(w.vec, d_adj, d_R, w.perm_fwd, w.pw_i, B, N, c_rec, d_up, w.dvec,
+                              w.dnode, s));
+  else
+    TRY(launch_loss_bwd(w.vec, w.node, d_adj, d_R, B, N, d_pos_weight,
+                        loss_variant == GVAE_LOSS_DUMMY_MASKED, c_rec, d_up, w.dvec, w.dnode, s));
+  // edge and node heads, layer by layer: the four contractions of a layer are independent
+  {
+    GemmDesc l2[4] = {
+        desc_linear_bwd_weight(w.dvec, w.he, H, G(GVAE_P_DE2_W), B, U, H, nullptr),
+        desc_linear_bwd_input(w.dvec, P.p[GVAE_P_DE2_W], w.dhe, B, U, H, 0, nullptr),
+        desc_linear_bwd_weight(w.dnode, w.hn, H, G(GVAE_P_DN2_W), B, N, H, nullptr),
+        desc_linear_bwd_input(w.dnode, P.p[GVAE_P_DN2_W], w.dhn, B, N, H, 0, nullptr)};
+    l2[1].relu_mask_act = w.he;   // backward of the hidden ReLUs, in the contraction's epilogue
+    l2[3].relu_mask_act = w.hn;
+    TRY(launch_gemm_group(l2, 4, w.splitk, w.splitk_floats, s));
+  }
+  return 0;
+}
+
+// Gradients from the decoder's hidden layers to the pooled vector (dgvec), kernel by kernel, with those of
+// the first decoder layers and the two heads, and the decoder's bias gradients.
+static int backward_heads(const gvae_dims *d, const Workspace &w, const Params &P, const int64_t *off,
+                          const float *d_eps, const float *d_up, float c_kl, int B, float *d_grads, hipStream_t s) {
+  const int H = d->H, Z = d->Z, N = d->N, U = N * (N - 1) / 2;
+  auto G = [&](int i) { return d_grads + off[i]; };
+  {
+    ColsumGroup cs;   // the four bias gradients of the two heads
+    cs.add(w.dvec, B, U, U, G(GVAE_P_DE2_B));
+    cs.add(w.dnode, B, N, N, G(GVAE_P_DN2_B));
+    cs.add(w.dhe, B, H, H, G(GVAE_P_DE1_B));
+    cs.add(w.dhn, B, H, H, G(GVAE_P_DN1_B));
+    TRY(launch_colsum_group(cs, s));
+  }
+  {
+    GemmDesc l1[3] = {
+        desc_linear_bwd_weight(w.dhe, w.z, Z, G(GVAE_P_DE1_W), B, H, Z, nullptr),
+        desc_linear_bwd_weight(w.dhn, w.z, Z, G(GVAE_P_DN1_W), B, H, Z, nullptr),
+        desc_linear_bwd_input(w.dhe, P.p[GVAE_P_DE1_W], w.dz, B, H, Z, 0, nullptr)};
+    TRY(launch_gemm_group(l1, 3, w.splitk, w.splitk_floats, s));
+  }
+  // dz = edge-head term + node-head term, in this order
+  TRY(linear_bwd_input(w.dhn, P.p[GVAE_P_DN1_W], w.dz, B, H, Z, 1, w.splitk, s));
+  // reparameterisation + KL
+  TRY(launch_reparam_bwd(w.dz, w.mu, w.lvraw, d_eps, B, Z, c_kl, d_up, w.dmu, w.dlv, s));
+  {
+    GemmDesc hd[3] = {
+        desc_linear_bwd_weight(w.dmu, w.gvec, H, G(GVAE_P_MU_W), B, Z, H, nullptr),
+        desc_linear_bwd_weight(w.dlv, w.gvec, H, G(GVAE_P_LV_W), B, Z, H, nullptr),
+        desc_linear_bwd_input(w.dmu, P.p[GVAE_P_MU_W], w.dgvec, B, Z, H, 0, nullptr)};
+    TRY(launch_gemm_group(hd, 3, w.splitk, w.splitk_floats, s));
+  }
+  {
+    ColsumGroup cs;
+    cs.add(w.dmu, B, Z, Z, G(GVAE_P_MU_B));
+    cs.add(w.dlv, B, Z, Z, G(GVAE_P_LV_B));
+    TRY(launch_colsum_group(cs, s));
+  }
+  TRY(linear_bwd_input(w.dlv, P.p[GVAE_P_LV_W], w.dgvec, B, Z, H, 1, w.splitk, s));
+  return 0;
+}
+
 int gvae_step_backward(const gvae_dims *d, const float *d_params, const float *d_x,
                        const float *d_adj, const int32_t *d_n_x, const int32_t *d_R, int n_graphs,
                        const float *d_eps, const float *d_pos_weight, int loss_variant, float c_rec,
@@ -558,23 +667,7 @@ int gvae_step_backward(const gvae_dims *d, const float *d_params, const float *d
   param_layout(d, off, nullptr);
   auto G = [&](int i) { return d_grads + off[i]; };
 
-  if (loss_variant == GVAE_LOSS_INDIVIDUAL_RHO)
-    TRY(launch_loss_bwd_indiv(w.vec, d_adj, d_R, w.perm_fwd, w.pw_i, B, N, c_rec, d_up, w.dvec,
-                              w.dnode, s));
-  else
-    TRY(launch_loss_bwd(w.vec, w.node, d_adj, d_R, B, N, d_pos_weight,
-                        loss_variant == GVAE_LOSS_DUMMY_MASKED, c_rec, d_up, w.dvec, w.dnode, s));
-  // edge and node heads, layer by layer: the four contractions of a layer are independent
-  {
-    GemmDesc l2[4] = {
-        desc_linear_bwd_weight(w.dvec, w.he, H, G(GVAE_P_DE2_W), B, U, H, nullptr),
-        desc_linear_bwd_input(w.dvec, P.p[GVAE_P_DE2_W], w.dhe, B, U, H, 0, nullptr),
-        desc_linear_bwd_weight(w.dnode, w.hn, H, G(GVAE_P_DN2_W), B, N, H, nullptr),
-        desc_linear_bwd_input(w.dnode, P.p[GVAE_P_DN2_W], w.dhn, B, N, H, 0, nullptr)};
-    l2[1].relu_mask_act = w.he;   // backward of the hidden ReLUs, in the contraction's epilogue
-    l2[3].relu_mask_act = w.hn;
-    TRY(launch_gemm_group(l2, 4, w.splitk, w.splitk_floats, s));
-  }
+  TRY(backward_decoder(d, w, P, off, d_adj, d_R, d_pos_weight, loss_variant, c_rec, d_up, B, d_grads, s));
   if (model_chain_resident(N, H, Z)) {
     // the per-graph part of the chain in one launch, then everything that is summed over the
     // batch: six weight gradients as one group, twelve column sums as another
@@ -618,39 +711,7 @@ int gvae_step_backward(const gvae_dims *d, const float *d_params, const float *d
     TRY(launch_colsum_group(cs, s));
     return check_launch("step_backward");
   }
-  {
-    ColsumGroup cs;   // the four bias gradients of the two heads
-    cs.add(w.dvec, B, U, U, G(GVAE_P_DE2_B));
-    cs.add(w.dnode, B, N, N, G(GVAE_P_DN2_B));
-    cs.add(w.dhe, B, H, H, G(GVAE_P_DE1_B));
-    cs.add(w.dhn, B, H, H, G(GVAE_P_DN1_B));
-    TRY(launch_colsum_group(cs, s));
-  }
-  {
-    GemmDesc l1[3] = {
-        desc_linear_bwd_weight(w.dhe, w.z, Z, G(GVAE_P_DE1_W), B, H, Z, nullptr),
-        desc_linear_bwd_weight(w.dhn, w.z, Z, G(GVAE_P_DN1_W), B, H, Z, nullptr),
-        desc_linear_bwd_input(w.dhe, P.p[GVAE_P_DE1_W], w.dz, B, H, Z, 0, nullptr)};
-    TRY(launch_gemm_group(l1, 3, w.splitk, w.splitk_floats, s));
-  }
-  // dz = edge-head term + node-head term, in this order
-  TRY(linear_bwd_input(w.dhn, P.p[GVAE_P_DN1_W], w.dz, B, H, Z, 1, w.splitk, s));
-  // reparameterisation + KL
-  TRY(launch_reparam_bwd(w.dz, w.mu, w.lvraw, d_eps, B, Z, c_kl, d_up, w.dmu, w.dlv, s));
-  {
-    GemmDesc hd[3] = {
-        desc_linear_bwd_weight(w.dmu, w.gvec, H, G(GVAE_P_MU_W), B, Z, H, nullptr),
-        desc_linear_bwd_weight(w.dlv, w.gvec, H, G(GVAE_P_LV_W), B, Z, H, nullptr),
-        desc_linear_bwd_input(w.dmu, P.p[GVAE_P_MU_W], w.dgvec, B, Z, H, 0, nullptr)};
-    TRY(launch_gemm_group(hd, 3, w.splitk, w.splitk_floats, s));
-  }
-  {
-    ColsumGroup cs;
-    cs.add(w.dmu, B, Z, Z, G(GVAE_P_MU_B));
-    cs.add(w.dlv, B, Z, Z, G(GVAE_P_LV_B));
-    TRY(launch_colsum_group(cs, s));
-  }
-  TRY(linear_bwd_input(w.dlv, P.p[GVAE_P_LV_W], w.dgvec, B, Z, H, 1, w.splitk, s));
+  TRY(backward_heads(d, w, P, off, d_eps, d_up, c_kl, B, d_grads, s));
   // encoder layer 2
   TRY(launch_pool_bwd(w.dgvec, d_n_x, d_R, B, N, H, w.dAct, s));
   TRY(launch_bn_relu_bwd(w.dAct, w.Y2, P.p[GVAE_P_CONV2_B], w.H2, P.p[GVAE_P_BN2_W], w.mean2,
@@ -682,6 +743,111 @@ int gvae_step_backward(const gvae_dims *d, const float *d_params, const float *d
   TRY(aggregate(w.Ahat, w.dY, w.dH0, B, N, H, s));
   TRY(linear_bwd_weight(w.dH0, d_x, F, G(GVAE_P_CONV1_W), B * N, H, F, w.splitk, s));
   return check_launch("step_backward");
+}
+
+// --------------------------------------------------------------------------- group norm in the encoder
+static int check_gn(const gvae_dims *d, const gvae_gn_opts *gn, const char *who) {
+  GVAE_REQUIRE(d && gn && d->F > 0 && d->H > 0 && d->Z > 0 && d->N >= 2 && d->N <= 1024, GVAE_EINVAL,
+               "%s: bad dimensions", who);
+  GVAE_REQUIRE(gn->groups > 0 && d->H % gn->groups == 0, GVAE_EINVAL, "%s: %d channels do not divide into %d groups",
+               who, d->H, gn->groups);
+  GVAE_REQUIRE(gn->act_bits == 8 || gn->act_bits == 32, GVAE_EINVAL, "%s: activations are kept in 8 or 32 bits, not %d",
+               who, gn->act_bits);
+  GVAE_REQUIRE(gn->eps > 0.0f && std::isfinite(gn->eps), GVAE_EINVAL, "%s: eps must be positive", who);
+  return 0;
+}
+
+int64_t gvae_step_gn_ws_bytes(const gvae_dims *d, const gvae_gn_opts *gn, int n_graphs) {
+  if (n_graphs <= 0 || check_gn(d, gn, "step_gn_ws_bytes")) return 0;
+  return carve(d, n_graphs, nullptr, gn).bytes;
+}
+
+int gvae_step_gn_forward_model(const gvae_dims *d, const gvae_gn_opts *gn, const float *d_params, const float *d_x,
+                               const float *d_adj, const int32_t *d_n_x, const int32_t *d_R, int n_graphs,
+                               const float *d_eps, void *d_ws, void *stream) {
+  GVAE_REQUIRE(d_params && d_x && d_adj && d_n_x && d_R && d_eps && d_ws, GVAE_EINVAL,
+               "step_gn_forward_model: null pointer");
+  TRY(check_gn(d, gn, "step_gn_forward_model"));
+  GVAE_REQUIRE(n_graphs > 0 && n_graphs <= 65535, GVAE_EINVAL, "step_gn_forward_model: bad n_graphs=%d", n_graphs);
+  hipStream_t s = (hipStream_t)stream;
+  const int B = n_graphs, F = d->F, H = d->H, Z = d->Z, N = d->N, U = N * (N - 1) / 2;
+  const Workspace w = carve(d, B, (char *)d_ws, gn);
+  const Params P = bind(d, d_params);
+  const bool kept8 = gn->act_bits == 8;
+  // one layer: Y = Ahat (A W^T) + bias, out = relu(group norm(Y)); what the backward needs is left in 8 bits or
+  // as it is (Y and, for the next layer's weight gradient, the output)
+  auto layer = [&](const float *A, int K, int pw, int pb, int pg, int pbe, float *lin, float *Y, float *out,
+                   float *mean, float *rstd, int8_t *Yq, uint8_t *Ys, int8_t *Oq, uint8_t *Os) -> int {
+    TRY(linear_fwd(A, K, P.p[pw], nullptr, lin, B * N, H, K, 0, s));
+    TRY(aggregate(w.Ahat, lin, Y, B, N, H, s, P.p[pb]));
+    return gvae_group_norm_fwd(Y, GVAE_F32, (int64_t)N * H, H, d_n_x, B, N, H, gn->groups, P.p[pg], P.p[pbe], gn->eps,
+                               GVAE_ACT_RELU, out, mean, rstd, Yq, Ys, Oq, Os, w.op_ws, s);
+  };
+  TRY(launch_gcn_adjacency(d_adj, d_n_x, d_R, B, N, w.Ahat, s));
+  float *H1 = kept8 ? w.T0 : w.H1;
+  TRY(layer(d_x, F, GVAE_P_CONV1_W, GVAE_P_CONV1_B, GVAE_P_BN1_W, GVAE_P_BN1_B, w.T0, kept8 ? w.T1 : w.Y1, H1, w.mean1,
+            w.rstd1, w.Y1q, w.Y1s, w.H1q, w.H1s));
+  TRY(layer(H1, H, GVAE_P_CONV2_W, GVAE_P_CONV2_B, GVAE_P_BN2_W, GVAE_P_BN2_B, w.T2, kept8 ? w.T1 : w.Y2, w.T0, w.mean2,
+            w.rstd2, w.Y2q, w.Y2s, nullptr, nullptr));
+  TRY(launch_pool_fwd(w.T0, d_n_x, d_R, B, N, H, w.gvec, s));
+  {
+    GemmDesc hd[2] = {desc_linear_fwd(w.gvec, H, P.p[GVAE_P_MU_W], P.p[GVAE_P_MU_B], w.mu, B, Z, H, 0),
+                      desc_linear_fwd(w.gvec, H, P.p[GVAE_P_LV_W], P.p[GVAE_P_LV_B], w.lvraw, B, Z, H, 0)};
+    TRY(launch_gemm_group(hd, 2, w.splitk, w.splitk_floats, s));
+  }
+  TRY(launch_reparam_fwd(w.mu, w.lvraw, d_eps, B, Z, w.z, s));
+  {
+    GemmDesc l1[2] = {desc_linear_fwd(w.z, Z, P.p[GVAE_P_DE1_W], P.p[GVAE_P_DE1_B], w.he, B, H, Z, 1),
+                      desc_linear_fwd(w.z, Z, P.p[GVAE_P_DN1_W], P.p[GVAE_P_DN1_B], w.hn, B, H, Z, 1)};
+    TRY(launch_gemm_group(l1, 2, w.splitk, w.splitk_floats, s));
+    GemmDesc l2[2] = {desc_linear_fwd(w.he, H, P.p[GVAE_P_DE2_W], P.p[GVAE_P_DE2_B], w.vec, B, U, H, 0),
+                      desc_linear_fwd(w.hn, H, P.p[GVAE_P_DN2_W], P.p[GVAE_P_DN2_B], w.node, B, N, H, 0)};
+    TRY(launch_gemm_group(l2, 2, w.splitk, w.splitk_floats, s));
+  }
+  return check_launch("step_gn_forward_model");
+}
+
+int gvae_step_gn_backward(const gvae_dims *d, const gvae_gn_opts *gn, const float *d_params, const float *d_x,
+                          const float *d_adj, const int32_t *d_n_x, const int32_t *d_R, int n_graphs,
+                          const float *d_eps, const float *d_pos_weight, int loss_variant, float c_rec, float c_kl,
+                          const float *d_up, void *d_ws, float *d_grads, void *stream) {
+  GVAE_REQUIRE(d_params && d_x && d_adj && d_n_x && d_R && d_eps && d_pos_weight && d_ws && d_grads, GVAE_EINVAL,
+               "step_gn_backward: null pointer");
+  TRY(check_gn(d, gn, "step_gn_backward"));
+  GVAE_REQUIRE(n_graphs > 0 && n_graphs <= 65535, GVAE_EINVAL, "step_gn_backward: bad n_graphs=%d", n_graphs);
+  GVAE_REQUIRE(loss_variant >= GVAE_LOSS_CURRENT && loss_variant <= GVAE_LOSS_INDIVIDUAL_RHO, GVAE_EINVAL,
+               "step_gn_backward: unknown loss variant %d", loss_variant);
+  hipStream_t s = (hipStream_t)stream;
+  const int B = n_graphs, F = d->F, H = d->H, N = d->N;
+  const Workspace w = carve(d, B, (char *)d_ws, gn);
+  const Params P = bind(d, d_params);
+  int64_t off[GVAE_P_COUNT];
+  param_layout(d, off, nullptr);
+  auto G = [&](int i) { return d_grads + off[i]; };
+  const bool kept8 = gn->act_bits == 8;
+  TRY(backward_decoder(d, w, P, off, d_adj, d_R, d_pos_weight, loss_variant, c_rec, d_up, B, d_grads, s));
+  TRY(backward_heads(d, w, P, off, d_eps, d_up, c_kl, B, d_grads, s));
+  TRY(launch_pool_bwd(w.dgvec, d_n_x, d_R, B, N, H, w.T0, s));
+  // from T0 = gradient of a layer's output to T2 = gradient of its linear part (Ahat is symmetric), with the
+  // gradients of the norm's parameters and of the layer's bias (column sums of the norm's input gradient)
+  auto layer = [&](const float *Y, const int8_t *Yq, const uint8_t *Ys, const float *mean, const float *rstd, int pg,
+                   int pbe, int pb) -> int {
+    TRY(gvae_group_norm_bwd(w.T0, GVAE_F32, (int64_t)N * H, H, kept8 ? nullptr : Y, (int64_t)N * H, H, Yq, Ys, d_n_x, B,
+                            N, H, gn->groups, P.p[pg], P.p[pbe], mean, rstd, GVAE_ACT_RELU, w.T1, G(pg), G(pbe),
+                            w.op_ws, s));
+    TRY(launch_colsum_rows(w.T1, (int64_t)B * N, H, w.colsum_part, kColsumParts, G(pb), s));
+    return aggregate(w.Ahat, w.T1, w.T2, B, N, H, s);
+  };
+  TRY(layer(w.Y2, w.Y2q, w.Y2s, w.mean2, w.rstd2, GVAE_P_BN2_W, GVAE_P_BN2_B, GVAE_P_CONV2_B));
+  if (kept8)
+    TRY(gvae_linear_wgrad8(w.T2, GVAE_F32, H, w.H1q, w.H1s, (int64_t)B * N, H, H, G(GVAE_P_CONV2_W), nullptr, w.op_ws,
+                           s));
+  else
+    TRY(linear_bwd_weight(w.T2, w.H1, H, G(GVAE_P_CONV2_W), B * N, H, H, w.splitk, s));
+  TRY(linear_bwd_input(w.T2, P.p[GVAE_P_CONV2_W], w.T0, B * N, H, H, 0, w.splitk, s));
+  TRY(layer(w.Y1, w.Y1q, w.Y1s, w.mean1, w.rstd1, GVAE_P_BN1_W, GVAE_P_BN1_B, GVAE_P_CONV1_B));
+  TRY(linear_bwd_weight(w.T2, d_x, F, G(GVAE_P_CONV1_W), B * N, H, F, w.splitk, s));
+  return check_launch("step_gn_backward");
 }
 
 int gvae_step_read_debug(const gvae_dims *d, int n_graphs, void *d_ws, int which, float **out_ptr,

@@ -37,6 +37,26 @@ class Dims(ctypes.Structure):
     _fields_ = [("F", c_int32), ("H", c_int32), ("Z", c_int32), ("N", c_int32)]
 
 
+class GnOpts(ctypes.Structure):
+    _fields_ = [("groups", c_int32), ("act_bits", c_int32), ("eps", c_float)]
+
+
+def norm_options(norm: str, groups: int, act_bits: int, H: int) -> "GnOpts | None":
+    """Options of the encoder's norm: None for "batch" (BatchNorm; activations kept in fp32), GnOpts for
+    "group" (group norm over each graph's rows; activations kept in `act_bits` = 32 or 8 bits)."""
+    if norm not in ("batch", "group"):
+        raise ValueError(f"norm must be batch | group, got {norm!r}")
+    if act_bits not in (8, 32):
+        raise ValueError(f"act_bits must be 8 or 32, got {act_bits}")
+    if norm == "batch":
+        if act_bits != 32:
+            raise ValueError("act_bits=8 needs norm='group' (BatchNorm's backward keeps fp32 activations)")
+        return None
+    if groups < 1 or H % groups:
+        raise ValueError(f"norm='group': {H} channels do not divide into {groups} groups")
+    return GnOpts(groups, act_bits, 1e-5)
+
+
 _bound = False
 
 
@@ -63,6 +83,13 @@ def _bind():
                                                c_void_p, c_int, c_int, c_int, c_float, c_int,
                                                c_void_p, c_void_p, POINTER(c_int32), c_int, c_void_p,
                                                c_void_p, c_void_p, c_void_p, c_int, c_void_p]
+    L.gvae_step_gn_ws_bytes.argtypes = [POINTER(Dims), POINTER(GnOpts), c_int]
+    L.gvae_step_gn_ws_bytes.restype = c_int64
+    L.gvae_step_gn_forward_model.argtypes = [POINTER(Dims), POINTER(GnOpts), c_void_p, c_void_p, c_void_p, c_void_p,
+                                             c_void_p, c_int, c_void_p, c_void_p, c_void_p]
+    L.gvae_step_gn_backward.argtypes = [POINTER(Dims), POINTER(GnOpts), c_void_p, c_void_p, c_void_p, c_void_p,
+                                        c_void_p, c_int, c_void_p, c_void_p, c_int, c_float, c_float, c_void_p,
+                                        c_void_p, c_void_p, c_void_p]
     L.gvae_step_read_debug.argtypes = [POINTER(Dims), c_int, c_void_p, c_int, POINTER(c_void_p),
                                        POINTER(c_int64)]
     L.gvae_adam_ws_bytes.restype = c_int64
@@ -153,7 +180,9 @@ class StepEngine:
 
     def __init__(self, F: int, H: int, Z: int, N: int, device, matching: str = "auto",
                  mpm_iters: int = 50, tol: float = 1e-4, early_stop: bool = True,
-                 s_budget_bytes: int | None = None):
+                 s_budget_bytes: int | None = None, norm: str = "batch", norm_groups: int = 8,
+                 act_bits: int = 32):
+        self.gn = norm_options(norm, norm_groups, act_bits, H)
         self.L = _bind()
         self.dims = Dims(F, H, Z, N)
         self.F, self.H, self.Z, self.N = F, H, Z, N
@@ -188,7 +217,8 @@ class StepEngine:
     # ------------------------------------------------------------------ helpers
     def _ensure(self, B: int) -> None:
         if self._ws is None or B > self._ws_graphs:
-            need = self.L.gvae_step_ws_bytes(ctypes.byref(self.dims), B)
+            need = (self.L.gvae_step_ws_bytes(ctypes.byref(self.dims), B) if self.gn is None else
+                    self.L.gvae_step_gn_ws_bytes(ctypes.byref(self.dims), ctypes.byref(self.gn), B))
             # (zeroed once: the streamed matching's statistics words in it are only ever added to)
             self._ws = torch.zeros(need, dtype=torch.uint8, device=self.device)
             self._ws_graphs = B
@@ -273,6 +303,17 @@ class StepEngine:
         model_legacy.py:257-363); the backward of this batch uses the same variant."""
         B, r_max, mode = self._prepare(params, bn_state, batch, eps, pos_weight, loss_variant)
         S_ptr, Soff_ptr, chunks, n_chunks = self._S_args(mode, batch, loss_variant)
+        if self.gn is not None:
+            self._gn_forward_model(params, batch, eps)
+            _hip._check(self.L.gvae_step_forward_match_loss(
+                ctypes.byref(self.dims), batch.adj_dense.data_ptr(), batch.num_real_nodes.data_ptr(), B, r_max,
+                pos_weight.data_ptr(), int(loss_variant), mode, self.mpm_iters, self.tol, int(self.early_stop), S_ptr,
+                Soff_ptr, chunks, n_chunks, self._ws.data_ptr(), self.out4.data_ptr(), self.perm.data_ptr(),
+                self.iters_done.data_ptr(), PHASE_MATCH | PHASE_ASSIGN_LOSS, _hip._stream()))
+            self.generation += 1
+            self._fwd_batch = (batch, eps, int(loss_variant))
+            self.last_mode = mode
+            return self.out4
         _hip._check(self.L.gvae_step_forward(
             ctypes.byref(self.dims), params.data_ptr(), bn_state.data_ptr(), batch.x.data_ptr(),
             batch.adj_dense.data_ptr(), batch.n_x.data_ptr(), batch.num_real_nodes.data_ptr(), B, r_max,
@@ -285,6 +326,12 @@ class StepEngine:
         self.last_mode = mode
         return self.out4
 
+    def _gn_forward_model(self, params, batch, eps) -> None:
+        _hip._check(self.L.gvae_step_gn_forward_model(
+            ctypes.byref(self.dims), ctypes.byref(self.gn), params.data_ptr(), batch.x.data_ptr(),
+            batch.adj_dense.data_ptr(), batch.n_x.data_ptr(), batch.num_real_nodes.data_ptr(), batch.num_graphs,
+            eps.data_ptr(), self._ws.data_ptr(), _hip._stream()))
+
     def forward_model(self, params: torch.Tensor, bn_state: torch.Tensor, batch: DenseGraphBatch,
                       eps: torch.Tensor, pos_weight: torch.Tensor, train: bool,
                       loss_variant: int = LOSS_CURRENT) -> None:
@@ -295,10 +342,13 @@ class StepEngine:
             raise _hip.GvaeHipError("the individual-rho loss has no split forward: its backward reads the "
                                     "permutation, so the whole forward() has to precede it")
         B, r_max, mode = self._prepare(params, bn_state, batch, eps, pos_weight, loss_variant)
-        _hip._check(self.L.gvae_step_forward_model(
-            ctypes.byref(self.dims), params.data_ptr(), bn_state.data_ptr(), batch.x.data_ptr(),
-            batch.adj_dense.data_ptr(), batch.n_x.data_ptr(), batch.num_real_nodes.data_ptr(), B,
-            eps.data_ptr(), int(train), self._ws.data_ptr(), _hip._stream()))
+        if self.gn is not None:
+            self._gn_forward_model(params, batch, eps)
+        else:
+            _hip._check(self.L.gvae_step_forward_model(
+                ctypes.byref(self.dims), params.data_ptr(), bn_state.data_ptr(), batch.x.data_ptr(),
+                batch.adj_dense.data_ptr(), batch.n_x.data_ptr(), batch.num_real_nodes.data_ptr(), B,
+                eps.data_ptr(), int(train), self._ws.data_ptr(), _hip._stream()))
         self.generation += 1
         self._fwd_batch = (batch, eps, int(loss_variant))
         self._pending = (B, r_max, mode, pos_weight, PHASE_MATCH | PHASE_ASSIGN_LOSS)
@@ -368,8 +418,10 @@ class StepEngine:
         if d_up is not None:
             _hip._dev(d_up, torch.float32)
             up = d_up.data_ptr()
-        _hip._check(self.L.gvae_step_backward(
-            ctypes.byref(self.dims), params.data_ptr(), batch.x.data_ptr(), batch.adj_dense.data_ptr(),
+        gn = () if self.gn is None else (ctypes.byref(self.gn),)
+        backward = self.L.gvae_step_backward if self.gn is None else self.L.gvae_step_gn_backward
+        _hip._check(backward(
+            ctypes.byref(self.dims), *gn, params.data_ptr(), batch.x.data_ptr(), batch.adj_dense.data_ptr(),
             batch.n_x.data_ptr(), batch.num_real_nodes.data_ptr(), batch.num_graphs, eps.data_ptr(),
             pos_weight.data_ptr(), loss_variant, float(c_rec), float(c_kl), up, self._ws.data_ptr(),
             grads.data_ptr(), _hip._stream()))
@@ -425,6 +477,8 @@ class StepEngine:
 
     def debug_tensor(self, name: str, B: int) -> torch.Tensor:
         """Copy of an intermediate buffer of the last forward of B graphs."""
+        if self.gn is not None and name in ("Y1", "H1", "Y2", "H2", "Ahat", "dY1"):
+            raise _hip.GvaeHipError(f"debug_tensor: {name} is not kept with norm='group'")
         ptr, cnt = c_void_p(), c_int64()
         _hip._check(self.L.gvae_step_read_debug(ctypes.byref(self.dims), B, self._ws.data_ptr(),
                                                 self._DEBUG[name], ctypes.byref(ptr), ctypes.byref(cnt)))

@@ -2,6 +2,7 @@
 
 Drop-in surface (reference graphvae/models/model.py):
   GraphVAE(in_dim, hid_dim, z_dim, max_nodes, *, pool="sum")          :63-94
+      (norm="group", norm_groups, act_bits: group norm and 8-bit checkpoints in the encoder, not in the reference)
   .precompute_dataset_rho(loader)                                       :99-118
   .forward(data) -> {"rec","kl","loss","max_logit","logvar_max"}        :281-373
   ._edge_sim_tensor(A, B) -> (R,R,R,R)                                  :171-216
@@ -29,7 +30,7 @@ import torch.nn as nn
 from .. import _hip
 from ..data import DenseGraphBatch, as_dense_batch
 from ..engine import (LOSS_CURRENT, LOSS_DUMMY_MASKED, LOSS_INDIVIDUAL_RHO, PARAM_NAMES, StepEngine,
-                      param_layout)
+                      norm_options, param_layout)
 
 
 def vec_to_adj(vec: torch.Tensor, N: int, *, diag: bool = False) -> torch.Tensor:
@@ -160,8 +161,17 @@ class _StepFunction(torch.autograd.Function):
 class GraphVAE(nn.Module):
     def __init__(self, in_dim: int, hid_dim: int, z_dim: int, max_nodes: int, *, pool: str = "sum",
                  matching: str = "auto", mpm_iters: int = 50, mpm_tol: float = 1e-4,
-                 mpm_early_stop: bool = True, s_budget_bytes: int | None = None) -> None:
+                 mpm_early_stop: bool = True, s_budget_bytes: int | None = None, norm: str = "batch",
+                 norm_groups: int = 8, act_bits: int = 32) -> None:
+        """`norm`: "batch" (the reference's BatchNorm1d) or "group": group norm over each graph's own rows in
+        `norm_groups` runs of channels, the same in training and evaluation.  Its weight and bias are
+        `bn{1,2}.weight` / `.bias`; the running statistics stay as they are.  `act_bits` (norm="group"):
+        the encoder's activations are kept for the backward in 32 bits or as 8-bit checkpoints, which
+        leaves the forward as it is (up to the order of its sums) and gives the gradients the checkpoints'
+        rounding."""
         super().__init__()
+        norm_options(norm, norm_groups, act_bits, int(hid_dim))
+        self.norm, self.norm_groups, self.act_bits = norm, int(norm_groups), int(act_bits)
         # bytes of HBM the streamed matching may use for the similarity tensor at a time
         # (None: a third of the device); larger batches are matched in chunks
         self.s_budget_bytes = s_budget_bytes
@@ -271,7 +281,8 @@ class GraphVAE(nn.Module):
             self._engine = StepEngine(self.in_dim, self.hid_dim, self.z_dim, self.max_nodes, dev,
                                       matching=self.matching, mpm_iters=self.mpm_iters,
                                       tol=self.mpm_tol, early_stop=self.mpm_early_stop,
-                                      s_budget_bytes=self.s_budget_bytes)
+                                      s_budget_bytes=self.s_budget_bytes, norm=self.norm,
+                                      norm_groups=self.norm_groups, act_bits=self.act_bits)
         return self._engine
 
     # ------------------------------------------------------------------ dataset statistics
@@ -393,7 +404,7 @@ class GraphVAE(nn.Module):
         variant = LOSS_INDIVIDUAL_RHO if individual_rho else (LOSS_DUMMY_MASKED if legacy else LOSS_CURRENT)
         rec, kl, max_logit, logvar_max = _StepFunction.apply(self, batch, eps, variant,
                                                              *self._named_param_list())
-        if self.training:
+        if self.training and self.norm == "batch":
             for bn in (self.bn1, self.bn2):
                 bn.num_batches_tracked += batch.num_graphs
         if legacy or individual_rho:   # reference model.py:439-440 / model_legacy.py:363: no "loss" entry

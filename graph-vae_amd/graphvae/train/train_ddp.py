@@ -484,8 +484,9 @@ class TrainStep:
             # join: what follows on this stream (the caller reading the losses, the next forward
             # overwriting the workspace) is ordered behind the matching half
             main.wait_event(self._ev_match[k])
-        torch._foreach_add_([model.bn1.num_batches_tracked, model.bn2.num_batches_tracked],
-                            batch.num_graphs)
+        if getattr(model, "norm", "batch") == "batch":
+            torch._foreach_add_([model.bn1.num_batches_tracked, model.bn2.num_batches_tracked],
+                                batch.num_graphs)
         return out4
 
 
@@ -574,7 +575,9 @@ def _ddp_worker(rank: int, world: int, args) -> None:
                         lambda ep: shard_indices(n_va, world, rank, False, ep), device) if n_va else []
 
     model = GraphVAE(in_dim=args.in_dim, hid_dim=args.hid_dim, z_dim=args.z_dim, max_nodes=max_nodes,
-                     pool=args.pool, matching=getattr(args, "matching", "auto")).to(device)
+                     pool=args.pool, matching=getattr(args, "matching", "auto"),
+                     norm=getattr(args, "norm", "batch"), norm_groups=getattr(args, "norm_groups", 8),
+                     act_bits=getattr(args, "act_bits", 32)).to(device)
     # rho over the full training set, identical on every rank (same data, same arithmetic)
     model.precompute_dataset_rho([dense_tr])
     if world > 1:
@@ -655,6 +658,7 @@ _DEFAULTS = dict(
     dataset="grid", feature_type="deg", lr=1e-4, epochs=200, max_nodes=None, log_dir="runs",
     use_wandb=True, run_name=None, batch_size=64, weight_decay=1e-4, beta0=0.0, beta_final=0.5,
     warm_epochs=40, clip_max=5.0, hid_dim=128, z_dim=64, pool="sum", debug=False, matching="auto",
+    norm="batch", norm_groups=8, act_bits=32,
 )
 
 
@@ -724,6 +728,11 @@ def main(argv=None) -> None:
     pa.add_argument("--max_nodes", type=int, default=None)
     pa.add_argument("--matching", choices=["auto", "stream", "fused"], default=None,
                     help="MPM kernel: stream the materialised similarity tensor, or the fused S-free form")
+    pa.add_argument("--norm", choices=["batch", "group"], default=None,
+                    help="encoder norm: BatchNorm (as the reference) or group norm over each graph's rows")
+    pa.add_argument("--norm_groups", type=int, default=None, help="channel groups of --norm group")
+    pa.add_argument("--act_bits", type=int, choices=[8, 32], default=None,
+                    help="--norm group: bits in which the encoder's activations are kept for the backward")
     pa.add_argument("--log_dir", default="runs")
     pa.add_argument("--config", help="YAML config with a 'trainer:' section")
     pa.add_argument("--no_wandb", action="store_true", help="disable Weights & Biases logging")

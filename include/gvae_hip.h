@@ -434,6 +434,33 @@ int gvae_linear_wgrad8(const void *d_dy, int dtype, int64_t row_stride, const in
                        const uint8_t *d_scales, int64_t rows, int O, int I, void *d_dw, void *d_db, void *d_ws,
                        void *stream);
 
+/* The training step with group norm in the encoder: as GraphVAE.forward (graphvae/models/model.py:281-373)
+ * with both BatchNorm layers replaced by group norm over a graph's n_x live rows, the same in training
+ * and evaluation.  The norm's weight and bias are the parameters GVAE_P_BN1_* / GVAE_P_BN2_*. */
+typedef struct gvae_gn_opts {
+  int32_t groups;     /* runs of consecutive channels; divides H */
+  int32_t act_bits;   /* what the forward keeps of the encoder for the backward: 32 (fp32) or 8 (checkpoints) */
+  float eps;
+} gvae_gn_opts;
+
+int64_t gvae_step_gn_ws_bytes(const gvae_dims *d, const gvae_gn_opts *gn, int n_graphs);
+
+/* gvae_step_forward_model with group norm (no statistics to update, hence no mode argument).  The
+ * workspace (gvae_step_gn_ws_bytes) then takes gvae_step_forward_match_loss as it does after
+ * gvae_step_forward_model, and gvae_step_gn_backward with the same options.  gvae_step_read_debug
+ * knows the buffers 0-8, 13, 16 and 17 in it. */
+int gvae_step_gn_forward_model(const gvae_dims *d, const gvae_gn_opts *gn, const float *d_params, const float *d_x,
+                               const float *d_adj, const int32_t *d_n_x, const int32_t *d_R, int n_graphs,
+                               const float *d_eps, void *d_ws, void *stream);
+
+/* gvae_step_backward behind gvae_step_gn_forward_model.  With act_bits 8 the encoder's normalised
+ * activations and the second layer's weight gradient come from the checkpoints; the forward
+ * computes the same from the same values (its sums possibly in another order). */
+int gvae_step_gn_backward(const gvae_dims *d, const gvae_gn_opts *gn, const float *d_params, const float *d_x,
+                          const float *d_adj, const int32_t *d_n_x, const int32_t *d_R, int n_graphs,
+                          const float *d_eps, const float *d_pos_weight, int loss_variant, float c_rec, float c_kl,
+                          const float *d_up, void *d_ws, float *d_grads, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
