@@ -74,24 +74,22 @@ __global__ __launch_bounds__(NT) void norm_bwd_resident_kernel(NormArgs a) {
       mean[e] = a.mean[q];
       rstd[e] = a.rstd[q];
     }
-    float p1[V], p2[V];
+    // (dz stays in fp32: the slope costs more than the registers)
+    float p1[V], p2[V], dz[K][V];
 #pragma unroll
     for (int v = 0; v < V; ++v) p1[v] = p2[v] = 0.0f;
 #pragma unroll
     for (int u = 0; u < K; ++u)
       if (on && r0 + u * a.rp < live) {
-        float h[V], dz[V];
+        float h[V], s[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[v] = (x[u].at(v) - mean[IN ? 0 : v]) * rstd[IN ? 0 : v];
+        act_slopes<V>(a.act, h, w, bias, s);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          h[v] = (x[u].at(v) - mean[IN ? 0 : v]) * rstd[IN ? 0 : v];
-          dz[v] = h[v] * w[v] + bias[v];
-        }
-        act_slopes<V>(a.act, dz);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float d = v < nv ? (float)g[u][v] * dz[v] : 0.0f;
-          p1[v] += d;
-          p2[v] += v < nv ? d * h[v] : 0.0f;
+          dz[u][v] = v < nv ? (float)g[u][v] * s[v] : 0.0f;
+          p1[v] += dz[u][v];
+          p2[v] = v < nv ? __fmaf_rn(dz[u][v], h[v], p2[v]) : 0.0f;
         }
       }
     {
@@ -113,10 +111,7 @@ __global__ __launch_bounds__(NT) void norm_bwd_resident_kernel(NormArgs a) {
         }
     }
 #pragma unroll
-    for (int u = 0; u < K; ++u) {
-      keep_raw<T>(g[u]);
-      x[u].keep();
-    }
+    for (int u = 0; u < K; ++u) x[u].keep();
     __syncthreads();
     join_groups<2, NT * V, NT * E>(ent, a.lanes * E, ge, ng, a.rp, a.join, NT, grp);
     __syncthreads();
@@ -132,20 +127,12 @@ __global__ __launch_bounds__(NT) void norm_bwd_resident_kernel(NormArgs a) {
     for (int u = 0; u < K; ++u) {
       const int i = r0 + u * a.rp;
       if (i >= a.N) break;
-      float h[V], dx[V];
-      if (i < live) {
+      float dx[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          h[v] = (x[u].at(v) - mean[IN ? 0 : v]) * rstd[IN ? 0 : v];
-          dx[v] = h[v] * w[v] + bias[v];
-        }
-        act_slopes<V>(a.act, dx);
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          dx[v] = rstd[IN ? 0 : v] * ((float)g[u][v] * dx[v] * w[v] - __fmaf_rn(h[v], a2[IN ? 0 : v], a1[IN ? 0 : v]));
-      } else {
-#pragma unroll
-        for (int v = 0; v < V; ++v) dx[v] = 0.0f;
+      for (int v = 0; v < V; ++v) {
+        const int e = IN ? 0 : v;
+        const float h = (x[u].at(v) - mean[e]) * rstd[e];
+        dx[v] = i < live ? rstd[e] * __fmaf_rn(dz[u][v], w[v], -__fmaf_rn(h, a2[e], a1[e])) : 0.0f;
       }
       store_piece<T>((T *)a.out + ((int64_t)b * a.N + i) * a.C + c0, dx, nv);
     }
@@ -196,9 +183,9 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_sums_kernel(NormArgs a) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const float h = (x[u].at(v) - k.mean[v]) * k.rstd[v];
-          const float dz = v < p.nv ? (float)g[u][v] * act_slope<ACT>(h * k.w[v] + k.b[v]) : 0.0f;
+          const float dz = v < p.nv ? (float)g[u][v] * act_slope<ACT>(pre_act<ACT>(h, k.w[v], k.b[v])) : 0.0f;
           s1[v] += dz;
-          s2[v] += v < p.nv ? dz * h : 0.0f;
+          s2[v] = v < p.nv ? __fmaf_rn(dz, h, s2[v]) : 0.0f;
         }
       }
     }
@@ -313,8 +300,8 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_apply_kernel(NormArgs a) {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const float h = (x[u].at(v) - k.mean[v]) * k.rstd[v];
-        const float dz = (float)g[u][v] * act_slope<ACT>(h * k.w[v] + k.b[v]);
-        dx[v] = i < live ? k.rstd[v] * (dz * k.w[v] - __fmaf_rn(h, a2[v], a1[v])) : 0.0f;
+        const float dz = (float)g[u][v] * act_slope<ACT>(pre_act<ACT>(h, k.w[v], k.b[v]));
+        dx[v] = i < live ? k.rstd[v] * __fmaf_rn(dz, k.w[v], -__fmaf_rn(h, a2[v], a1[v])) : 0.0f;
       }
       store_piece<T>((T *)a.out + ((int64_t)p.b * a.N + i) * a.C + p.c0, dx, p.nv);
     }
@@ -348,7 +335,6 @@ static void resident_launch(NormArgs &a, hipStream_t s) {
     RUN(256, 4);
   }
   RUN(512, 4);
-  RUN(512, 8);
 #undef RUN
 }
 template <class T, int ACT, bool KEPT>

@@ -28,6 +28,12 @@ __global__ __launch_bounds__(NT) void norm_resident_kernel(NormArgs a) {
     k[u] = typename Piece<T>::raw{};
     if (on && i < live) k[u] = load_piece<T>(x + (int64_t)i * a.xr, nv);
   }
+  float w[V], bias[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    w[v] = v < nv ? (a.w ? a.w[c0 + v] : 1.0f) : 0.0f;
+    bias[v] = v < nv && a.b ? a.b[c0 + v] : 0.0f;
+  }
   // this thread's entry e of group entries starts at the piece's own group
   const int mine = (threadIdx.x < a.rp * a.lanes) ? (int)threadIdx.x * E : -1;
   const int ge = IN ? a.cpg / V : a.cpg;
@@ -85,12 +91,6 @@ __global__ __launch_bounds__(NT) void norm_resident_kernel(NormArgs a) {
     a.rstd[q] = 1.0f / sqrtf(grp[1][g] * inv + a.eps);
   }
   if (r0 >= a.rp) return;
-  float w[V], bias[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    w[v] = v < nv ? (a.w ? a.w[c0 + v] : 1.0f) : 0.0f;
-    bias[v] = v < nv && a.b ? a.b[c0 + v] : 0.0f;
-  }
 #pragma unroll
   for (int u = 0; u < K; ++u) {
     const int i = r0 + u * a.rp;
@@ -99,9 +99,9 @@ __global__ __launch_bounds__(NT) void norm_resident_kernel(NormArgs a) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       xf[v] = (float)k[u][v];
-      y[v] = (xf[v] - mean[IN ? 0 : v]) * rstd[IN ? 0 : v] * w[v] + bias[v];
+      y[v] = (xf[v] - mean[IN ? 0 : v]) * rstd[IN ? 0 : v];
     }
-    act_values<V>(a.act, y);
+    act_values<V>(a.act, y, w, bias, y);
 #pragma unroll
     for (int v = 0; v < V; ++v) y[v] = i < live && v < nv ? (float)(T)y[v] : 0.0f;
     const int64_t row = (int64_t)b * a.N + i;
@@ -253,7 +253,7 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(NormArgs a) {
       for (int v = 0; v < V; ++v) {
         xf[v] = (float)r[u][v];
         y[v] = i < live && v < p.nv
-                   ? (float)(T)act_value<ACT>((xf[v] - k.mean[v]) * k.rstd[v] * k.w[v] + k.b[v]) : 0.0f;
+                   ? (float)(T)act_value<ACT>(pre_act<ACT>((xf[v] - k.mean[v]) * k.rstd[v], k.w[v], k.b[v])) : 0.0f;
       }
       const int64_t row = (int64_t)p.b * a.N + i;
       if (p.nv > 0) store_piece<T>((T *)a.out + row * a.C + p.c0, y, p.nv);
@@ -287,7 +287,6 @@ static void resident_launch(NormArgs &a, hipStream_t s) {
     RUN(256, 16);
   }
   RUN(1024, 8);
-  RUN(1024, 16);
 #undef RUN
 }
 

@@ -48,34 +48,49 @@ def _bind():
     return _bound
 
 
+_device_index = torch._C._cuda_getDevice      # of the current device
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_empty = torch.empty
+
+
 def _act_code(act: str) -> int:
-    if act not in _ACT:
+    code = _ACT.get(act)
+    if code is None:
         raise ValueError(f"act must be one of {sorted(_ACT)}, got {act!r}")
-    return _ACT[act]
+    return code
 
 
-def _on_device(t: torch.Tensor, what: str) -> torch.Tensor:
+def _on_device(t: torch.Tensor, what: str) -> int:
+    """Checks that t is on the current device; returns its index."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise _hip.GvaeHipError(f"{what}: expected a device tensor (the HIP path has no CPU fallback)")
-    if t.device.index != torch._C._cuda_getDevice():
-        raise _hip.GvaeHipError(f"{what} on {t.device} but the current device is cuda:"
-                                f"{torch.cuda.current_device()}: wrap the call in torch.cuda.device(...)")
-    return t
+    index = _device_index()
+    if t.get_device() != index:
+        raise _hip.GvaeHipError(f"{what} on {t.device} but the current device is cuda:{index}: wrap the call in "
+                                "torch.cuda.device(...)")
+    return index
 
 
-def _activation(t: torch.Tensor, what: str, shape=None, dtype=None) -> int:
-    """Checks an activation or gradient of any row and batch stride; returns its type code."""
-    _on_device(t, what)
+def _activation(t: torch.Tensor, what: str) -> int:
+    """Checks the type and the channels of an activation or gradient; returns its type code."""
     code = _DTYPE.get(t.dtype)
-    if code is None or (dtype is not None and t.dtype != dtype):
-        raise _hip.GvaeHipError(f"{what}: expected {dtype or 'float32, bfloat16 or float16'}, got {t.dtype}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise _hip.GvaeHipError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    if t.numel() == 0:
+    if code is None:
+        raise _hip.GvaeHipError(f"{what}: expected float32, bfloat16 or float16, got {t.dtype}")
+    if t.dim() < 1 or t.numel() == 0:
         raise _hip.GvaeHipError(f"{what}: no element in shape {tuple(t.shape)}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise _hip.GvaeHipError(f"{what}: channels must be last and contiguous, got strides {t.stride()}")
     return code
+
+
+def _small(t, shape: tuple, dtype: torch.dtype, index: int, what: str, name: str):
+    """Address of a contiguous side input (None for None) of the given shape and type."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.get_device() != index or t.shape != shape or not t.is_contiguous():
+        raise _hip.GvaeHipError(f"{what}: {name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on "
+                                f"cuda:{index}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
 
 
 def _rows_of(t: torch.Tensor, what: str) -> tuple[int, int]:
@@ -100,10 +115,6 @@ def _graph_strides(t: torch.Tensor, what: str) -> tuple[int, int]:
 
 
 _NONE = (None, None)
-
-
-def _workspace(n: int, device):
-    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
 class Checkpoint8:
@@ -132,22 +143,18 @@ class Checkpoint8:
             raise _hip.GvaeHipError("Checkpoint8: codes must be 16-byte aligned")
         self._codes, self._scales, self._buf = codes, scales, None
         self._at = (codes.data_ptr(), scales.data_ptr())
-        self.shape, self.dtype, self.device = lead + (C,), dtype, codes.device
+        self.shape, self.dtype, self.device = torch.Size(lead + (C,)), dtype, codes.device
 
     @classmethod
-    def _new(cls, shape: tuple, device, dtype: torch.dtype) -> "Checkpoint8":
+    def _new(cls, shape, rows: int, C: int, device, dtype: torch.dtype) -> "Checkpoint8":
         """Room for a checkpoint: one allocation, the codes first."""
         self = object.__new__(cls)
-        C = shape[-1]
-        rows = 1
-        for n in shape[:-1]:
-            rows *= n
         n_codes = rows * ((C + 15) // 16 * 16)
-        self._buf = torch.empty(n_codes + rows * ((C + 31) // 32), dtype=torch.uint8, device=device)
-        base = self._buf.data_ptr()
+        self._buf = buf = _empty(n_codes + rows * ((C + 31) // 32), dtype=torch.uint8, device=device)
+        base = buf.data_ptr()
         self._codes = self._scales = None
         self._at = (base, base + n_codes)
-        self.shape, self.dtype, self.device = tuple(shape), dtype, device
+        self.shape, self.dtype, self.device = shape, dtype, device
         return self
 
     def __reduce__(self):
@@ -172,10 +179,11 @@ class Checkpoint8:
                 self.shape[:-1] + ((self.shape[-1] + 31) // 32,))
         return self._scales
 
-    def _check(self, what: str) -> None:
-        _on_device(self._buf if self._codes is None else self._codes, what)
+    def _check(self, what: str) -> int:
+        index = _on_device(self._buf if self._codes is None else self._codes, what)
         if 0 in self.shape:
-            raise _hip.GvaeHipError(f"{what}: no element in shape {self.shape}")
+            raise _hip.GvaeHipError(f"{what}: no element in shape {tuple(self.shape)}")
+        return index
 
     def read(self, dtype: torch.dtype | None = None) -> torch.Tensor:
         """The values the checkpoint stands for, as `dtype` (default: the type that was written);
@@ -184,23 +192,27 @@ class Checkpoint8:
         code = _DTYPE.get(dtype)
         if code is None:
             raise _hip.GvaeHipError(f"Checkpoint8.read: cannot be read as {dtype}")
-        self._check("Checkpoint8.read")
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        index = self._check("Checkpoint8.read")
+        out = _empty(self.shape, dtype=dtype, device=self.device)
         C = self.shape[-1]
-        _hip._check(_bind().gvae_ckpt8_read(self._at[0], self._at[1], out.numel() // C, C, out.data_ptr(), code, C,
-                                            _hip._stream()))
+        rc = (_bound or _bind()).gvae_ckpt8_read(self._at[0], self._at[1], out.numel() // C, C, out.data_ptr(), code, C,
+                                                 _raw_stream(index))
+        if rc:
+            _hip._check(rc)
         return out
 
 
 def checkpoint8(x: torch.Tensor) -> Checkpoint8:
     """8-bit checkpoint of x (..., C) float32 / bfloat16 / float16: contiguous, or a matrix with any
     row stride.  A block of 32 channels that holds an infinity or a NaN reads back as NaN."""
+    index = _on_device(x, "checkpoint8")
     code = _activation(x, "checkpoint8")
-    if x.dim() < 1:
-        raise _hip.GvaeHipError("checkpoint8: expected at least one axis")
     rows, ld = _rows_of(x, "checkpoint8")
-    c = Checkpoint8._new(x.shape, x.device, x.dtype)
-    _hip._check(_bind().gvae_ckpt8_write(x.data_ptr(), code, rows, x.shape[-1], ld, *c._at, _hip._stream()))
+    C = x.shape[-1]
+    c = Checkpoint8._new(x.shape, rows, C, x.device, x.dtype)
+    rc = (_bound or _bind()).gvae_ckpt8_write(x.data_ptr(), code, rows, C, ld, c._at[0], c._at[1], _raw_stream(index))
+    if rc:
+        _hip._check(rc)
     return c
 
 
@@ -210,24 +222,6 @@ class GroupNormOut(NamedTuple):
     rstd: torch.Tensor          # (graphs, groups) float32
     x8: Checkpoint8 | None      # checkpoint of x, if asked for
     y8: Checkpoint8 | None      # checkpoint of y, if asked for
-
-
-def _norm_params(weight, bias, C: int, what: str):
-    for t in (weight, bias):
-        if t is not None:
-            _hip._dev(t, torch.float32)
-            if tuple(t.shape) != (C,):
-                raise _hip.GvaeHipError(f"{what}: weight and bias must have shape ({C},), got {tuple(t.shape)}")
-    return (weight.data_ptr() if weight is not None else None, bias.data_ptr() if bias is not None else None)
-
-
-def _live_rows(rows, B: int, what: str):
-    if rows is None:
-        return None
-    _hip._dev(rows, torch.int32)
-    if tuple(rows.shape) != (B,):
-        raise _hip.GvaeHipError(f"{what}: rows must have shape ({B},), got {tuple(rows.shape)}")
-    return rows.data_ptr()
 
 
 def _norm_sizes(x_shape, groups: int, what: str):
@@ -252,22 +246,29 @@ def group_norm_act(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Ten
     (dead rows as 0) and of y, the same as `checkpoint8` of them."""
     what = "group_norm_act"
     B, N, C = _norm_sizes(x.shape, groups, what)
-    code, act_code = _activation(x, what), _act_code(act)
+    act_code = _act_code(act)
+    index = _on_device(x, what)
+    code = _activation(x, what)
     batch, row = _graph_strides(x, what)
-    w, b = _norm_params(weight, bias, C, what)
-    live = _live_rows(rows, B, what)
+    w, b = (_small(weight, (C,), torch.float32, index, what, "weight"),
+            _small(bias, (C,), torch.float32, index, what, "bias"))
+    live = _small(rows, (B,), torch.int32, index, what, "rows")
     if not eps > 0.0:
         raise ValueError(f"{what}: eps must be positive, got {eps}")
-    L, dev = _bind(), x.device
-    y = torch.empty((B, N, C), dtype=x.dtype, device=dev)
-    mean, rstd = torch.empty((2, B, groups), dtype=torch.float32, device=dev).unbind(0)
-    x8 = Checkpoint8._new((B, N, C), dev, x.dtype) if keep_x else None
-    y8 = Checkpoint8._new((B, N, C), dev, x.dtype) if keep_y else None
-    ws = _workspace(L.gvae_group_norm_ws_bytes(0, code, B, N, C, groups, keep_x or keep_y), dev)
-    _hip._check(L.gvae_group_norm_fwd(
-        x.data_ptr(), code, batch, row, live, B, N, C, groups, w, b, eps, act_code, y.data_ptr(), mean.data_ptr(),
-        rstd.data_ptr(), *(x8._at if keep_x else _NONE), *(y8._at if keep_y else _NONE),
-        None if ws is None else ws.data_ptr(), _hip._stream()))
+    L, dev = _bound or _bind(), x.device
+    y = _empty((B, N, C), dtype=x.dtype, device=dev)
+    mean, rstd = _empty((2, B, groups), dtype=torch.float32, device=dev).unbind(0)
+    x8 = Checkpoint8._new(x.shape, B * N, C, dev, x.dtype) if keep_x else None
+    y8 = Checkpoint8._new(x.shape, B * N, C, dev, x.dtype) if keep_y else None
+    need = L.gvae_group_norm_ws_bytes(0, code, B, N, C, groups, keep_x or keep_y)
+    ws = _empty(need, dtype=torch.uint8, device=dev) if need else None
+    xc, xs = x8._at if keep_x else _NONE
+    yc, ys = y8._at if keep_y else _NONE
+    rc = L.gvae_group_norm_fwd(x.data_ptr(), code, batch, row, live, B, N, C, groups, w, b, eps, act_code, y.data_ptr(),
+                               mean.data_ptr(), rstd.data_ptr(), xc, xs, yc, ys, ws.data_ptr() if need else None,
+                               _raw_stream(index))
+    if rc:
+        _hip._check(rc)
     return GroupNormOut(y, mean, rstd, x8, y8)
 
 
@@ -281,31 +282,39 @@ def group_norm_act_backward(dy: torch.Tensor, x, weight: torch.Tensor | None, bi
     what = "group_norm_act_backward"
     kept = isinstance(x, Checkpoint8)
     B, N, C = _norm_sizes(dy.shape, groups, what)
-    code, act_code = _activation(dy, what), _act_code(act)
+    act_code = _act_code(act)
+    index = _on_device(dy, what)
+    code = _activation(dy, what)
+    if x.shape != dy.shape:
+        raise _hip.GvaeHipError(f"{what}: input of shape {tuple(x.shape)}, gradient {tuple(dy.shape)}")
     if kept:
         x._check(what)
-        if x.shape != (B, N, C):
-            raise _hip.GvaeHipError(f"{what}: checkpoint of shape {x.shape}, gradient {tuple(dy.shape)}")
-        xs, xb, xr, x8, x8s = None, 0, C, x._at[0], x._at[1]
+        xs, xb, xr = None, 0, C
+        x8, x8s = x._at
     else:
-        _activation(x, what, dy.shape, dy.dtype)
+        _on_device(x, what)
+        if x.dtype is not dy.dtype:
+            raise _hip.GvaeHipError(f"{what}: input is {x.dtype}, gradient {dy.dtype}")
+        _activation(x, what)
         xb, xr = _graph_strides(x, what)
         xs, x8, x8s = x.data_ptr(), None, None
     db_, dr_ = _graph_strides(dy, what)
-    w, b = _norm_params(weight, bias, C, what)
-    live = _live_rows(rows, B, what)
-    for t in (mean, rstd):
-        _hip._dev(t, torch.float32)
-        if tuple(t.shape) != (B, groups):
-            raise _hip.GvaeHipError(f"{what}: mean and rstd must have shape ({B}, {groups}), got {tuple(t.shape)}")
-    L, dev = _bind(), dy.device
-    dx = torch.empty((B, N, C), dtype=dy.dtype, device=dev)
-    dweight, dbias = torch.empty((2, C), dtype=torch.float32, device=dev).unbind(0)
-    ws = _workspace(L.gvae_group_norm_ws_bytes(1, code, B, N, C, groups, kept), dev)
-    _hip._check(L.gvae_group_norm_bwd(
-        dy.data_ptr(), code, db_, dr_, xs, xb, xr, x8, x8s, live, B, N, C, groups, w, b, mean.data_ptr(),
-        rstd.data_ptr(), act_code, dx.data_ptr(), dweight.data_ptr(), dbias.data_ptr(), ws.data_ptr(),
-        _hip._stream()))
+    w, b = (_small(weight, (C,), torch.float32, index, what, "weight"),
+            _small(bias, (C,), torch.float32, index, what, "bias"))
+    live = _small(rows, (B,), torch.int32, index, what, "rows")
+    if mean is None or rstd is None:
+        raise _hip.GvaeHipError(f"{what}: needs the mean and rstd of the forward")
+    mu, rs = (_small(mean, (B, groups), torch.float32, index, what, "mean"),
+              _small(rstd, (B, groups), torch.float32, index, what, "rstd"))
+    L, dev = _bound or _bind(), dy.device
+    dx = _empty((B, N, C), dtype=dy.dtype, device=dev)
+    dweight, dbias = _empty((2, C), dtype=torch.float32, device=dev).unbind(0)
+    ws = _empty(L.gvae_group_norm_ws_bytes(1, code, B, N, C, groups, kept), dtype=torch.uint8, device=dev)
+    rc = L.gvae_group_norm_bwd(dy.data_ptr(), code, db_, dr_, xs, xb, xr, x8, x8s, live, B, N, C, groups, w, b, mu, rs,
+                               act_code, dx.data_ptr(), dweight.data_ptr(), dbias.data_ptr(), ws.data_ptr(),
+                               _raw_stream(index))
+    if rc:
+        _hip._check(rc)
     return dx, dweight, dbias
 
 
@@ -317,15 +326,19 @@ def linear_wgrad8(dy: torch.Tensor, x8: Checkpoint8) -> tuple[torch.Tensor, torc
     if not isinstance(x8, Checkpoint8):
         raise _hip.GvaeHipError(f"{what}: the input must be a Checkpoint8")
     x8._check(what)
+    index = _on_device(dy, what)
     code = _activation(dy, what)
-    if dy.dim() < 2 or tuple(dy.shape[:-1]) != x8.shape[:-1]:
-        raise _hip.GvaeHipError(f"{what}: gradient {tuple(dy.shape)} and checkpoint {x8.shape} differ in their rows")
+    if dy.dim() < 2 or dy.shape[:-1] != x8.shape[:-1]:
+        raise _hip.GvaeHipError(f"{what}: gradient {tuple(dy.shape)} and checkpoint {tuple(x8.shape)} differ in their "
+                                "rows")
     rows, ld = _rows_of(dy, what)
-    O, I = dy.shape[-1], x8.channels
-    L, dev = _bind(), dy.device
-    dw = torch.empty((O, I), dtype=dy.dtype, device=dev)
-    db = torch.empty((O,), dtype=dy.dtype, device=dev)
-    ws = _workspace(L.gvae_linear_wgrad8_ws_bytes(rows, O, I), dev)
-    _hip._check(L.gvae_linear_wgrad8(dy.data_ptr(), code, ld, *x8._at, rows, O, I, dw.data_ptr(), db.data_ptr(),
-                                     ws.data_ptr(), _hip._stream()))
+    O, I = dy.shape[-1], x8.shape[-1]
+    L, dev = _bound or _bind(), dy.device
+    dw = _empty((O, I), dtype=dy.dtype, device=dev)
+    db = _empty((O,), dtype=dy.dtype, device=dev)
+    ws = _empty(L.gvae_linear_wgrad8_ws_bytes(rows, O, I), dtype=torch.uint8, device=dev)
+    rc = L.gvae_linear_wgrad8(dy.data_ptr(), code, ld, x8._at[0], x8._at[1], rows, O, I, dw.data_ptr(), db.data_ptr(),
+                              ws.data_ptr(), _raw_stream(index))
+    if rc:
+        _hip._check(rc)
     return dw, db

@@ -180,7 +180,7 @@ def test_python_refusals_on_gpu():
         ops.group_norm_act(x, w, w, 4, eps=0.0)
     r = ops.group_norm_act(x, w, w, 4, keep_x=True)
     dy = torch.zeros_like(x)
-    for kw in [dict(dy=dy.half()), dict(dy=dy[:1]), dict(x=x[:, :2]), dict(mean=r.mean[:1]), dict(rstd=r.rstd.double()),
+    for kw in [dict(dy=dy.half()), dict(dy=dy[:1]), dict(mean=None), dict(rstd=None), dict(x=x.double()), dict(x=x[:, :2]), dict(mean=r.mean[:1]), dict(rstd=r.rstd.double()),
                dict(x=ops.checkpoint8(x[:1])), dict(x=x.cpu())]:
         a = dict(dy=dy, x=x, mean=r.mean, rstd=r.rstd)
         a.update(kw)
