@@ -90,7 +90,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad8_kernel(WgradArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
   const int64_t t0 = (int64_t)split * a.split_rows;
   const int64_t t1 = t0 + a.split_rows < a.rows ? t0 + a.split_rows : a.rows;
-  const int steps = (int)((t1 - t0 + KT - 1) / KT);
 
   typename Piece<T>::raw ra[S::NA];
   uint4 rb[S::NB];
@@ -99,75 +98,88 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad8_kernel(WgradArgs a) {
 #pragma unroll
   for (int v = 0; v < V; ++v) bias[v] = 0.0f;
 
-  // a thread's piece: always the same columns, rows k = first + j * step
+  // A thread's pieces: always the same columns, rows k = first + j * step.  Columns behind the last are
+  // read from the first one instead: they end up in columns of the tile that are not stored.
   constexpr int CA = TM / V, CB = TN / 16;
   const int ca = (tid % CA) * V, ka = tid / CA, cb = (tid % CB) * 16, kb = tid / CB;
   const int nva = a.O - (o0 + ca) < V ? a.O - (o0 + ca) : V;
-  const bool onb = i0 + cb < a.ld8;
-  const T *dy = (const T *)a.dy + o0 + ca;
-  const int8_t *codes = a.codes + i0 + cb;
-  const uint8_t *scales = a.scales + (i0 + cb) / kBlock8;
-
-  auto load = [&](int step) {
-    const int64_t t = t0 + (int64_t)step * KT;
+  const int cola = nva > 0 ? o0 + ca : 0, colb = i0 + cb < a.ld8 ? i0 + cb : 0;
+  const T *dy = (const T *)a.dy + t0 * a.ldy;
+  const int8_t *codes = a.codes + t0 * a.ld8;
+  const uint8_t *scales = a.scales + t0 * a.nb8;
+  // 32-bit offsets from the step's first row; a piece's distance from the first is the same for all threads
+  const uint32_t va = (uint32_t)ka * (uint32_t)a.ldy + cola, vb = (uint32_t)kb * (uint32_t)a.ld8 + colb;
+  const uint32_t vs = (uint32_t)kb * (uint32_t)a.nb8 + colb / kBlock8;
+  // Steps of whole rows run with unconditional loads (their waits then count loads and not worst cases).  A
+  // last piece of a row may run into the row behind it; the steps with the last row of all, and those
+  // that are not full, take guarded loads.
+  const int64_t own_rows = t1 - t0;
+  const int all = (int)((own_rows + KT - 1) / KT);
+  int fast = (int)(own_rows / KT);
+  if (a.O % V != 0 && (a.ldy < V || (t1 == a.rows && own_rows % KT == 0))) fast = a.ldy < V ? 0 : fast - 1;
+  auto load_a = [&](int j, int step) {
+    const T *d = dy + ((int64_t)step * KT + j * (NT / CA)) * a.ldy;
+    ra[j] = *reinterpret_cast<const typename Piece<T>::mem *>(d + va);
+  };
+  auto load_b = [&](int j, int step) {
+    const int64_t row = (int64_t)step * KT + j * (NT / CB);
+    rb[j] = *reinterpret_cast<const uint4 *>(codes + row * a.ld8 + vb);
+    rs[j] = (scales + row * a.nb8)[vs];
+  };
+  auto load_guarded = [&](int step) {
+    const int left = (int)(own_rows - (int64_t)step * KT < KT ? own_rows - (int64_t)step * KT : KT);
 #pragma unroll
     for (int j = 0; j < S::NA; ++j) {
-      const int64_t row = t + ka + j * (NT / CA);
       ra[j] = typename Piece<T>::raw{};
-      if (row < t1 && nva > 0) ra[j] = load_piece<T>(dy + row * a.ldy, nva);
+      if (ka + j * (NT / CA) < left && nva > 0)
+        ra[j] = load_piece<T>(dy + ((int64_t)step * KT + j * (NT / CA)) * a.ldy + va, nva);
     }
 #pragma unroll
     for (int j = 0; j < S::NB; ++j) {
-      const int64_t row = t + kb + j * (NT / CB);
       rb[j] = make_uint4(0, 0, 0, 0);
       rs[j] = 0;
-      if (row < t1 && onb) {
-        rb[j] = *reinterpret_cast<const uint4 *>(codes + row * a.ld8);
-        rs[j] = scales[row * a.nb8];
-      }
+      if (kb + j * (NT / CB) < left) load_b(j, step);
     }
   };
-  auto stage = [&](int step, char *buf) {
+  auto add_bias = [&](int j) {
 #pragma unroll
-    for (int j = 0; j < S::NA; ++j) {
-      const int k = ka + j * (NT / CA);
-      uint16_t out[V][3];
+    for (int v = 0; v < V; ++v) bias[v] += (float)ra[j][v];
+  };
+  auto stage_a = [&](int j, char *buf) {
+    const int k = ka + j * (NT / CA);
+    char *dst = buf + tile_at<TM>(k, ca & ~7) + 2 * (ca & 7);
+    if constexpr (P == 1) {
+      *reinterpret_cast<typename Piece<T>::raw *>(dst) = ra[j];
+    } else {
+      uint16_t out[V][P];
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        if constexpr (P == 1) out[v][0] = __builtin_bit_cast(uint16_t, (T)ra[j][v]);
-        else cut<P>((float)ra[j][v], out[v]);
-      }
-      if (step % a.tx == ix)
-#pragma unroll
-        for (int v = 0; v < V; ++v) bias[v] += (float)ra[j][v];
+      for (int v = 0; v < V; ++v) cut<P>((float)ra[j][v], out[v]);
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         uint32_t w[V / 2];
 #pragma unroll
         for (int v = 0; v < V / 2; ++v) w[v] = out[2 * v][p] | ((uint32_t)out[2 * v + 1][p] << 16);
-        char *dst = buf + p * S::kBytesA + tile_at<TM>(k, ca & ~7) + 2 * (ca & 7);
-        if (V == 8) *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[V / 2 - 2], w[V / 2 - 1]);
-        else *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
+        if constexpr (V == 8) *reinterpret_cast<uint4 *>(dst + p * S::kBytesA) = make_uint4(w[0], w[1], w[2], w[3]);
+        else *reinterpret_cast<uint2 *>(dst + p * S::kBytesA) = make_uint2(w[0], w[1]);
       }
     }
+  };
+  auto stage_b = [&](int j, char *buf) {
     char *bb = buf + P * S::kBytesA;
+    const int k = kb + j * (NT / CB);
+    const float p = pow2_field(rs[j]);
+    const uint32_t src[4] = {rb[j].x, rb[j].y, rb[j].z, rb[j].w};
 #pragma unroll
-    for (int j = 0; j < S::NB; ++j) {
-      const int k = kb + j * (NT / CB);
-      const float p = pow2_field(rs[j]);
-      const uint32_t src[4] = {rb[j].x, rb[j].y, rb[j].z, rb[j].w};
+    for (int h = 0; h < 2; ++h) {
+      uint32_t w[4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t w[4];
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          // (exact in bf16: the upper half of the float is all of it)
-          const uint32_t c = src[2 * h + (v >> 1)] >> (16 * (v & 1));
-          const uint32_t lo = __float_as_uint((float)(int8_t)c * p), hi = __float_as_uint((float)(int8_t)(c >> 8) * p);
-          w[v] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
-        }
-        *reinterpret_cast<uint4 *>(bb + tile_at<TN>(k, cb + 8 * h)) = make_uint4(w[0], w[1], w[2], w[3]);
+      for (int v = 0; v < 4; ++v) {
+        // (exact in bf16: the upper half of the float is all of it)
+        const uint32_t c = src[2 * h + (v >> 1)] >> (16 * (v & 1));
+        const uint32_t lo = __float_as_uint((float)(int8_t)c * p), hi = __float_as_uint((float)(int8_t)(c >> 8) * p);
+        w[v] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
       }
+      *reinterpret_cast<uint4 *>(bb + tile_at<TN>(k, cb + 8 * h)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   };
 
@@ -189,35 +201,81 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad8_kernel(WgradArgs a) {
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 4 * rowbytes));
     return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   };
-  auto compute = [&](char *buf) {
+  // A step is a run of items: one fragment of dY (32 columns, 16 rows, one piece) against the FN fragments
+  // of x.  Fragments are read from LDS two items ahead, those of x a 16-row chunk ahead.  Between the
+  // items the next step's rows, which arrived during the last step, are converted and written to LDS part by
+  // part, and a part's registers at once take the rows of the step after: every load has a whole step.
+  constexpr int kChunks = KT / 16, kPer = P * FM, kItems = kChunks * kPer, kParts = S::NA + S::NB;
+  auto frag_a = [&](char *buf, int t) {
+    const int c = t / kPer, p = (t % kPer) / FM, m = t % FM;
+    return frag(buf + p * S::kBytesA, 2 * TM, 16 * c, wm * FM + m, swa);
+  };
+  auto frag_b = [&](char *buf, int c, int n) { return frag(buf + P * S::kBytesA, 2 * TN, 16 * c, wn * FN + n, swb); };
+  // part j of the rows of `step` to buf
+  auto stage_part = [&](int j, bool sums, char *buf) {
+    if (j < S::NB) {
+      stage_b(j, buf);
+    } else {
+      if (sums) add_bias(j - S::NB);
+      stage_a(j - S::NB, buf);
+    }
+  };
+  // the items of the step in buf; `between(t)` after item t
+  auto multiply = [&](char *buf, auto between) {
+    bf16x8 fa[3], fb[2][FN];
 #pragma unroll
-    for (int k0 = 0; k0 < KT; k0 += 16) {
-      bf16x8 bf[FN];
+    for (int n = 0; n < FN; ++n) fb[0][n] = frag_b(buf, 0, n);
+    fa[0] = frag_a(buf, 0);
+    fa[1] = frag_a(buf, 1);
 #pragma unroll
-      for (int n = 0; n < FN; ++n) bf[n] = frag(buf + P * S::kBytesA, 2 * TN, k0, wn * FN + n, swb);
+    for (int t = 0; t < kItems; ++t) {
+      const int c = t / kPer;
+      if (t + 2 < kItems) fa[(t + 2) % 3] = frag_a(buf, t + 2);
+      if (t % kPer == 0 && c + 1 < kChunks)
 #pragma unroll
-      for (int p = 0; p < P; ++p)
+        for (int n = 0; n < FN; ++n) fb[(c + 1) & 1][n] = frag_b(buf, c + 1, n);
 #pragma unroll
-        for (int m = 0; m < FM; ++m) {
-          const bf16x8 af = frag(buf + p * S::kBytesA, 2 * TM, k0, wm * FM + m, swa);
-#pragma unroll
-          for (int n = 0; n < FN; ++n)
-            acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af, bf[n], acc[m][n], 0, 0, 0);
-        }
+      for (int n = 0; n < FN; ++n)
+        acc[t % FM][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[t % 3], fb[c & 1][n], acc[t % FM][n], 0, 0, 0);
+      between(t);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  load(0);
-  stage(0, lds);
-  __syncthreads();
-  for (int s = 0; s < steps; ++s) {
-    char *cur = lds + (s & 1) * S::kStage, *nxt = lds + ((s & 1) ^ 1) * S::kStage;
-    const bool more = s + 1 < steps;
-    if (more) load(s + 1);
-    compute(cur);
-    if (more) stage(s + 1, nxt);
+  if (fast > 0) {
+    const int last = fast - 1;      // (loads behind it repeat its rows, which are staged and not read)
+#pragma unroll
+    for (int j = 0; j < kParts; ++j) j < S::NB ? load_b(j, 0) : load_a(j - S::NB, 0);
+#pragma unroll
+    for (int j = 0; j < kParts; ++j) {
+      stage_part(j, ix == 0, lds);
+      j < S::NB ? load_b(j, last < 1 ? last : 1) : load_a(j - S::NB, last < 1 ? last : 1);
+    }
     __syncthreads();
+    for (int s = 0; s < fast; ++s) {
+      char *cur = lds + (s & 1) * S::kStage, *nxt = lds + ((s & 1) ^ 1) * S::kStage;
+      const bool sums = (s + 1) % a.tx == ix && s + 1 < fast;
+      const int ahead = s + 2 < last ? s + 2 : last;
+      multiply(cur, [&](int t) {
+#pragma unroll
+        for (int j = 0; j < kParts; ++j)
+          if (t == j * kItems / kParts) {
+            stage_part(j, sums, nxt);
+            j < S::NB ? load_b(j, ahead) : load_a(j - S::NB, ahead);
+          }
+      });
+      __syncthreads();
+    }
   }
+  for (int s = fast; s < all; ++s) {
+    load_guarded(s);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kParts; ++j) stage_part(j, s % a.tx == ix, lds);
+    __syncthreads();
+    multiply(lds, [](int) {});
+  }
+  __syncthreads();
 
   const bool whole = a.splits == 1;
   float *part = a.part + (int64_t)split * a.O * a.I;
@@ -366,7 +424,7 @@ int gvae_linear_wgrad8(const void *d_dy, int dtype, int64_t row_stride, const in
                (long long)row_stride);
   const WgradShape sh = wgrad_shape(rows, O, I);
   GVAE_REQUIRE(O <= (1 << 20) && I <= (1 << 20) && (int64_t)sh.tx * sh.ty * sh.splits < (1LL << 31) &&
-                   sh.split_rows < (1LL << 36) && (int64_t)O * I < (1LL << 36), GVAE_ELIMIT,
+                   row_stride < (1LL << 26) && (sh.split_rows < (1LL << 31)) && (int64_t)O * I < (1LL << 36), GVAE_ELIMIT,
                "linear_wgrad8: %lld rows, %d x %d weights", (long long)rows, O, I);
   WgradArgs a;
   a.dy = d_dy; a.codes = d_codes; a.scales = d_scales; a.dw = d_dw; a.db = d_db;
