@@ -54,6 +54,7 @@ struct NormArgs {
   int graph_step;             // resident backward: graphs walked in steps of this
   int join;                   // resident: lanes (a power of two) that add up one group
   int ld8, nb8;
+  bool past;                  // large results: nontemporal stores
 };
 
 __device__ __forceinline__ int live_rows(const NormArgs &a, int b) {

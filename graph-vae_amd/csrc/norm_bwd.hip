@@ -134,7 +134,7 @@ __global__ __launch_bounds__(NT) void norm_bwd_resident_kernel(NormArgs a) {
         const float h = (x[u].at(v) - mean[e]) * rstd[e];
         dx[v] = i < live ? rstd[e] * __fmaf_rn(dz[u][v], w[v], -__fmaf_rn(h, a2[e], a1[e])) : 0.0f;
       }
-      store_piece<T>((T *)a.out + ((int64_t)b * a.N + i) * a.C + c0, dx, nv);
+      store_piece<T>((T *)a.out + ((int64_t)b * a.N + i) * a.C + c0, dx, nv, a.past);
     }
   }
   // this work-group's row of partial sums
@@ -303,7 +303,7 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_apply_kernel(NormArgs a) {
         const float dz = (float)g[u][v] * act_slope<ACT>(pre_act<ACT>(h, k.w[v], k.b[v]));
         dx[v] = i < live ? k.rstd[v] * __fmaf_rn(dz, k.w[v], -__fmaf_rn(h, a2[v], a1[v])) : 0.0f;
       }
-      store_piece<T>((T *)a.out + ((int64_t)p.b * a.N + i) * a.C + p.c0, dx, p.nv);
+      store_piece<T>((T *)a.out + ((int64_t)p.b * a.N + i) * a.C + p.c0, dx, p.nv, a.past);
     }
   }
 }
@@ -379,6 +379,7 @@ int gvae_group_norm_bwd(const void *d_dy, int dtype, int64_t dy_batch_stride, in
   a.mean = const_cast<float *>(d_mean); a.rstd = const_cast<float *>(d_rstd);   // (read only in the backward)
   a.B = B; a.N = N; a.C = C; a.G = G; a.cpg = C / G;
   a.ld8 = ckpt8_ld(C); a.nb8 = ckpt8_blocks(C);
+  a.past = (int64_t)B * N * C * dtype_bytes(dtype) >= kPastCaches;
   a.act = act;
   hipStream_t s = (hipStream_t)stream;
   const int V = 16 / dtype_bytes(dtype);

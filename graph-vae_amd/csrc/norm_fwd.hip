@@ -105,12 +105,12 @@ __global__ __launch_bounds__(NT) void norm_resident_kernel(NormArgs a) {
 #pragma unroll
     for (int v = 0; v < V; ++v) y[v] = i < live && v < nv ? (float)(T)y[v] : 0.0f;
     const int64_t row = (int64_t)b * a.N + i;
-    if (nv > 0) store_piece<T>((T *)a.out + row * a.C + c0, y, nv);
+    if (nv > 0) store_piece<T>((T *)a.out + row * a.C + c0, y, nv, a.past);
     // (the lanes of a block share a row: with checkpoints kept, `lanes` is a whole number of blocks)
     const int nc = a.ld8 - c0;
     const bool first = c0 % kBlock8 == 0 && nv > 0;
-    if (a.x8) emit8<V>(xf, a.x8 + row * a.ld8 + c0, nc, a.x8s + row * a.nb8 + c0 / kBlock8, first);
-    if (a.y8) emit8<V>(y, a.y8 + row * a.ld8 + c0, nc, a.y8s + row * a.nb8 + c0 / kBlock8, first);
+    if (a.x8) emit8<V>(xf, a.x8 + row * a.ld8 + c0, nc, a.x8s + row * a.nb8 + c0 / kBlock8, first, a.past);
+    if (a.y8) emit8<V>(y, a.y8 + row * a.ld8 + c0, nc, a.y8s + row * a.nb8 + c0 / kBlock8, first, a.past);
   }
 }
 
@@ -256,12 +256,12 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(NormArgs a) {
                    ? (float)(T)act_value<ACT>(pre_act<ACT>((xf[v] - k.mean[v]) * k.rstd[v], k.w[v], k.b[v])) : 0.0f;
       }
       const int64_t row = (int64_t)p.b * a.N + i;
-      if (p.nv > 0) store_piece<T>((T *)a.out + row * a.C + p.c0, y, p.nv);
+      if (p.nv > 0) store_piece<T>((T *)a.out + row * a.C + p.c0, y, p.nv, a.past);
       // (the lanes of a block share a row: with checkpoints kept, `lanes` is a whole number of blocks)
       const int nc = a.ld8 - p.c0;
       const bool first = p.c0 % kBlock8 == 0 && p.nv > 0;
-      if (a.x8) emit8<V>(xf, a.x8 + row * a.ld8 + p.c0, nc, a.x8s + row * a.nb8 + p.c0 / kBlock8, first);
-      if (a.y8) emit8<V>(y, a.y8 + row * a.ld8 + p.c0, nc, a.y8s + row * a.nb8 + p.c0 / kBlock8, first);
+      if (a.x8) emit8<V>(xf, a.x8 + row * a.ld8 + p.c0, nc, a.x8s + row * a.nb8 + p.c0 / kBlock8, first, a.past);
+      if (a.y8) emit8<V>(y, a.y8 + row * a.ld8 + p.c0, nc, a.y8s + row * a.nb8 + p.c0 / kBlock8, first, a.past);
     }
   }
 }
@@ -335,6 +335,7 @@ int gvae_group_norm_fwd(const void *d_x, int dtype, int64_t batch_stride, int64_
   a.x8 = d_x8; a.x8s = d_x8_scales; a.y8 = d_y8; a.y8s = d_y8_scales;
   a.B = B; a.N = N; a.C = C; a.G = G; a.cpg = C / G;
   a.ld8 = ckpt8_ld(C); a.nb8 = ckpt8_blocks(C);
+  a.past = (int64_t)B * N * C * dtype_bytes(dtype) >= kPastCaches;
   a.act = act;
   const int V = 16 / dtype_bytes(dtype);
   const NormPlan plan = norm_plan(false, dtype, B, N, C, G, d_x8 || d_y8);

@@ -356,19 +356,23 @@ struct WgradShape {
   int tm, tx, ty, splits;
   int64_t split_rows;
 };
-// A tile of 256 x 256 where both sides fill one and the rows are many, else of 128 x 128; of 64 x 64
-// where the larger ones would leave most of the chip without a work-group.  Rows are split until
-// there is a work-group for each CU (two of the smaller ones), no range shorter than 128 rows.
+// Larger tiles need fewer bytes and conversions per product, smaller ones fill the chip sooner.  Measured
+// (us, tiles of 64 / 128 / 256): 8192 rows of 256 x 256 float 18 / 23 / 29; 4096 x 1024 x 1024 bf16
+// 31 / 28 / 34; 50001 x 515 x 387 half 124 / 107 / 98; 65536 x 1024 x 1024 bf16 277 / 170 / 142; 100000 x
+// 64 x 64 float 18 / 28 / 46.  So: 256 from 200000 rows times tiles on, 64 below 100000 or where a side has
+// no more than 64.  Rows are split until there is a work-group for each CU (two of the smaller ones; one
+// range where that makes half of them already), no range shorter than 128 rows.
 static WgradShape wgrad_shape(int64_t rows, int O, int I) {
   WgradShape s;
-  const int64_t most = (rows + 127) / 128;
+  auto tiles_of = [&](int tm) { return (int64_t)ceil_div(I, tm) * ceil_div(O, tm); };
   s.tm = 128;
-  if (O >= 256 && I >= 256 && rows >= 1024) s.tm = 256;
-  else if ((int64_t)ceil_div(I, 128) * ceil_div(O, 128) * most < 256) s.tm = 64;
+  if (O >= 256 && I >= 256 && tiles_of(256) * rows >= 200000) s.tm = 256;
+  else if (O <= 64 || I <= 64 || tiles_of(128) * rows < 100000) s.tm = 64;
   s.tx = ceil_div(I, s.tm);
   s.ty = ceil_div(O, s.tm);
   const int64_t tiles = (int64_t)s.tx * s.ty, fill = s.tm == 256 ? 256 : 512;
-  int64_t want = tiles >= fill ? 1 : fill / tiles;
+  int64_t want = tiles >= fill / 2 ? 1 : fill / tiles;
+  const int64_t most = (rows + 127) / 128;
   if (want > most) want = most;
   s.split_rows = ((rows + want - 1) / want + 63) / 64 * 64;
   s.splits = (int)((rows + s.split_rows - 1) / s.split_rows);
