@@ -15,10 +15,9 @@ struct Ckpt8Args {
   int64_t rows, ld;
   int C, ld8, nb8, lanes;   // lanes: pieces of a row, whole blocks
   int group_rows;           // rows of a work-group
-  bool past;                // large results: nontemporal stores
 };
 
-template <class T>
+template <class T, bool PAST>
 __global__ __launch_bounds__(256) void ckpt8_write_kernel(Ckpt8Args a) {
   constexpr int V = Piece<T>::V;
   const int64_t row0 = (int64_t)blockIdx.x * a.group_rows;
@@ -32,12 +31,11 @@ __global__ __launch_bounds__(256) void ckpt8_write_kernel(Ckpt8Args a) {
     float f[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) f[v] = (float)r[v];
-    emit8<V>(f, a.codes + row * a.ld8 + c0, a.ld8 - c0, a.scales + row * a.nb8 + c0 / kBlock8, c0 % kBlock8 == 0,
-             a.past);
+    emit8<PAST, V>(f, a.codes + row * a.ld8 + c0, a.ld8 - c0, a.scales + row * a.nb8 + c0 / kBlock8, c0 % kBlock8 == 0);
   }
 }
 
-template <class T>
+template <class T, bool PAST>
 __global__ __launch_bounds__(256) void ckpt8_read_kernel(Ckpt8Args a) {
   constexpr int V = Piece<T>::V;
   const int64_t row0 = (int64_t)blockIdx.x * a.group_rows;
@@ -53,7 +51,7 @@ __global__ __launch_bounds__(256) void ckpt8_read_kernel(Ckpt8Args a) {
     if (std::is_same<T, f16_t>::value)
 #pragma unroll
       for (int v = 0; v < V; ++v) f[v] = f[v] == f[v] ? fminf(fmaxf(f[v], -65504.0f), 65504.0f) : f[v];
-    store_piece<T>((T *)a.x + row * a.ld + c0, f, nv, a.past);
+    store_piece<PAST, T>((T *)a.x + row * a.ld + c0, f, nv);
   }
 }
 
@@ -62,7 +60,7 @@ __global__ __launch_bounds__(256) void ckpt8_read_kernel(Ckpt8Args a) {
 using namespace gvae;
 
 static int ckpt8_args(const char *who, void *x, int dtype, int64_t rows, int C, int64_t ld, int8_t *codes,
-                      uint8_t *scales, int out_bytes, Ckpt8Args *a) {
+                      uint8_t *scales, Ckpt8Args *a) {
   GVAE_REQUIRE(x && codes && scales, GVAE_EINVAL, "%s: null pointer", who);
   GVAE_REQUIRE(dtype_known(dtype), GVAE_EINVAL, "%s: unknown element type %d", who, dtype);
   GVAE_REQUIRE(rows > 0 && C > 0 && ld >= C, GVAE_EINVAL, "%s: bad sizes (rows=%lld channels=%d stride=%lld)", who,
@@ -70,7 +68,6 @@ static int ckpt8_args(const char *who, void *x, int dtype, int64_t rows, int C, 
   GVAE_REQUIRE(C <= (1 << 24), GVAE_ELIMIT, "%s: %d channels", who, C);
   a->x = x; a->codes = codes; a->scales = scales; a->rows = rows; a->ld = ld;
   a->C = C; a->ld8 = ckpt8_ld(C); a->nb8 = ckpt8_blocks(C); a->lanes = a->nb8 * (kBlock8 * dtype_bytes(dtype) / 16);
-  a->past = rows * C * out_bytes >= kPastCaches;
   // about four pieces a thread, at least one row
   a->group_rows = a->lanes >= 1024 ? 1 : 1024 / a->lanes;
   GVAE_REQUIRE((rows + a->group_rows - 1) / a->group_rows < (1LL << 31), GVAE_ELIMIT, "%s: %lld rows", who,
@@ -86,10 +83,13 @@ int gvae_ckpt8_row_scales(int C) { return C > 0 ? ckpt8_blocks(C) : 0; }
 int gvae_ckpt8_write(const void *d_x, int dtype, int64_t rows, int C, int64_t row_stride, int8_t *d_codes,
                      uint8_t *d_scales, void *stream) {
   Ckpt8Args a;
-  if (int rc = ckpt8_args("ckpt8_write", const_cast<void *>(d_x), dtype, rows, C, row_stride, d_codes, d_scales, 1, &a))
+  if (int rc = ckpt8_args("ckpt8_write", const_cast<void *>(d_x), dtype, rows, C, row_stride, d_codes, d_scales, &a))
     return rc;
   const dim3 grid((unsigned)((rows + a.group_rows - 1) / a.group_rows));
-  GVAE_DTYPE_SWITCH(dtype, T, hipLaunchKernelGGL((ckpt8_write_kernel<T>), grid, dim3(256), 0, (hipStream_t)stream, a));
+  GVAE_DTYPE_SWITCH(dtype, T, {
+    auto kernel = rows * C >= kPastCaches ? ckpt8_write_kernel<T, true> : ckpt8_write_kernel<T, false>;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, a);
+  });
   return check_launch("ckpt8_write");
 }
 
@@ -97,10 +97,13 @@ int gvae_ckpt8_read(const int8_t *d_codes, const uint8_t *d_scales, int64_t rows
                     int64_t row_stride, void *stream) {
   Ckpt8Args a;
   if (int rc = ckpt8_args("ckpt8_read", d_x, dtype, rows, C, row_stride, const_cast<int8_t *>(d_codes),
-                          const_cast<uint8_t *>(d_scales), dtype_bytes(dtype), &a))
+                          const_cast<uint8_t *>(d_scales), &a))
     return rc;
   const dim3 grid((unsigned)((rows + a.group_rows - 1) / a.group_rows));
-  GVAE_DTYPE_SWITCH(dtype, T, hipLaunchKernelGGL((ckpt8_read_kernel<T>), grid, dim3(256), 0, (hipStream_t)stream, a));
+  GVAE_DTYPE_SWITCH(dtype, T, {
+    auto kernel = rows * C * (int64_t)sizeof(T) >= kPastCaches ? ckpt8_read_kernel<T, true> : ckpt8_read_kernel<T, false>;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, a);
+  });
   return check_launch("ckpt8_read");
 }
 

@@ -60,17 +60,18 @@ __device__ __forceinline__ void keep_raw(typename Piece<T>::raw &r) {
 
 // Results of this size or more are stored past the caches (nontemporal): they would not stay there for
 // their reader, and what is still to be read would make room for them.  Measured: group norm of 192 graphs of
-// 1000 rows, 512 channels, bf16 (197 MB) 107 -> 95 us; a few MB are the same or 5 % slower.
+// 1000 rows, 512 channels, bf16 (197 MB) 111 -> 104 us, its backward 215 -> 203; 4 graphs of 65536 rows,
+// 320 channels 111 -> 99; a few MB are the same or 5 % slower.
 constexpr int64_t kPastCaches = 64LL << 20;
 
-template <class T>
-__device__ __forceinline__ void store_piece(T *p, const float *f, int nv, bool past) {
+template <bool PAST, class T>
+__device__ __forceinline__ void store_piece(T *p, const float *f, int nv) {
   constexpr int V = Piece<T>::V;
   typename Piece<T>::raw r;
 #pragma unroll
   for (int v = 0; v < V; ++v) r[v] = (T)f[v];
   if (nv == V) {
-    if (past) __builtin_nontemporal_store(r, reinterpret_cast<typename Piece<T>::mem *>(p));
+    if (PAST) __builtin_nontemporal_store(r, reinterpret_cast<typename Piece<T>::mem *>(p));
     else *reinterpret_cast<typename Piece<T>::mem *>(p) = r;
     return;
   }
@@ -103,9 +104,8 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t absmax) {
 // V values of a row's block, spread over W = 32 / V neighbouring lanes that all make this call:
 // codes to `codes` (ld bytes a row, nc of this lane's places inside it) and the block's byte.
 // Places behind the last channel are given as 0.
-template <int V>
-__device__ __forceinline__ void emit8(const float *f, int8_t *codes, int nc, uint8_t *scale, bool first,
-                                      bool past) {
+template <bool PAST, int V>
+__device__ __forceinline__ void emit8(const float *f, int8_t *codes, int nc, uint8_t *scale, bool first) {
   uint32_t m = 0;
 #pragma unroll
   for (int v = 0; v < V; ++v) m = max(m, __float_as_uint(f[v]) & 0x7fffffffu);
@@ -128,7 +128,7 @@ __device__ __forceinline__ void emit8(const float *f, int8_t *codes, int nc, uin
   if (nc >= V) {
     typedef uint32_t words __attribute__((ext_vector_type(V / 4)));
     const words x = __builtin_bit_cast(words, w);
-    if (past) __builtin_nontemporal_store(x, reinterpret_cast<words *>(codes));
+    if (PAST) __builtin_nontemporal_store(x, reinterpret_cast<words *>(codes));
     else *reinterpret_cast<words *>(codes) = x;
   }
   if (first) *scale = (uint8_t)s;

@@ -134,7 +134,7 @@ __global__ __launch_bounds__(NT) void norm_bwd_resident_kernel(NormArgs a) {
         const float h = (x[u].at(v) - mean[e]) * rstd[e];
         dx[v] = i < live ? rstd[e] * __fmaf_rn(dz[u][v], w[v], -__fmaf_rn(h, a2[e], a1[e])) : 0.0f;
       }
-      store_piece<T>((T *)a.out + ((int64_t)b * a.N + i) * a.C + c0, dx, nv, a.past);
+      store_piece<false, T>((T *)a.out + ((int64_t)b * a.N + i) * a.C + c0, dx, nv);
     }
   }
   // this work-group's row of partial sums
@@ -267,7 +267,7 @@ __global__ __launch_bounds__(NT) void norm_bwd_join_kernel(NormArgs a, float *dw
 }
 
 // (walked from the last graph to the first: what the sums read last may still be in the caches)
-template <class T, int ACT, bool KEPT>
+template <class T, int ACT, bool KEPT, bool PAST>
 __global__ __launch_bounds__(kThreads) void norm_bwd_apply_kernel(NormArgs a) {
   constexpr int V = Piece<T>::V;
   const Place<V> p(a, false, true);
@@ -303,7 +303,7 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_apply_kernel(NormArgs a) {
         const float dz = (float)g[u][v] * act_slope<ACT>(pre_act<ACT>(h, k.w[v], k.b[v]));
         dx[v] = i < live ? k.rstd[v] * __fmaf_rn(dz, k.w[v], -__fmaf_rn(h, a2[v], a1[v])) : 0.0f;
       }
-      store_piece<T>((T *)a.out + ((int64_t)p.b * a.N + i) * a.C + p.c0, dx, p.nv, a.past);
+      store_piece<PAST, T>((T *)a.out + ((int64_t)p.b * a.N + i) * a.C + p.c0, dx, p.nv);
     }
   }
 }
@@ -346,7 +346,8 @@ static void norm_bwd_launch(const NormArgs &a, const SplitShape &sh, float *dw, 
     hipLaunchKernelGGL((norm_bwd_join_kernel<64>), joins, dim3(64), 0, s, a, dw, db);
   else
     hipLaunchKernelGGL((norm_bwd_join_kernel<512>), joins, dim3(512), 0, s, a, dw, db);
-  hipLaunchKernelGGL((norm_bwd_apply_kernel<T, ACT, KEPT>), grid, dim3(kThreads), 0, s, a);
+  auto kernel = a.past ? norm_bwd_apply_kernel<T, ACT, KEPT, true> : norm_bwd_apply_kernel<T, ACT, KEPT, false>;
+  hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, a);
 }
 template <class T, bool KEPT>
 static void norm_bwd_act(const NormArgs &a, const SplitShape &sh, int act, float *dw, float *db, hipStream_t s) {

@@ -10,7 +10,7 @@ namespace gvae {
 // One graph and one slab per work-group; K pieces a thread, kept as they were loaded.  Two passes over
 // the registers (mean, then centred squares).  IN: a piece lies inside one group (one entry per
 // thread in LDS), else every channel has its own.
-template <class T, bool IN, int NT, int K>
+template <class T, bool IN, int NT, int K, bool PAST>
 __global__ __launch_bounds__(NT) void norm_resident_kernel(NormArgs a) {
   constexpr int V = Piece<T>::V, E = IN ? 1 : V;
   __shared__ float ent[1][NT * E], grp[2][NT * E];
@@ -105,12 +105,12 @@ __global__ __launch_bounds__(NT) void norm_resident_kernel(NormArgs a) {
 #pragma unroll
     for (int v = 0; v < V; ++v) y[v] = i < live && v < nv ? (float)(T)y[v] : 0.0f;
     const int64_t row = (int64_t)b * a.N + i;
-    if (nv > 0) store_piece<T>((T *)a.out + row * a.C + c0, y, nv, a.past);
+    if (nv > 0) store_piece<PAST, T>((T *)a.out + row * a.C + c0, y, nv);
     // (the lanes of a block share a row: with checkpoints kept, `lanes` is a whole number of blocks)
     const int nc = a.ld8 - c0;
     const bool first = c0 % kBlock8 == 0 && nv > 0;
-    if (a.x8) emit8<V>(xf, a.x8 + row * a.ld8 + c0, nc, a.x8s + row * a.nb8 + c0 / kBlock8, first, a.past);
-    if (a.y8) emit8<V>(y, a.y8 + row * a.ld8 + c0, nc, a.y8s + row * a.nb8 + c0 / kBlock8, first, a.past);
+    if (a.x8) emit8<PAST, V>(xf, a.x8 + row * a.ld8 + c0, nc, a.x8s + row * a.nb8 + c0 / kBlock8, first);
+    if (a.y8) emit8<PAST, V>(y, a.y8 + row * a.ld8 + c0, nc, a.y8s + row * a.nb8 + c0 / kBlock8, first);
   }
 }
 
@@ -129,15 +129,18 @@ __global__ __launch_bounds__(kThreads) void norm_stats_kernel(NormArgs a) {
   for (int v = 0; v < V; ++v) mean[v] = m2[v] = 0.0f;
   if (p.on && p.nv > 0) {
     const T *x = (const T *)a.x + p.b * a.xb + p.c0;
-    for (int i = row0 + p.r; i < p.row_end; i += kBatch * a.rp) {
-      typename Piece<T>::raw k[kBatch];
-      int cnt = 0;
+    typename Piece<T>::raw k[kBatch], ahead[kBatch];
+    auto request = [&](int i, typename Piece<T>::raw *to) {
 #pragma unroll
       for (int u = 0; u < kBatch; ++u)
-        if (i + u * a.rp < p.row_end) {
-          k[u] = load_piece<T>(x + (int64_t)(i + u * a.rp) * a.xr, p.nv);
-          ++cnt;
-        }
+        if (i + u * a.rp < p.row_end) to[u] = load_piece<T>(x + (int64_t)(i + u * a.rp) * a.xr, p.nv);
+    };
+    request(row0 + p.r, ahead);
+    for (int i = row0 + p.r; i < p.row_end; i += kBatch * a.rp) {
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) k[u] = ahead[u];
+      request(i + kBatch * a.rp, ahead);
+      const int left = (p.row_end - i + a.rp - 1) / a.rp, cnt = left < kBatch ? left : kBatch;
       const float inv = 1.0f / (float)cnt;
       const float share = (float)cnt / (float)(n + cnt), cross = (float)n * share;
 #pragma unroll
@@ -190,45 +193,56 @@ __global__ __launch_bounds__(kThreads) void norm_stats_kernel(NormArgs a) {
   }
 }
 
-// mean and 1/sqrt(var + eps) of a group from its chunks' channels, a work-group per group
+// mean and 1/sqrt(var + eps) of a group from its chunks' channels, a work-group per group.  One pass in
+// fp64: sum n mean and sum (M2 + n mean^2), whose difference keeps 2^-53 (mean / deviation)^2.
 template <int NT>
 __global__ __launch_bounds__(NT) void norm_stats_join_kernel(NormArgs a) {
-  __shared__ float sh[NT / 64];
+  __shared__ double sh[2][NT / 64];
   const int64_t q = blockIdx.x;
   const int b = (int)(q / a.G), g = (int)(q - (int64_t)b * a.G);
   const int live = live_rows(a, b), total = a.chunks * a.cpg;
-  auto rows_of = [&](int k) {
+  const float *p1 = a.part1 + (int64_t)b * a.chunks * a.C + g * a.cpg;
+  const float *p2 = a.part2 + (int64_t)b * a.chunks * a.C + g * a.cpg;
+  double s = 0.0, v = 0.0;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < total; e += NT) {
+    const int k = e / a.cpg, c = e - k * a.cpg;
     const int n = live - k * a.chunk_rows;
-    return (float)(n < 0 ? 0 : (n > a.chunk_rows ? a.chunk_rows : n));
-  };
-  const int64_t base = (int64_t)b * a.chunks * a.C + g * a.cpg;
-  float s = 0.0f;
-#pragma unroll 4
-  for (int e = threadIdx.x; e < total; e += NT) {
-    const int k = e / a.cpg, c = e - k * a.cpg;
-    s = __fmaf_rn(rows_of(k), a.part1[base + (int64_t)k * a.C + c], s);
+    const double rows = (double)(n < 0 ? 0 : (n > a.chunk_rows ? a.chunk_rows : n));
+    const double mu = (double)p1[(int64_t)k * a.C + c];
+    s = fma(rows, mu, s);
+    v += fma(rows * mu, mu, (double)p2[(int64_t)k * a.C + c]);
   }
-  s = group_sum<NT>(s, sh);
-  const float m = (float)live * (float)a.cpg;
-  const float mu = live > 0 ? s / m : 0.0f;
-  float v = 0.0f;
-#pragma unroll 4
-  for (int e = threadIdx.x; e < total; e += NT) {
-    const int k = e / a.cpg, c = e - k * a.cpg;
-    const float d = a.part1[base + (int64_t)k * a.C + c] - mu;
-    v += __fmaf_rn(rows_of(k) * d, d, a.part2[base + (int64_t)k * a.C + c]);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    s += __shfl_xor(s, off, 64);
+    v += __shfl_xor(v, off, 64);
   }
-  v = group_sum<NT>(v, sh);
+  if (NT > 64) {
+    if ((threadIdx.x & 63) == 0) {
+      sh[0][threadIdx.x >> 6] = s;
+      sh[1][threadIdx.x >> 6] = v;
+    }
+    __syncthreads();
+    s = v = 0.0;
+    for (int k = 0; k < NT / 64; ++k) {
+      s += sh[0][k];
+      v += sh[1][k];
+    }
+  }
   if (threadIdx.x == 0) {
-    a.mean[q] = mu;
-    a.rstd[q] = 1.0f / sqrtf((live > 0 ? v / m : 0.0f) + a.eps);
+    const double m = (double)(live > 0 ? live : 1) * (double)a.cpg;
+    const double mu = s / m, var = v / m - mu * mu;
+    a.mean[q] = (float)mu;
+    // (an infinity or a NaN in the group: var is NaN and stays one)
+    a.rstd[q] = 1.0f / sqrtf((float)(var < 0.0 ? 0.0 : var) + a.eps);
   }
 }
 
 // Rows of a thread are requested kAhead at a time.  The graphs are walked from the last to the first: what
 // the statistics read last may still be in the caches.
 constexpr int kAhead = 4;
-template <class T, int ACT>
+template <class T, int ACT, bool PAST>
 __global__ __launch_bounds__(kThreads) void norm_apply_kernel(NormArgs a) {
   constexpr int V = Piece<T>::V;
   const Place<V> p(a, false, true);
@@ -256,14 +270,20 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(NormArgs a) {
                    ? (float)(T)act_value<ACT>(pre_act<ACT>((xf[v] - k.mean[v]) * k.rstd[v], k.w[v], k.b[v])) : 0.0f;
       }
       const int64_t row = (int64_t)p.b * a.N + i;
-      if (p.nv > 0) store_piece<T>((T *)a.out + row * a.C + p.c0, y, p.nv, a.past);
+      if (p.nv > 0) store_piece<PAST, T>((T *)a.out + row * a.C + p.c0, y, p.nv);
       // (the lanes of a block share a row: with checkpoints kept, `lanes` is a whole number of blocks)
       const int nc = a.ld8 - p.c0;
       const bool first = p.c0 % kBlock8 == 0 && p.nv > 0;
-      if (a.x8) emit8<V>(xf, a.x8 + row * a.ld8 + p.c0, nc, a.x8s + row * a.nb8 + p.c0 / kBlock8, first, a.past);
-      if (a.y8) emit8<V>(y, a.y8 + row * a.ld8 + p.c0, nc, a.y8s + row * a.nb8 + p.c0 / kBlock8, first, a.past);
+      if (a.x8) emit8<PAST, V>(xf, a.x8 + row * a.ld8 + p.c0, nc, a.x8s + row * a.nb8 + p.c0 / kBlock8, first);
+      if (a.y8) emit8<PAST, V>(y, a.y8 + row * a.ld8 + p.c0, nc, a.y8s + row * a.nb8 + p.c0 / kBlock8, first);
     }
   }
+}
+
+template <class T, int ACT>
+static void apply_launch(const NormArgs &a, dim3 grid, hipStream_t s) {
+  auto kernel = a.past ? norm_apply_kernel<T, ACT, true> : norm_apply_kernel<T, ACT, false>;
+  hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, a);
 }
 
 template <class T, bool IN>
@@ -275,7 +295,8 @@ static void resident_launch(NormArgs &a, hipStream_t s) {
     a.rp = NT / a.lanes;                                                                  \
     a.join = join_lanes(groups, NT);                                                      \
     if ((int64_t)a.rp * K >= a.N) {                                                       \
-      hipLaunchKernelGGL((norm_resident_kernel<T, IN, NT, K>), grid, dim3(NT), 0, s, a);  \
+      auto kernel = a.past ? norm_resident_kernel<T, IN, NT, K, true> : norm_resident_kernel<T, IN, NT, K, false>; \
+      hipLaunchKernelGGL(kernel, grid, dim3(NT), 0, s, a);                                \
       return;                                                                             \
     }                                                                                     \
   } while (0)
@@ -359,10 +380,10 @@ int gvae_group_norm_fwd(const void *d_x, int dtype, int64_t batch_stride, int64_
     if ((int64_t)sh.chunks * a.cpg <= 256) hipLaunchKernelGGL((norm_stats_join_kernel<64>), joins, dim3(64), 0, s, a);
     else hipLaunchKernelGGL((norm_stats_join_kernel<512>), joins, dim3(512), 0, s, a);
     switch (act) {
-      case GVAE_ACT_NONE: hipLaunchKernelGGL((norm_apply_kernel<T, GVAE_ACT_NONE>), grid, dim3(kThreads), 0, s, a); break;
-      case GVAE_ACT_RELU: hipLaunchKernelGGL((norm_apply_kernel<T, GVAE_ACT_RELU>), grid, dim3(kThreads), 0, s, a); break;
-      case GVAE_ACT_SILU: hipLaunchKernelGGL((norm_apply_kernel<T, GVAE_ACT_SILU>), grid, dim3(kThreads), 0, s, a); break;
-      default: hipLaunchKernelGGL((norm_apply_kernel<T, GVAE_ACT_GELU>), grid, dim3(kThreads), 0, s, a); break;
+      case GVAE_ACT_NONE: apply_launch<T, GVAE_ACT_NONE>(a, grid, s); break;
+      case GVAE_ACT_RELU: apply_launch<T, GVAE_ACT_RELU>(a, grid, s); break;
+      case GVAE_ACT_SILU: apply_launch<T, GVAE_ACT_SILU>(a, grid, s); break;
+      default: apply_launch<T, GVAE_ACT_GELU>(a, grid, s); break;
     }
   });
   return check_launch("group_norm_fwd");
