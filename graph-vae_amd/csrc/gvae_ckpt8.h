@@ -80,6 +80,17 @@ __device__ __forceinline__ void store_piece(T *p, const float *f, int nv) {
     if (v < nv) p[v] = r[v];
 }
 
+// the values as they are stored
+template <class T>
+struct rounded {
+  float f[Piece<T>::V];
+  __device__ __forceinline__ explicit rounded(const float *y) {
+#pragma unroll
+    for (int v = 0; v < Piece<T>::V; ++v) f[v] = (float)(T)y[v];
+  }
+  __device__ __forceinline__ operator const float *() const { return f; }
+};
+
 __device__ __forceinline__ float pow2_field(uint32_t field) { return __uint_as_float(field << 23); }
 
 // max over the 2, 4 or 8 neighbouring lanes that share a block (lane groups aligned to their size)

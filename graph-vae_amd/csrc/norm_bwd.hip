@@ -87,9 +87,9 @@ __global__ __launch_bounds__(NT) void norm_bwd_resident_kernel(NormArgs a) {
         act_slopes<V>(a.act, h, w, bias, s);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          dz[u][v] = v < nv ? (float)g[u][v] * s[v] : 0.0f;
+          dz[u][v] = (float)g[u][v] * s[v];
           p1[v] += dz[u][v];
-          p2[v] = v < nv ? __fmaf_rn(dz[u][v], h[v], p2[v]) : 0.0f;
+          p2[v] = __fmaf_rn(dz[u][v], h[v], p2[v]);
         }
       }
     {
@@ -129,11 +129,14 @@ __global__ __launch_bounds__(NT) void norm_bwd_resident_kernel(NormArgs a) {
       if (i >= a.N) break;
       float dx[V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const int e = IN ? 0 : v;
-        const float h = (x[u].at(v) - mean[e]) * rstd[e];
-        dx[v] = i < live ? rstd[e] * __fmaf_rn(dz[u][v], w[v], -__fmaf_rn(h, a2[e], a1[e])) : 0.0f;
-      }
+      for (int v = 0; v < V; ++v) dx[v] = 0.0f;
+      if (i < live)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const int e = IN ? 0 : v;
+          const float h = (x[u].at(v) - mean[e]) * rstd[e];
+          dx[v] = rstd[e] * __fmaf_rn(dz[u][v], w[v], -__fmaf_rn(h, a2[e], a1[e]));
+        }
       store_piece<false, T>((T *)a.out + ((int64_t)b * a.N + i) * a.C + c0, dx, nv);
     }
   }
@@ -165,7 +168,7 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_sums_kernel(NormArgs a) {
 #pragma unroll
   for (int v = 0; v < V; ++v) s1[v] = s2[v] = 0.0f;
   if (p.on && p.nv > 0) {
-    const Scale<V> k(a, p.b, p.c0, p.nv);
+    const Scale<V, sizeof(T) == 2 && ACT != GVAE_ACT_RELU> k(a, p.b, p.c0, p.nv);
     const T *dy = (const T *)a.dy + p.b * a.dyb + p.c0;
     for (int i0 = p.chunk * a.chunk_rows + p.r; i0 < p.row_end; i0 += kAhead * a.rp) {
       typename Piece<T>::raw g[kAhead];
@@ -182,10 +185,10 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_sums_kernel(NormArgs a) {
         if (i0 + u * a.rp >= p.row_end) break;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float h = (x[u].at(v) - k.mean[v]) * k.rstd[v];
-          const float dz = v < p.nv ? (float)g[u][v] * act_slope<ACT>(pre_act<ACT>(h, k.w[v], k.b[v])) : 0.0f;
+          const float h = k.h(v, x[u].at(v));
+          const float dz = (float)g[u][v] * act_slope<ACT>(pre_act<ACT>(h, k.w[v], k.b[v]));
           s1[v] += dz;
-          s2[v] = v < p.nv ? __fmaf_rn(dz, h, s2[v]) : 0.0f;
+          s2[v] = __fmaf_rn(dz, h, s2[v]);
         }
       }
     }
@@ -273,13 +276,14 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_apply_kernel(NormArgs a) {
   const Place<V> p(a, false, true);
   if (!p.on || p.nv <= 0) return;
   const int live = live_rows(a, p.b);
-  const Scale<V> k(a, p.b, p.c0, p.nv);
-  float a1[V], a2[V];
+  const Scale<V, sizeof(T) == 2 && ACT != GVAE_ACT_RELU> k(a, p.b, p.c0, p.nv);
+  float a1[V], a2[V], wr[V];       // dx = dz (w r) - (A1 r + h (A2 r))
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int64_t q = (int64_t)p.b * a.G + (p.c0 + (v < p.nv ? v : 0)) / a.cpg;
-    a1[v] = a.A[2 * q];
-    a2[v] = a.A[2 * q + 1];
+    a1[v] = a.A[2 * q] * k.rstd[v];
+    a2[v] = a.A[2 * q + 1] * k.rstd[v];
+    wr[v] = k.w[v] * k.rstd[v];
   }
   const T *dy = (const T *)a.dy + p.b * a.dyb + p.c0;
   for (int i0 = p.chunk * a.chunk_rows + p.r; i0 < p.row_end; i0 += kAhead * a.rp) {
@@ -298,11 +302,14 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_apply_kernel(NormArgs a) {
       if (i >= p.row_end) break;
       float dx[V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float h = (x[u].at(v) - k.mean[v]) * k.rstd[v];
-        const float dz = (float)g[u][v] * act_slope<ACT>(pre_act<ACT>(h, k.w[v], k.b[v]));
-        dx[v] = i < live ? k.rstd[v] * __fmaf_rn(dz, k.w[v], -__fmaf_rn(h, a2[v], a1[v])) : 0.0f;
-      }
+      for (int v = 0; v < V; ++v) dx[v] = 0.0f;
+      if (i < live)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float h = k.h(v, x[u].at(v));
+          const float dz = (float)g[u][v] * act_slope<ACT>(pre_act<ACT>(h, k.w[v], k.b[v]));
+          dx[v] = __fmaf_rn(dz, wr[v], -__fmaf_rn(h, a2[v], a1[v]));
+        }
       store_piece<PAST, T>((T *)a.out + ((int64_t)p.b * a.N + i) * a.C + p.c0, dx, p.nv);
     }
   }

@@ -71,7 +71,7 @@ __global__ __launch_bounds__(NT) void norm_resident_kernel(NormArgs a) {
       if (on && r0 + u * a.rp < live)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float d = v < nv ? (float)k[u][v] - mean[IN ? 0 : v] : 0.0f;
+          const float d = (float)k[u][v] - mean[IN ? 0 : v];
           s[IN ? 0 : v] = __fmaf_rn(d, d, s[IN ? 0 : v]);
         }
     if (mine >= 0)
@@ -97,20 +97,22 @@ __global__ __launch_bounds__(NT) void norm_resident_kernel(NormArgs a) {
     if (i >= a.N) break;
     float xf[V], y[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      xf[v] = (float)k[u][v];
-      y[v] = (xf[v] - mean[IN ? 0 : v]) * rstd[IN ? 0 : v];
-    }
-    act_values<V>(a.act, y, w, bias, y);
+    for (int v = 0; v < V; ++v) xf[v] = y[v] = 0.0f;
+    if (i < live) {      // (channels behind the last: weight and bias 0, and every activation of 0 is 0)
 #pragma unroll
-    for (int v = 0; v < V; ++v) y[v] = i < live && v < nv ? (float)(T)y[v] : 0.0f;
+      for (int v = 0; v < V; ++v) {
+        xf[v] = (float)k[u][v];
+        y[v] = (xf[v] - mean[IN ? 0 : v]) * rstd[IN ? 0 : v];
+      }
+      act_values<V>(a.act, y, w, bias, y);
+    }
     const int64_t row = (int64_t)b * a.N + i;
     if (nv > 0) store_piece<PAST, T>((T *)a.out + row * a.C + c0, y, nv);
     // (the lanes of a block share a row: with checkpoints kept, `lanes` is a whole number of blocks)
     const int nc = a.ld8 - c0;
     const bool first = c0 % kBlock8 == 0 && nv > 0;
     if (a.x8) emit8<PAST, V>(xf, a.x8 + row * a.ld8 + c0, nc, a.x8s + row * a.nb8 + c0 / kBlock8, first);
-    if (a.y8) emit8<PAST, V>(y, a.y8 + row * a.ld8 + c0, nc, a.y8s + row * a.nb8 + c0 / kBlock8, first);
+    if (a.y8) emit8<PAST, V>(rounded<T>(y), a.y8 + row * a.ld8 + c0, nc, a.y8s + row * a.nb8 + c0 / kBlock8, first);
   }
 }
 
@@ -143,22 +145,26 @@ __global__ __launch_bounds__(kThreads) void norm_stats_kernel(NormArgs a) {
       const int left = (p.row_end - i + a.rp - 1) / a.rp, cnt = left < kBatch ? left : kBatch;
       const float inv = 1.0f / (float)cnt;
       const float share = (float)cnt / (float)(n + cnt), cross = (float)n * share;
+      auto batch = [&](auto whole) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float s = 0.0f;
+        for (int v = 0; v < V; ++v) {
+          float s = 0.0f;
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) if (u < cnt) s += (float)k[u][v];
-        const float mb = s * inv;
-        float q = 0.0f;
+          for (int u = 0; u < kBatch; ++u) if (whole || u < cnt) s += (float)k[u][v];
+          const float mb = s * inv;
+          float q = 0.0f;
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) if (u < cnt) {
-          const float d = (float)k[u][v] - mb;
-          q = __fmaf_rn(d, d, q);
+          for (int u = 0; u < kBatch; ++u) if (whole || u < cnt) {
+            const float d = (float)k[u][v] - mb;
+            q = __fmaf_rn(d, d, q);
+          }
+          const float d = mb - mean[v];
+          mean[v] = __fmaf_rn(d, share, mean[v]);
+          m2[v] += __fmaf_rn(d * d, cross, q);
         }
-        const float d = mb - mean[v];
-        mean[v] = __fmaf_rn(d, share, mean[v]);
-        m2[v] += __fmaf_rn(d * d, cross, q);
-      }
+      };
+      if (cnt == kBatch) batch(std::true_type{});
+      else batch(std::false_type{});
       n += cnt;
     }
   }
@@ -248,7 +254,7 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(NormArgs a) {
   const Place<V> p(a, false, true);
   if (!p.on) return;
   const int live = live_rows(a, p.b);
-  const Scale<V> k(a, p.b, p.c0, p.nv);
+  const Scale<V, sizeof(T) == 2 && ACT != GVAE_ACT_RELU> k(a, p.b, p.c0, p.nv);
   const T *x = (const T *)a.x + p.b * a.xb + p.c0;
   for (int i0 = p.chunk * a.chunk_rows + p.r; i0 < p.row_end; i0 += kAhead * a.rp) {
     typename Piece<T>::raw r[kAhead];
@@ -264,10 +270,13 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(NormArgs a) {
       if (i >= p.row_end) break;
       float xf[V], y[V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        xf[v] = (float)r[u][v];
-        y[v] = i < live && v < p.nv
-                   ? (float)(T)act_value<ACT>(pre_act<ACT>((xf[v] - k.mean[v]) * k.rstd[v], k.w[v], k.b[v])) : 0.0f;
+      for (int v = 0; v < V; ++v) xf[v] = y[v] = 0.0f;
+      if (i < live) {    // (channels behind the last: weight and bias 0, and every activation of 0 is 0)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          xf[v] = (float)r[u][v];
+          y[v] = act_value<ACT>(pre_act<ACT>(k.h(v, xf[v]), k.w[v], k.b[v]));
+        }
       }
       const int64_t row = (int64_t)p.b * a.N + i;
       if (p.nv > 0) store_piece<PAST, T>((T *)a.out + row * a.C + p.c0, y, p.nv);
@@ -275,7 +284,7 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(NormArgs a) {
       const int nc = a.ld8 - p.c0;
       const bool first = p.c0 % kBlock8 == 0 && p.nv > 0;
       if (a.x8) emit8<PAST, V>(xf, a.x8 + row * a.ld8 + p.c0, nc, a.x8s + row * a.nb8 + p.c0 / kBlock8, first);
-      if (a.y8) emit8<PAST, V>(y, a.y8 + row * a.ld8 + p.c0, nc, a.y8s + row * a.nb8 + p.c0 / kBlock8, first);
+      if (a.y8) emit8<PAST, V>(rounded<T>(y), a.y8 + row * a.ld8 + p.c0, nc, a.y8s + row * a.nb8 + p.c0 / kBlock8, first);
     }
   }
 }
