@@ -164,6 +164,37 @@ __device__ __forceinline__ float group_sum(float v, float *sh) {
   return v;
 }
 
+// a (graphs, groups) table at the channels of a piece, 0 behind the last channel
+template <int V>
+__device__ __forceinline__ void per_group(const NormArgs &a, const float *table, int g, int c0, int nv, float *f) {
+  const float *row = table + (int64_t)g * a.G;
+  if (a.cpg % V == 0) {          // (uniform: a piece then lies inside one group)
+    const float one = nv > 0 ? row[c0 / a.cpg] : 0.0f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) f[v] = one;
+    return;
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) f[v] = v < nv ? row[(c0 + v) / a.cpg] : 0.0f;
+}
+
+// V floats of a per-channel parameter (`none` where there is no parameter), 0 behind the last channel
+template <int V>
+__device__ __forceinline__ void load_params(const float *p, int c0, int nv, float none, float *f) {
+  typedef float four __attribute__((ext_vector_type(4), aligned(4)));
+  if (p && nv == V) {
+#pragma unroll
+    for (int h = 0; h < V / 4; ++h) {
+      const four q = *reinterpret_cast<const four *>(p + c0 + 4 * h);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) f[4 * h + v] = q[v];
+    }
+    return;
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) f[v] = v < nv ? (p ? p[c0 + v] : none) : 0.0f;
+}
+
 // What the channels of a piece are scaled and shifted by.  FOLD: `mean` holds -mean * rstd.
 template <int V, bool FOLD>
 struct Scale {
@@ -172,16 +203,13 @@ struct Scale {
     return FOLD ? __fmaf_rn(x, rstd[v], mean[v]) : (x - mean[v]) * rstd[v];
   }
   __device__ Scale(const NormArgs &a, int g, int c0, int nv) {
+    load_params<V>(a.w, c0, nv, 1.0f, w);
+    load_params<V>(a.b, c0, nv, 0.0f, b);
+    per_group<V>(a, a.mean, g, c0, nv, mean);
+    per_group<V>(a, a.rstd, g, c0, nv, rstd);
+    if (FOLD)
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const bool in = v < nv;
-      const int c = in ? c0 + v : 0;
-      const int64_t q = (int64_t)g * a.G + c / a.cpg;
-      rstd[v] = in ? a.rstd[q] : 0.0f;
-      mean[v] = in ? (FOLD ? -a.mean[q] * rstd[v] : a.mean[q]) : 0.0f;
-      w[v] = in && a.w ? a.w[c] : (in ? 1.0f : 0.0f);
-      b[v] = in && a.b ? a.b[c] : 0.0f;
-    }
+      for (int v = 0; v < V; ++v) mean[v] = -mean[v] * rstd[v];
   }
 };
 
@@ -280,7 +308,8 @@ inline SplitShape split_shape(int B, int N, int C, int V, bool whole_blocks) {
 
 // Slab of the resident form.  `align`: channels a slab has to start at a multiple of (32 where
 // checkpoints are written, the piece where one is read); `least`: pieces of a row segment that are worth a
-// memory transaction (4 of 16 bytes; 8 where checkpoints are written, whose segments are half as long);
+// memory transaction (4 of 16 bytes; 8 where checkpoints are written, whose segments are half as long; 1
+// where everything is a few MB and stays in the caches);
 // `threads` and `held`: the largest work-group and the pieces a thread holds in it.  The slab is the
 // widest that leaves 1024 work-groups and has at most 2048 pieces, so that several work-groups share a CU
 // and one's loads run beside another's sums; the narrowest may have 4096.  false: no slab of whole
@@ -332,8 +361,9 @@ struct NormPlan {
 inline NormPlan norm_plan(bool backward, int dtype, int B, int N, int C, int G, bool checkpoints) {
   NormPlan p{};
   const int V = dtype == GVAE_F32 ? 4 : 8, cpg = C / G;
-  p.resident = backward ? resident_shape(B, N, C, cpg, V, checkpoints ? V : 1, 4, 512, 4, &p.rs)
-                        : resident_shape(B, N, C, cpg, V, checkpoints ? kBlock8 : 1, checkpoints ? 8 : 4, 1024, 16, &p.rs);
+  const int least = (int64_t)B * N * C * (16 / V) <= (8 << 20) ? 1 : 4;
+  p.resident = backward ? resident_shape(B, N, C, cpg, V, checkpoints ? V : 1, least, 512, 4, &p.rs)
+                        : resident_shape(B, N, C, cpg, V, checkpoints ? kBlock8 : 1, checkpoints ? 8 : least, 1024, 16, &p.rs);
   if (p.resident) {
     // about 1024 work-groups walk the graphs of the backward
     p.graph_step = p.rs.nslab >= 1024 ? 1 : 1024 / p.rs.nslab;

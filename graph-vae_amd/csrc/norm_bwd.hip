@@ -46,12 +46,10 @@ __global__ __launch_bounds__(NT) void norm_bwd_resident_kernel(NormArgs a) {
   const int mine = (threadIdx.x < a.rp * a.lanes) ? (int)threadIdx.x * E : -1;
   float w[V], bias[V], t1[V], t2[V];
   int group[E];
+  load_params<V>(a.w, c0, nv, 1.0f, w);
+  load_params<V>(a.b, c0, nv, 0.0f, bias);
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    w[v] = v < nv ? (a.w ? a.w[c0 + v] : 1.0f) : 0.0f;
-    bias[v] = v < nv && a.b ? a.b[c0 + v] : 0.0f;
-    t1[v] = t2[v] = 0.0f;
-  }
+  for (int v = 0; v < V; ++v) t1[v] = t2[v] = 0.0f;
 #pragma unroll
   for (int e = 0; e < E; ++e) group[e] = ((c0 + e < s1 ? c0 + e : s1 - 1) - s0) / a.cpg;
   for (int b = lane_b; b < a.B; b += a.graph_step) {

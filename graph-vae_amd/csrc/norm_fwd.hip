@@ -29,11 +29,8 @@ __global__ __launch_bounds__(NT) void norm_resident_kernel(NormArgs a) {
     if (on && i < live) k[u] = load_piece<T>(x + (int64_t)i * a.xr, nv);
   }
   float w[V], bias[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    w[v] = v < nv ? (a.w ? a.w[c0 + v] : 1.0f) : 0.0f;
-    bias[v] = v < nv && a.b ? a.b[c0 + v] : 0.0f;
-  }
+  load_params<V>(a.w, c0, nv, 1.0f, w);
+  load_params<V>(a.b, c0, nv, 0.0f, bias);
   // this thread's entry e of group entries starts at the piece's own group
   const int mine = (threadIdx.x < a.rp * a.lanes) ? (int)threadIdx.x * E : -1;
   const int ge = IN ? a.cpg / V : a.cpg;
