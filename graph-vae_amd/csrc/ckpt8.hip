@@ -70,7 +70,7 @@ static int ckpt8_args(const char *who, void *x, int dtype, int64_t rows, int C, 
   a->C = C; a->ld8 = ckpt8_ld(C); a->nb8 = ckpt8_blocks(C); a->lanes = a->nb8 * (kBlock8 * dtype_bytes(dtype) / 16);
   // about four pieces a thread, at least one row
   a->group_rows = a->lanes >= 1024 ? 1 : 1024 / a->lanes;
-  GVAE_REQUIRE((rows + a->group_rows - 1) / a->group_rows < (1LL << 31), GVAE_ELIMIT, "%s: %lld rows", who,
+  GVAE_REQUIRE((rows + a->group_rows - 1) / a->group_rows < (1LL << 24), GVAE_ELIMIT, "%s: %lld rows", who,
                (long long)rows);
   return GVAE_OK;
 }

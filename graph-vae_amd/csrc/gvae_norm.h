@@ -363,7 +363,7 @@ inline NormPlan norm_plan(bool backward, int dtype, int B, int N, int C, int G, 
   const int V = dtype == GVAE_F32 ? 4 : 8, cpg = C / G;
   const int least = (int64_t)B * N * C * (16 / V) <= (8 << 20) ? 1 : 4;
   p.resident = backward ? resident_shape(B, N, C, cpg, V, checkpoints ? V : 1, least, 512, 4, &p.rs)
-                        : resident_shape(B, N, C, cpg, V, checkpoints ? kBlock8 : 1, checkpoints ? 8 : least, 1024, 16, &p.rs);
+                        : resident_shape(B, N, C, cpg, V, checkpoints ? kBlock8 : 1, checkpoints ? 8 : least, 1024, 8, &p.rs);
   if (p.resident) {
     // about 1024 work-groups walk the graphs of the backward
     p.graph_step = p.rs.nslab >= 1024 ? 1 : 1024 / p.rs.nslab;

@@ -322,7 +322,7 @@ static void params_launch(const NormArgs &a, int64_t rows, float *dw, float *db,
 }
 
 template <class T, bool KEPT, bool IN>
-static void resident_launch(NormArgs &a, hipStream_t s) {
+static bool resident_launch(NormArgs &a, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)a.graph_step * a.nslab));
   const int groups = a.slab / a.cpg;
 #define RUN(NT, K)                                                                                  \
@@ -331,7 +331,7 @@ static void resident_launch(NormArgs &a, hipStream_t s) {
     a.join = join_lanes(groups, NT);                                                                \
     if ((int64_t)a.rp * K >= a.N) {                                                                 \
       hipLaunchKernelGGL((norm_bwd_resident_kernel<T, KEPT, IN, NT, K>), grid, dim3(NT), 0, s, a);  \
-      return;                                                                                       \
+      return true;                                                                                  \
     }                                                                                               \
   } while (0)
   if (a.lanes <= 64) RUN(64, 4);
@@ -341,6 +341,7 @@ static void resident_launch(NormArgs &a, hipStream_t s) {
   }
   RUN(512, 4);
 #undef RUN
+  return false;
 }
 template <class T, int ACT, bool KEPT>
 static void norm_bwd_launch(const NormArgs &a, const SplitShape &sh, float *dw, float *db, hipStream_t s) {
@@ -376,8 +377,7 @@ int gvae_group_norm_bwd(const void *d_dy, int dtype, int64_t dy_batch_stride, in
   GVAE_REQUIRE(!d_x == (d_x8 && d_x8_scales) && !d_x8 == !d_x8_scales, GVAE_EINVAL,
                "group_norm_bwd: give either the input or its checkpoint (codes and scales)");
   if (int rc = norm_check("group_norm_bwd", dtype, B, N, C, G, act, dy_row_stride)) return rc;
-  GVAE_REQUIRE(d_x8 || row_stride >= C, GVAE_EINVAL, "group_norm_bwd: rows of x overlap");
-  GVAE_REQUIRE(dy_batch_stride >= 0 && batch_stride >= 0, GVAE_EINVAL, "group_norm_bwd: negative stride");
+  GVAE_REQUIRE(dy_batch_stride >= 0 && batch_stride >= 0 && row_stride >= 0, GVAE_EINVAL, "group_norm_bwd: negative stride");
   NormArgs a{};
   a.dy = d_dy; a.dyb = dy_batch_stride; a.dyr = dy_row_stride;
   a.x = d_x; a.xb = batch_stride; a.xr = row_stride; a.codes = d_x8; a.scales = d_x8_scales; a.rows = d_rows;
@@ -398,12 +398,12 @@ int gvae_group_norm_bwd(const void *d_dy, int dtype, int64_t dy_batch_stride, in
     a.part1 = direct ? d_dbias : (float *)d_ws;
     a.part2 = direct ? d_dweight : a.part1 + (int64_t)a.graph_step * C;
     const bool in = a.cpg % V == 0;
+    bool ran = false;
     GVAE_DTYPE_SWITCH(dtype, T, {
-      if (d_x8 && in) resident_launch<T, true, true>(a, s);
-      else if (d_x8) resident_launch<T, true, false>(a, s);
-      else if (in) resident_launch<T, false, true>(a, s);
-      else resident_launch<T, false, false>(a, s);
+      if (d_x8) ran = in ? resident_launch<T, true, true>(a, s) : resident_launch<T, true, false>(a, s);
+      else ran = in ? resident_launch<T, false, true>(a, s) : resident_launch<T, false, false>(a, s);
     });
+    GVAE_REQUIRE(ran, GVAE_ELIMIT, "group_norm_bwd: no kernel holds %d rows of %d pieces", N, a.lanes);
     if (d_dweight && !direct) params_launch(a, a.graph_step, d_dweight, d_dbias, s);
     return check_launch("group_norm_bwd");
   }

@@ -293,7 +293,7 @@ static void apply_launch(const NormArgs &a, dim3 grid, hipStream_t s) {
 }
 
 template <class T, bool IN>
-static void resident_launch(NormArgs &a, hipStream_t s) {
+static bool resident_launch(NormArgs &a, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)a.B * a.nslab));
   const int groups = a.slab / a.cpg;
 #define RUN(NT, K)                                                                        \
@@ -303,7 +303,7 @@ static void resident_launch(NormArgs &a, hipStream_t s) {
     if ((int64_t)a.rp * K >= a.N) {                                                       \
       auto kernel = a.past ? norm_resident_kernel<T, IN, NT, K, true> : norm_resident_kernel<T, IN, NT, K, false>; \
       hipLaunchKernelGGL(kernel, grid, dim3(NT), 0, s, a);                                \
-      return;                                                                             \
+      return true;                                                                        \
     }                                                                                     \
   } while (0)
   if (a.lanes <= 64) RUN(64, 4);
@@ -315,6 +315,7 @@ static void resident_launch(NormArgs &a, hipStream_t s) {
   }
   RUN(1024, 8);
 #undef RUN
+  return false;
 }
 
 }  // namespace gvae
@@ -335,9 +336,10 @@ int gvae::norm_check(const char *who, int dtype, int B, int N, int C, int G, int
   GVAE_REQUIRE(B > 0 && N > 0 && C > 0 && G > 0 && C % G == 0, GVAE_EINVAL,
                "%s: bad sizes (graphs=%d rows=%d channels=%d groups=%d)", who, B, N, C, G);
   GVAE_REQUIRE(act >= GVAE_ACT_NONE && act <= GVAE_ACT_GELU, GVAE_EINVAL, "%s: unknown activation %d", who, act);
-  GVAE_REQUIRE(ld >= C, GVAE_EINVAL, "%s: rows overlap (stride %lld for %d channels)", who, (long long)ld, C);
-  GVAE_REQUIRE((int64_t)B * G < (1LL << 31) && (int64_t)N * (C / G) < (1LL << 31) && C <= 65535 * 32 &&
-                   (int64_t)B + 2048 < (1LL << 31), GVAE_ELIMIT,
+  GVAE_REQUIRE(ld >= 0, GVAE_EINVAL, "%s: negative stride", who);
+  // (grids of up to 1024 threads a group or slab stay under 2^32 threads; row numbers and the values of a
+  // group stay under 2^30)
+  GVAE_REQUIRE((int64_t)B * G < (1LL << 22) && (int64_t)N * (C / G) < (1LL << 30) && C <= (1 << 20), GVAE_ELIMIT,
                "%s: too many groups or values per group (graphs=%d rows=%d channels=%d groups=%d)", who, B, N, C, G);
   return GVAE_OK;
 }
@@ -370,10 +372,9 @@ int gvae_group_norm_fwd(const void *d_x, int dtype, int64_t batch_stride, int64_
   if (plan.resident) {
     const ResidentShape &rs = plan.rs;
     a.slab = rs.slab; a.nslab = rs.nslab; a.lanes = rs.lanes;
-    GVAE_DTYPE_SWITCH(dtype, T, {
-      if (a.cpg % V == 0) resident_launch<T, true>(a, s);
-      else resident_launch<T, false>(a, s);
-    });
+    bool ran = false;
+    GVAE_DTYPE_SWITCH(dtype, T, ran = a.cpg % V == 0 ? resident_launch<T, true>(a, s) : resident_launch<T, false>(a, s));
+    GVAE_REQUIRE(ran, GVAE_ELIMIT, "group_norm_fwd: no kernel holds %d rows of %d pieces", N, a.lanes);
     return check_launch("group_norm_fwd");
   }
   const SplitShape &sh = plan.sp;

@@ -427,9 +427,11 @@ int gvae_linear_wgrad8(const void *d_dy, int dtype, int64_t row_stride, const in
                "linear_wgrad8: bad sizes (rows=%lld out=%d in=%d stride=%lld)", (long long)rows, O, I,
                (long long)row_stride);
   const WgradShape sh = wgrad_shape(rows, O, I);
-  GVAE_REQUIRE(O <= (1 << 20) && I <= (1 << 20) && (int64_t)sh.tx * sh.ty * sh.splits < (1LL << 31) &&
-                   row_stride < (1LL << 26) && (sh.split_rows < (1LL << 31)) && (int64_t)O * I < (1LL << 36), GVAE_ELIMIT,
-               "linear_wgrad8: %lld rows, %d x %d weights", (long long)rows, O, I);
+  // (grids under 2^32 threads, offsets within a step under 2^32)
+  GVAE_REQUIRE(O <= (1 << 20) && I <= (1 << 20) && (int64_t)O * I < (1LL << 31) &&
+                   (int64_t)sh.tx * sh.ty * sh.splits < (1LL << 22) && row_stride < (1LL << 26) &&
+                   sh.split_rows < (1LL << 31), GVAE_ELIMIT,
+               "linear_wgrad8: %lld rows, %d x %d weights, stride %lld", (long long)rows, O, I, (long long)row_stride);
   WgradArgs a;
   a.dy = d_dy; a.codes = d_codes; a.scales = d_scales; a.dw = d_dw; a.db = d_db;
   a.rows = rows; a.ldy = row_stride; a.O = O; a.I = I; a.ld8 = ckpt8_ld(I); a.nb8 = ckpt8_blocks(I);

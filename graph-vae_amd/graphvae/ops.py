@@ -104,14 +104,10 @@ def _rows_of(t: torch.Tensor, what: str) -> tuple[int, int]:
                             f"{tuple(t.shape)} with strides {t.stride()}")
 
 
-def _graph_strides(t: torch.Tensor, what: str) -> tuple[int, int]:
+def _graph_strides(t: torch.Tensor) -> tuple[int, int]:
     """(batch stride, row stride) of (graphs, rows, channels); an axis of length 1 has none of its own."""
     B, N, C = t.shape
-    row = t.stride(1) if N > 1 else C
-    batch = t.stride(0) if B > 1 else 0
-    if row < C:
-        raise _hip.GvaeHipError(f"{what}: rows overlap (strides {t.stride()})")
-    return batch, row
+    return (t.stride(0) if B > 1 else 0), (t.stride(1) if N > 1 else C)
 
 
 _NONE = (None, None)
@@ -240,8 +236,8 @@ def group_norm_act(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Ten
     channels.
 
     x: (graphs, rows, channels) float32 / bfloat16 / float16, channels contiguous, any row and batch
-    strides.  weight, bias: (channels,) float32 or None.  act: none | relu | silu | gelu (the erf form).
-    rows: live rows per graph (int32), None = all; rows behind them are not read and come out 0, a
+    strides (expanded axes included).  weight, bias: (channels,) float32 or None.  act: none | relu |
+    silu | gelu (the erf form).  rows: live rows per graph (int32), None = all; rows behind them are not read and come out 0, a
     graph without any has mean 0 and variance 0.  keep_x / keep_y: also return 8-bit checkpoints of x
     (dead rows as 0) and of y, the same as `checkpoint8` of them."""
     what = "group_norm_act"
@@ -249,7 +245,7 @@ def group_norm_act(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Ten
     act_code = _act_code(act)
     index = _on_device(x, what)
     code = _activation(x, what)
-    batch, row = _graph_strides(x, what)
+    batch, row = _graph_strides(x)
     w, b = (_small(weight, (C,), torch.float32, index, what, "weight"),
             _small(bias, (C,), torch.float32, index, what, "bias"))
     live = _small(rows, (B,), torch.int32, index, what, "rows")
@@ -278,7 +274,8 @@ def group_norm_act_backward(dy: torch.Tensor, x, weight: torch.Tensor | None, bi
     """Gradients of `group_norm_act`: (dx, dweight, dbias), dx of dy's type, the others float32 (summed
     over graphs and rows in a fixed order).  x: the forward's input, of dy's type, or its Checkpoint8;
     mean, rstd: as the forward returned them; weight, bias, groups, act, rows: as given to it.  dy: like x
-    of any row and batch strides (an expanded gradient is read in place).  dx of dead rows is 0."""
+    of any row and batch strides (a gradient expanded over graphs or rows is read in place).  dx of dead
+    rows is 0."""
     what = "group_norm_act_backward"
     kept = isinstance(x, Checkpoint8)
     B, N, C = _norm_sizes(dy.shape, groups, what)
@@ -296,9 +293,9 @@ def group_norm_act_backward(dy: torch.Tensor, x, weight: torch.Tensor | None, bi
         if x.dtype is not dy.dtype:
             raise _hip.GvaeHipError(f"{what}: input is {x.dtype}, gradient {dy.dtype}")
         _activation(x, what)
-        xb, xr = _graph_strides(x, what)
+        xb, xr = _graph_strides(x)
         xs, x8, x8s = x.data_ptr(), None, None
-    db_, dr_ = _graph_strides(dy, what)
+    db_, dr_ = _graph_strides(dy)
     w, b = (_small(weight, (C,), torch.float32, index, what, "weight"),
             _small(bias, (C,), torch.float32, index, what, "bias"))
     live = _small(rows, (B,), torch.int32, index, what, "rows")

@@ -403,7 +403,8 @@ int64_t gvae_group_norm_ws_bytes(int backward, int dtype, int B, int N, int C, i
 
 /* y = act(w * (x - mean) / sqrt(var + eps) + b), mean and variance over a graph's live rows and the
  * C/G consecutive channels of a group.
- *   d_x       (B, N, C): unit channel stride, any row stride >= C and batch stride >= 0 (elements)
+ *   d_x       (B, N, C): unit channel stride, any row and batch stride >= 0 (elements; 0 = one row or graph
+ *             for all).  B * G < 2^22, N * C / G < 2^30
  *   d_rows    live rows of each graph, clamped to [0, N]; NULL = N for all.  Rows of x behind them
  *             are not read; their y is 0.  A graph without a live row has mean 0 and variance 0.
  *   d_weight, d_bias   C floats each; NULL = ones / zeros

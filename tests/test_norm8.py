@@ -82,7 +82,7 @@ def _norm_fwd(L, x=16, dtype=0, bs=8, rs=8, B=1, N=1, C=8, G=2, act=1, eps=1e-5,
 
 @pytest.mark.parametrize("bad", [dict(x=None), dict(y=None), dict(ws=None, N=100000), dict(mean=None), dict(dtype=3),
                                  dict(dtype=-1), dict(B=0), dict(N=0), dict(C=0), dict(G=0), dict(G=3), dict(act=4),
-                                 dict(act=-1), dict(rs=7), dict(bs=-8), dict(eps=0.0), dict(eps=float("nan")),
+                                 dict(act=-1), dict(rs=-8), dict(bs=-8), dict(eps=0.0), dict(eps=float("nan")),
                                  dict(eps=float("inf")), dict(x8=16), dict(x8s=16), dict(y8=16), dict(y8s=16)])
 def test_norm_forward_refusals(bad):
     L = _lib()
@@ -94,12 +94,13 @@ def test_norm_limits():
     L = _lib()
     assert _norm_fwd(L, B=1 << 20, G=1 << 12, C=1 << 12, rs=1 << 12) == -3
     assert _norm_fwd(L, N=1 << 24, G=1, C=1 << 8, rs=1 << 8) == -3
+    assert _norm_fwd(L, B=1 << 22, G=1) == -3 and _norm_fwd(L, C=(1 << 20) + 8, rs=1 << 21, G=1) == -3
 
 
 @pytest.mark.parametrize("bad", [dict(dy=None), dict(dx=None), dict(x=None), dict(x8=16, x8s=16), dict(x8=16),
                                  dict(x=None, x8=16), dict(x=None, x8s=16), dict(dw=None), dict(db=None),
                                  dict(mean=None), dict(rstd=None), dict(ws=None), dict(dtype=9), dict(G=3), dict(C=0),
-                                 dict(rs=4), dict(drs=4), dict(bs=-1), dict(dbs=-1), dict(act=7)])
+                                 dict(rs=-1), dict(drs=-4), dict(bs=-1), dict(dbs=-1), dict(act=7)])
 def test_norm_backward_refusals(bad):
     L = _lib()
     k = dict(dy=16, dtype=0, dbs=8, drs=8, x=16, bs=8, rs=8, x8=None, x8s=None, B=1, N=1, C=8, G=2, mean=16, rstd=16,
@@ -127,7 +128,9 @@ def test_checkpoint_and_wgrad_refusals():
               (16, 0, 8, 16, 16, 4, 8, 8, None, 16, 16), (16, 0, 8, 16, 16, 4, 8, 8, 16, 16, None)]:
         assert L.gvae_linear_wgrad8(*a, None) == -1, a
         assert b"linear_wgrad8" in L.gvae_last_error()
-    assert L.gvae_linear_wgrad8(16, 0, 1 << 21, 16, 16, 4, 1 << 21, 8, 16, 16, 16, None) == -3
+    for dy_ld, rows, O, I in [(1 << 21, 4, 1 << 21, 8), (1 << 16, 4, 1 << 16, 1 << 16), (1 << 26, 4, 8, 8)]:
+        assert L.gvae_linear_wgrad8(16, 0, dy_ld, 16, 16, rows, O, I, 16, 16, 16, None) == -3
+    assert L.gvae_ckpt8_write(16, 0, 1 << 40, 1024, 1024, 16, 16, None) == -3
     for n in (L.gvae_group_norm_ws_bytes(1, 0, 0, 1, 1, 1, 0), L.gvae_group_norm_ws_bytes(0, 0, 1, 1, 3, 2, 0), L.gvae_linear_wgrad8_ws_bytes(0, 1, 1)):
         assert n == 0
 
@@ -169,7 +172,7 @@ def test_python_refusals_on_gpu():
     E = _hip.GvaeHipError
     for kw in [dict(x=x.double()), dict(x=x.transpose(1, 2)), dict(x=x[:, :, ::2]), dict(x=x[:0]), dict(w=w[:16]),
                dict(w=w.half()), dict(b=w.cpu()), dict(rows=torch.ones(2, device=dev)),
-               dict(rows=torch.ones(3, dtype=torch.int32, device=dev)), dict(x=x[:, :1].expand(2, 4, 32))]:
+               dict(rows=torch.ones(3, dtype=torch.int32, device=dev))]:
         a = dict(x=x, w=w, b=w, rows=None)
         a.update(kw)
         with pytest.raises(E):
@@ -428,13 +431,15 @@ def test_group_norm_strides(dtype):
     w, b = torch.randn(C, generator=g, device="cuda"), torch.randn(C, generator=g, device="cuda")
     buf = torch.randn(B, N + 3, C + 5, generator=g, device="cuda").to(dtype)
     views = [buf[:, 1:N + 1, 3:3 + C], buf[:, :N, :C], buf.transpose(0, 1)[:B, :B, 1:C + 1],
-             buf[:1, :N, :C].expand(4, N, C), buf[:, :1, 1:1 + C], buf[1:2, 2:3, :C]]
+             buf[:1, :N, :C].expand(4, N, C), buf[:, :1, 1:1 + C], buf[1:2, 2:3, :C], buf[:, :1, :C].expand(B, N, C),
+             buf[:1, :1, 5:5 + C].expand(B, 700, C)]
     for x in views:
         dy = torch.randn(x.shape, generator=g, device="cuda").to(dtype)
         r, c = (ops.group_norm_act(t, w, b, G, act="silu", keep_x=True) for t in (x, x.contiguous()))
         assert torch.equal(r.y, c.y) and torch.equal(r.x8.codes, c.x8.codes)
         one = dy[:, :1, :].expand(x.shape) if x.shape[1] == 1 else dy[:1].expand(x.shape)
-        for gy in (dy, one):
+        rows_one = dy[:, :1, :].expand(x.shape)
+        for gy in (dy, one, rows_one):
             a = ops.group_norm_act_backward(gy, x, w, b, r.mean, r.rstd, G, act="silu")
             e = ops.group_norm_act_backward(gy.contiguous(), x.contiguous(), w, b, r.mean, r.rstd, G, act="silu")
             assert all(torch.equal(p, q) for p, q in zip(a, e))
@@ -799,3 +804,68 @@ def test_group_norm_forms(dtype, shape):
         dx, dw, db, edx, edw, edb = bwd_ref(dy, used, w, b, r.mean.cpu(), r.rstd.cpu(), G, "silu", rows)
         assert ((got[0].cpu().double() - dx).abs() <= half_step(dtype) * dx.abs() + 1.01 * edx + subnormal(dtype)).all()
         assert ((got[1].cpu().double() - dw).abs() <= 2 * edw).all() and ((got[2].cpu().double() - db).abs() <= 2 * edb).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_group_norm_empty_batches_and_row_counts_out_of_range(dtype):
+    """No live row anywhere: zeros everywhere, gradients 0.  Row counts under 0 and over N count as 0 and N."""
+    from graphvae import ops
+    for B, N, C, G in [(2, 7, 24, 3), (2, 9000, 24, 3), (1, 50, 16, 2)]:
+        x, w, b, _, dy = make_x(B, N, C, dtype, 4)
+        x, w, b, dy = x.cuda(), w.cuda(), b.cuda(), dy.cuda()
+        none = torch.zeros(B, dtype=torch.int32, device="cuda")
+        r = ops.group_norm_act(x, w, b, G, act="gelu", rows=none, keep_x=True, keep_y=True)
+        assert not r.y.any() and not r.x8.read().any() and not r.y8.read().any() and not r.mean.any()
+        assert (r.rstd.double() - 1e-5 ** -0.5).abs().max() <= 4 * U32 * 1e-5 ** -0.5
+        for arg in (x, r.x8):
+            got = ops.group_norm_act_backward(dy, arg, w, b, r.mean, r.rstd, G, act="gelu", rows=none)
+            assert not any(t.any() for t in got)
+        odd = torch.tensor([-5, N + 100][:B], dtype=torch.int32, device="cuda")
+        fit = torch.tensor([0, N][:B], dtype=torch.int32, device="cuda")
+        a, e = (ops.group_norm_act(x, w, b, G, rows=k) for k in (odd, fit))
+        assert torch.equal(a.y, e.y) and torch.equal(a.rstd, e.rstd)
+        a, e = (ops.group_norm_act_backward(dy, x, w, b, a.mean, a.rstd, G, rows=k) for k in (odd, fit))
+        assert all(torch.equal(p, q) for p, q in zip(a, e))
+
+
+@gpu
+def test_group_norm_without_parameters():
+    from graphvae import ops
+    for shape in [(3, 40, 48, 6), (2, 9000, 20, 4)]:
+        x, _, _, rows, dy = make_x(*shape[:3], torch.float32, 6)
+        C, G = shape[2:]
+        one, zero = torch.ones(C, device="cuda"), torch.zeros(C, device="cuda")
+        a, e = (ops.group_norm_act(x.cuda(), w, b, G, act="silu", rows=rows.cuda()) for w, b in ((None, None), (one, zero)))
+        assert torch.equal(a.y, e.y)
+        a, e = (ops.group_norm_act_backward(dy.cuda(), x.cuda(), w, b, a.mean, a.rstd, G, act="silu", rows=rows.cuda())
+                for w, b in ((None, None), (one, zero)))
+        assert all(torch.equal(p, q) for p, q in zip(a, e))
+
+
+@gpu
+@pytest.mark.parametrize("scale", [2.0 ** -100, 2.0 ** -60, 2.0 ** 100])
+def test_wgrad_far_exponents(scale):
+    """Gradients far from one keep all their bits: the pieces of an fp32 gradient reach 2^-16 below it, which
+    for 2^-100 is still a normal number."""
+    from graphvae import ops
+    g = torch.Generator().manual_seed(1)
+    dy = torch.randn(1, 64, generator=g) * scale
+    c = ops.checkpoint8(torch.randn(1, 40, generator=g).cuda())
+    dw, db = ops.linear_wgrad8(dy.cuda(), c)
+    want = dy.double().t() @ c.read(torch.float32).cpu().double()
+    assert ((dw.cpu().double() - want).abs() <= 4 * U32 * want.abs()).all() and torch.equal(db.cpu(), dy[0])
+
+
+@gpu
+def test_checkpoint_copies_and_views():
+    import copy
+    from graphvae import ops
+    x = torch.randn(4, 5, 70, device="cuda")
+    c = ops.checkpoint8(x)
+    d = copy.deepcopy(c)
+    want = c.read()
+    c.codes.zero_()
+    assert torch.equal(d.read(), want) and not c.read().any() and d.shape == x.shape and d.dtype == x.dtype
+    e = ops.Checkpoint8(d.codes[1:3], d.scales[1:3], 70, torch.float32)
+    assert torch.equal(e.read(), want[1:3])
