@@ -237,9 +237,9 @@ def group_norm_act(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Ten
 
     x: (graphs, rows, channels) float32 / bfloat16 / float16, channels contiguous, any row and batch
     strides (expanded axes included).  weight, bias: (channels,) float32 or None.  act: none | relu |
-    silu | gelu (the erf form).  rows: live rows per graph (int32), None = all; rows behind them are not read and come out 0, a
-    graph without any has mean 0 and variance 0.  keep_x / keep_y: also return 8-bit checkpoints of x
-    (dead rows as 0) and of y, the same as `checkpoint8` of them."""
+    silu | gelu (the erf form).  rows: live rows per graph (int32), None = all; rows behind them are not read
+    and come out 0, a graph without any has mean 0 and variance 0.  keep_x / keep_y: also return 8-bit
+    checkpoints of x (dead rows as 0) and of y, the same as `checkpoint8` of them."""
     what = "group_norm_act"
     B, N, C = _norm_sizes(x.shape, groups, what)
     act_code = _act_code(act)
