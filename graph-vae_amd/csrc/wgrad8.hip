@@ -24,9 +24,9 @@ struct WgradArgs {
   const int8_t *codes;
   const uint8_t *scales;
   void *dw, *db;
-  float *part, *part_b;       // (splits, O, I) and (splits * tx, O)
+  float *part, *part_b;       // (splits, O, ldp) and (splits * tx, O)
   int64_t rows, ldy;
-  int O, I, ld8, nb8, splits, tx, ty;
+  int O, I, ldp, ld8, nb8, splits, tx, ty;
   int64_t split_rows;
 };
 
@@ -278,7 +278,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad8_kernel(WgradArgs a) {
   __syncthreads();
 
   const bool whole = a.splits == 1;
-  float *part = a.part + (int64_t)split * a.O * a.I;
+  float *part = a.part + (int64_t)split * a.O * a.ldp;
 #pragma unroll
   for (int m = 0; m < FM; ++m)
 #pragma unroll
@@ -289,7 +289,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad8_kernel(WgradArgs a) {
         const int o = o0 + (wm * FM + m) * 32 + (q & 3) + 8 * (q >> 2) + 4 * (lane >> 5);
         if (o < a.O && i < a.I) {
           if (whole) ((T *)a.dw)[(int64_t)o * a.I + i] = (T)acc[m][n][q];
-          else part[(int64_t)o * a.I + i] = acc[m][n][q];
+          else part[(int64_t)o * a.ldp + i] = acc[m][n][q];
         }
       }
     }
@@ -307,16 +307,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad8_kernel(WgradArgs a) {
 }
 
 // The parts of dW (if there is more than one) and of db, in a fixed order: a work-group's 256 threads are
-// PL lanes to a value's parts times lanes of VW neighbouring values.  The first `wide_groups`
-// work-groups sum dW, the others db.
-template <class T, int VW, int PL>
+// PL lanes to a value's parts times lanes of four neighbouring values (rows of a part are whole
+// vectors).  The first `wide_groups` work-groups sum dW, the others db.
+template <class T, int PL>
 __global__ __launch_bounds__(256) void wgrad8_sum_kernel(WgradArgs a, unsigned wide_groups) {
-  typedef float vec __attribute__((ext_vector_type(VW)));
+  typedef float vec __attribute__((ext_vector_type(4)));
   constexpr int L = 256 / PL;
   __shared__ vec sh[PL][L];
   const int lane = threadIdx.x % L, part = threadIdx.x / L;
   if (blockIdx.x < wide_groups) {
-    const int64_t n = (int64_t)a.O * a.I, e = ((int64_t)blockIdx.x * L + lane) * VW;
+    const int64_t n = (int64_t)a.O * a.ldp, e = ((int64_t)blockIdx.x * L + lane) * 4;
     vec s[4] = {};
     if (e < n) {
       int k = part;
@@ -334,9 +334,12 @@ __global__ __launch_bounds__(256) void wgrad8_sum_kernel(WgradArgs a, unsigned w
       for (int k = 1; k < PL; ++k) s[0] += sh[k][lane];
     }
     if (e >= n) return;
-    T *out = (T *)a.dw + e;
+    // (values behind a row's last are whatever the workspace held)
+    const unsigned o = (unsigned)e / (unsigned)a.ldp, i = (unsigned)e - o * (unsigned)a.ldp;
+    T *out = (T *)a.dw + (int64_t)o * a.I + i;
 #pragma unroll
-    for (int v = 0; v < VW; ++v) out[v] = (T)s[0][v];
+    for (int v = 0; v < 4; ++v)
+      if (i + v < (unsigned)a.I) out[v] = (T)s[0][v];
     return;
   }
   const int o = (blockIdx.x - wide_groups) * 16 + (threadIdx.x & 15), p0 = threadIdx.x >> 4, parts = a.splits * a.tx;
@@ -353,22 +356,28 @@ __global__ __launch_bounds__(256) void wgrad8_sum_kernel(WgradArgs a, unsigned w
 }
 
 struct WgradShape {
-  int tm, tx, ty, splits;
+  int tm, tn, tx, ty, splits;
   int64_t split_rows;
 };
 // Larger tiles need fewer bytes and conversions per product, smaller ones fill the chip sooner.  Measured
 // (us, tiles of 64 / 128 / 256): 8192 rows of 256 x 256 float 18 / 23 / 29; 4096 x 1024 x 1024 bf16
 // 31 / 28 / 34; 50001 x 515 x 387 half 124 / 107 / 98; 65536 x 1024 x 1024 bf16 277 / 170 / 142; 100000 x
 // 64 x 64 float 18 / 28 / 46.  So: 256 from 200000 rows times tiles on, 64 below 100000 or where a side has
-// no more than 64.  Rows are split until there is a work-group for each CU (two of the smaller ones; one
+// no more than 64.  Where tiles of 128 x 256 cover dW with 10 % less, they are taken in place of 256 x 256:
+// 50001 x 515 x 387 half 95 / 107, 100000 x 640 x 640 half 211 / 237 (fewer work-groups share a tile of x, so
+// with no less to cover they are slower: 65536 x 1024 x 1024 bf16 162 / 138).  Rows are split until there is a work-group for each CU (two of the smaller ones; one
 // range where that makes half of them already), no range shorter than 128 rows.
 static WgradShape wgrad_shape(int64_t rows, int O, int I) {
   WgradShape s;
-  auto tiles_of = [&](int tm) { return (int64_t)ceil_div(I, tm) * ceil_div(O, tm); };
-  s.tm = 128;
-  if (O >= 256 && I >= 256 && tiles_of(256) * rows >= 200000) s.tm = 256;
-  else if (O <= 64 || I <= 64 || tiles_of(128) * rows < 100000) s.tm = 64;
-  s.tx = ceil_div(I, s.tm);
+  auto tiles_of = [&](int tm, int tn) { return (int64_t)ceil_div(I, tn) * ceil_div(O, tm); };
+  s.tm = s.tn = 128;
+  if (O >= 256 && I >= 256 && tiles_of(256, 256) * rows >= 200000) {
+    s.tn = 256;
+    s.tm = 10 * tiles_of(128, 256) < 9 * 2 * tiles_of(256, 256) ? 128 : 256;
+  } else if (O <= 64 || I <= 64 || tiles_of(128, 128) * rows < 100000) {
+    s.tm = s.tn = 64;
+  }
+  s.tx = ceil_div(I, s.tn);
   s.ty = ceil_div(O, s.tm);
   const int64_t tiles = (int64_t)s.tx * s.ty, fill = s.tm == 256 ? 256 : 512;
   int64_t want = tiles >= fill / 2 ? 1 : fill / tiles;
@@ -378,6 +387,7 @@ static WgradShape wgrad_shape(int64_t rows, int O, int I) {
   s.splits = (int)((rows + s.split_rows - 1) / s.split_rows);
   return s;
 }
+static int wgrad_ldp(int I) { return (I + 3) / 4 * 4; }
 static int64_t wgrad_bias_floats(const WgradShape &s, int O) { return ((int64_t)s.splits * s.tx * O + 3) / 4 * 4; }
 
 template <class T, int FM, int FN, int WM, int WN, int KT>
@@ -392,19 +402,17 @@ static int wgrad_launch(const WgradArgs &a, hipStream_t s) {
   return GVAE_OK;
 }
 
-// many parts: 16 lanes to a value's parts (4 where rows of dW are not whole vectors); few: one
+// many parts: 16 lanes to a value's parts; few: one
 template <class T>
 static void sum_launch(const WgradArgs &a, hipStream_t s) {
-  const int64_t n = a.splits > 1 ? (int64_t)a.O * a.I : 0;
+  const int64_t n = a.splits > 1 ? (int64_t)a.O * a.ldp : 0;
   const unsigned bias_groups = a.db ? ceil_div(a.O, 16) : 0;
   auto run = [&](auto kernel, int values) {
     const unsigned wide = (unsigned)((n + values - 1) / values);
     if (wide + bias_groups > 0) hipLaunchKernelGGL(kernel, dim3(wide + bias_groups), dim3(256), 0, s, a, wide);
   };
-  if (n % 4 == 0 && a.splits <= 8) run(wgrad8_sum_kernel<T, 4, 1>, 1024);
-  else if (n % 4 == 0) run(wgrad8_sum_kernel<T, 4, 16>, 64);
-  else if (a.splits <= 8) run(wgrad8_sum_kernel<T, 1, 1>, 256);
-  else run(wgrad8_sum_kernel<T, 1, 4>, 64);
+  if (a.splits <= 8) run(wgrad8_sum_kernel<T, 1>, 1024);
+  else run(wgrad8_sum_kernel<T, 16>, 64);
 }
 
 }  // namespace gvae
@@ -416,7 +424,7 @@ extern "C" {
 int64_t gvae_linear_wgrad8_ws_bytes(int64_t rows, int O, int I) {
   if (rows <= 0 || O <= 0 || I <= 0) return 0;
   const WgradShape s = wgrad_shape(rows, O, I);
-  return 4 * (wgrad_bias_floats(s, O) + (s.splits > 1 ? (int64_t)s.splits * O * I : 0));
+  return 4 * (wgrad_bias_floats(s, O) + (s.splits > 1 ? (int64_t)s.splits * O * wgrad_ldp(I) : 0));
 }
 
 int gvae_linear_wgrad8(const void *d_dy, int dtype, int64_t row_stride, const int8_t *d_codes, const uint8_t *d_scales,
@@ -434,7 +442,7 @@ int gvae_linear_wgrad8(const void *d_dy, int dtype, int64_t row_stride, const in
                "linear_wgrad8: %lld rows, %d x %d weights, stride %lld", (long long)rows, O, I, (long long)row_stride);
   WgradArgs a;
   a.dy = d_dy; a.codes = d_codes; a.scales = d_scales; a.dw = d_dw; a.db = d_db;
-  a.rows = rows; a.ldy = row_stride; a.O = O; a.I = I; a.ld8 = ckpt8_ld(I); a.nb8 = ckpt8_blocks(I);
+  a.rows = rows; a.ldy = row_stride; a.O = O; a.I = I; a.ldp = wgrad_ldp(I); a.ld8 = ckpt8_ld(I); a.nb8 = ckpt8_blocks(I);
   a.splits = sh.splits; a.split_rows = sh.split_rows; a.tx = sh.tx; a.ty = sh.ty;
   a.part_b = (float *)d_ws;
   a.part = a.part_b + wgrad_bias_floats(sh, O);
@@ -442,7 +450,8 @@ int gvae_linear_wgrad8(const void *d_dy, int dtype, int64_t row_stride, const in
   int rc = GVAE_OK;
   GVAE_DTYPE_SWITCH(dtype, T, {
     constexpr int kDeep = Pieces<T>::P == 1 ? 64 : 32;
-    rc = sh.tm == 256 ? wgrad_launch<T, 4, 2, 2, 4, kDeep>(a, s)
+    rc = sh.tm != sh.tn ? wgrad_launch<T, 4, 2, 1, 4, 32>(a, s)
+         : sh.tm == 256 ? wgrad_launch<T, 4, 2, 2, 4, kDeep>(a, s)
          : sh.tm == 128 ? wgrad_launch<T, 2, 2, 2, 2, kDeep>(a, s) : wgrad_launch<T, 1, 1, 2, 2, 64>(a, s);
     if (rc == GVAE_OK) sum_launch<T>(a, s);
   });

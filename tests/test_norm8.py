@@ -743,7 +743,8 @@ def test_results_repeat_bit_for_bit():
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape", [(1024, 256, 256), (1500, 300, 260), (3001, 515, 387), (70000, 40, 30),
-                                   (20000, 128, 128), (4100, 257, 1000)])
+                                   (20000, 128, 128), (4100, 257, 1000), (100001, 260, 511), (66701, 500, 760),
+                                   (200000, 256, 256)])
 def test_wgrad_large_tiles_and_many_parts(dtype, shape):
     """Sizes that take the larger tiles, several of them, and many row ranges: against 64 bits, and
     small integers exactly."""
