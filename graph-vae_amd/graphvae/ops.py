@@ -53,6 +53,11 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 _empty = torch.empty
 
 
+def _empty_as(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of t's shape, type and device (empty_like is half a microsecond less than empty)."""
+    return torch.empty_like(t) if t.is_contiguous() else _empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _act_code(act: str) -> int:
     code = _ACT.get(act)
     if code is None:
@@ -252,7 +257,7 @@ def group_norm_act(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Ten
     if not eps > 0.0:
         raise ValueError(f"{what}: eps must be positive, got {eps}")
     L, dev = _bound or _bind(), x.device
-    y = _empty((B, N, C), dtype=x.dtype, device=dev)
+    y = _empty_as(x)
     mean, rstd = _empty((2, B, groups), dtype=torch.float32, device=dev).unbind(0)
     x8 = Checkpoint8._new(x.shape, B * N, C, dev, x.dtype) if keep_x else None
     y8 = Checkpoint8._new(x.shape, B * N, C, dev, x.dtype) if keep_y else None
@@ -304,7 +309,7 @@ def group_norm_act_backward(dy: torch.Tensor, x, weight: torch.Tensor | None, bi
     mu, rs = (_small(mean, (B, groups), torch.float32, index, what, "mean"),
               _small(rstd, (B, groups), torch.float32, index, what, "rstd"))
     L, dev = _bound or _bind(), dy.device
-    dx = _empty((B, N, C), dtype=dy.dtype, device=dev)
+    dx = _empty_as(dy)
     dweight, dbias = _empty((2, C), dtype=torch.float32, device=dev).unbind(0)
     ws = _empty(L.gvae_group_norm_ws_bytes(1, code, B, N, C, groups, kept), dtype=torch.uint8, device=dev)
     rc = L.gvae_group_norm_bwd(dy.data_ptr(), code, db_, dr_, xs, xb, xr, x8, x8s, live, B, N, C, groups, w, b, mu, rs,
