@@ -27,7 +27,11 @@ __global__ __launch_bounds__(256) void ckpt8_write_kernel(Ckpt8Args a) {
     const int64_t row = row0 + i;
     const int nv = a.C - c0 < V ? a.C - c0 : V;
     typename Piece<T>::raw r{};
-    if (nv > 0) r = load_piece<T>((const T *)a.x + row * a.ld + c0, nv);
+    if (nv > 0) {
+      const Cut<T> cut(c0, nv, a.C);
+      r = cut.load((const T *)a.x + row * a.ld);
+      cut.cut(r);
+    }
     float f[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) f[v] = (float)r[v];

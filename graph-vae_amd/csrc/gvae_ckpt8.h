@@ -1,5 +1,5 @@
 // Element types, 16-byte row pieces and the 8-bit checkpoint format, shared by the kernels of
-// norm.hip (group norm), ckpt8.hip (checkpoint write / read) and wgrad8.hip (weight gradients).
+// norm_fwd.hip and norm_bwd.hip (group norm), ckpt8.hip (checkpoint write / read) and wgrad8.hip (weight gradients).
 //
 // Checkpoint format.  A row of C values is cut into blocks of 32 consecutive channels.  A block
 // holds one byte s and a signed code per value, value = code * 2^(s - 127), where e = s - 127 is the
@@ -37,16 +37,31 @@ struct Piece {
   typedef raw mem __attribute__((aligned(sizeof(T))));
 };
 
-// nv (1..V) leading elements of the piece at p, zero behind them
+// The elements [c0, c0 + nv) of rows of C, zero behind them, nv in 1..V.  Fewer than V are cut out of a
+// whole piece that lies in the row, in two steps: every load of a thread can be on its way before the
+// first is cut (a cut beside its load waits for it).  Against elements one by one, group norm backward:
+// 300 graphs of 50 rows, 60 channels in groups of 3, bf16 19.0 -> 15.1 us; 37 graphs of 777 rows, 45 channels
+// in groups of 5, half 18.8 -> 16.6.
+typedef unsigned __int128 bits128;
 template <class T>
-__device__ __forceinline__ typename Piece<T>::raw load_piece(const T *p, int nv) {
-  constexpr int V = Piece<T>::V;
-  if (nv == V) return *reinterpret_cast<const typename Piece<T>::mem *>(p);
-  typename Piece<T>::raw r;
+struct Cut {
+  typedef typename Piece<T>::raw raw;
+  static constexpr int V = Piece<T>::V, kBits = 8 * (int)sizeof(T);
+  int c0, nv, C, off;
+  __device__ __forceinline__ Cut(int c0, int nv, int C) : c0(c0), nv(nv), C(C), off(c0 < C - V ? c0 : C - V) {}
+  __device__ __forceinline__ raw load(const T *row) const {
+    if (C >= V) return *reinterpret_cast<const typename Piece<T>::mem *>(row + off);
+    raw r;
 #pragma unroll
-  for (int v = 0; v < V; ++v) r[v] = v < nv ? p[v] : (T)0.0f;
-  return r;
-}
+    for (int v = 0; v < V; ++v) r[v] = v < nv ? row[c0 + v] : (T)0.0f;
+    return r;
+  }
+  __device__ __forceinline__ void cut(raw &r) const {
+    if (nv == V || C < V) return;
+    r = __builtin_bit_cast(raw, (__builtin_bit_cast(bits128, r) >> (kBits * (c0 - off))) &
+                                    (~(bits128)0 >> (kBits * (V - nv))));
+  }
+};
 // A piece held over several passes of a kernel: between two passes the compiler must not keep its
 // values converted to float (twice the registers for 16-bit types) instead of converting again.
 template <class T>
@@ -75,9 +90,22 @@ __device__ __forceinline__ void store_piece(T *p, const float *f, int nv) {
     else *reinterpret_cast<typename Piece<T>::mem *>(p) = r;
     return;
   }
-#pragma unroll
-  for (int v = 0; v < V; ++v)
-    if (v < nv) p[v] = r[v];
+  // (nv in binary: up to three stores)
+  bits128 w = __builtin_bit_cast(bits128, r);
+  auto part = [&](auto kind) {
+    typedef decltype(kind) word __attribute__((aligned(sizeof(T))));
+    *reinterpret_cast<word *>(p) = (word)w;
+    p += sizeof(word) / sizeof(T);
+    w >>= 8 * sizeof(word);
+  };
+  if (sizeof(T) == 2) {
+    if (nv & 4) part((uint64_t)0);
+    if (nv & 2) part((uint32_t)0);
+    if (nv & 1) part((uint16_t)0);
+  } else {
+    if (nv & 2) part((uint64_t)0);
+    if (nv & 1) part((uint32_t)0);
+  }
 }
 
 // the values as they are stored

@@ -284,6 +284,12 @@ __device__ __forceinline__ void join_groups(const float (*ent)[LA], int row_entr
   }
 }
 
+// The group of a slab's channel c (one after the last channel of group g or one of its own), the last
+// group behind the slab
+__device__ __forceinline__ int group_after(int g, int c, int cpg, int ng) {
+  return c >= (g + 1) * cpg && g + 1 < ng ? g + 1 : g;
+}
+
 // Column tiles, row lanes and row chunks of the split form: a row is cut into tiles of at most 256
 // pieces; the rows of a graph are cut so that about 2048 work-groups (eight per CU) share the
 // batch, each with at least kLeast rows per row lane.
@@ -309,7 +315,7 @@ inline SplitShape split_shape(int B, int N, int C, int V, bool whole_blocks) {
 // Slab of the resident form.  `align`: channels a slab has to start at a multiple of (32 where
 // checkpoints are written, the piece where one is read); `least`: pieces of a row segment that are worth a
 // memory transaction (4 of 16 bytes; 8 where checkpoints are written, whose segments are half as long; 1
-// where everything is a few MB and stays in the caches);
+// where everything is a few MB and stays in the caches: there a slab may end inside its one piece);
 // `threads` and `held`: the largest work-group and the pieces a thread holds in it.  The slab is the
 // widest that leaves 1024 work-groups and has at most 2048 pieces, so that several work-groups share a CU
 // and one's loads run beside another's sums; the narrowest may have 4096.  false: no slab of whole
@@ -328,7 +334,7 @@ inline bool resident_shape(int B, int N, int C, int cpg, int V, int align, int l
   auto lanes_of = [&](int64_t slab) { return (int)(((slab + align - 1) / align * align + V - 1) / V); };
   const int64_t want = B >= 1024 ? 1 : (1024 + B - 1) / B;
   int64_t units = ((C + unit - 1) / unit + want - 1) / want;
-  const int64_t fewest = (least * V + unit - 1) / unit;
+  const int64_t fewest = least > 1 ? (least * V + unit - 1) / unit : unit < V ? V / unit : 1;
   if (units < fewest) units = fewest;
   for (;; --units) {
     const int64_t slab = units * unit < C ? units * unit : C;

@@ -10,9 +10,10 @@ namespace gvae {
 template <class T, bool KEPT>
 struct XPiece {
   typename Piece<T>::raw r;
-  __device__ __forceinline__ void load(const NormArgs &a, int b, int i, int c0, int nv) {
-    r = load_piece<T>((const T *)a.x + b * a.xb + (int64_t)i * a.xr + c0, nv);
+  __device__ __forceinline__ void load(const NormArgs &a, int b, int i, int c0, const Cut<T> &cut) {
+    r = cut.load((const T *)a.x + b * a.xb + (int64_t)i * a.xr);
   }
+  __device__ __forceinline__ void cut(const Cut<T> &cut) { cut.cut(r); }
   __device__ __forceinline__ float at(int v) const { return (float)r[v]; }
   __device__ __forceinline__ void keep() { keep_raw<T>(r); }
 };
@@ -21,11 +22,12 @@ struct XPiece<T, true> {
   static constexpr int V = Piece<T>::V;
   Codes<V> c;
   float p;
-  __device__ __forceinline__ void load(const NormArgs &a, int b, int i, int c0, int) {
+  __device__ __forceinline__ void load(const NormArgs &a, int b, int i, int c0, const Cut<T> &) {
     const int64_t row = (int64_t)b * a.N + i;
     c = load_codes<V>(a.codes + row * a.ld8 + c0);
     p = pow2_field(a.scales[row * a.nb8 + c0 / kBlock8]);
   }
+  __device__ __forceinline__ void cut(const Cut<T> &) {}
   __device__ __forceinline__ float at(int v) const { return (float)(int8_t)(c.w[v >> 2] >> (8 * (v & 3))) * p; }
   __device__ __forceinline__ void keep() {
 #pragma unroll
@@ -44,6 +46,7 @@ __global__ __launch_bounds__(NT) void norm_bwd_resident_kernel(NormArgs a) {
   const bool on = r0 < a.rp && nv > 0;
   const int ng = (s1 - s0) / a.cpg, ge = IN ? a.cpg / V : a.cpg;
   const int mine = (threadIdx.x < a.rp * a.lanes) ? (int)threadIdx.x * E : -1;
+  const Cut<T> cut(c0, nv, a.C);
   float w[V], bias[V], t1[V], t2[V];
   int group[E];
   load_params<V>(a.w, c0, nv, 1.0f, w);
@@ -51,18 +54,19 @@ __global__ __launch_bounds__(NT) void norm_bwd_resident_kernel(NormArgs a) {
 #pragma unroll
   for (int v = 0; v < V; ++v) t1[v] = t2[v] = 0.0f;
 #pragma unroll
-  for (int e = 0; e < E; ++e) group[e] = ((c0 + e < s1 ? c0 + e : s1 - 1) - s0) / a.cpg;
+  for (int e = 0; e < E; ++e)
+    group[e] = e == 0 ? (c0 < s1 ? c0 - s0 : 0) / a.cpg : group_after(group[e - 1], c0 + e - s0, a.cpg, ng);
   for (int b = lane_b; b < a.B; b += a.graph_step) {
     const int live = live_rows(a, b);
-    const T *dy = (const T *)a.dy + b * a.dyb + c0;
+    const T *dy = (const T *)a.dy + b * a.dyb;
     typename Piece<T>::raw g[K];
     XPiece<T, KEPT> x[K];
 #pragma unroll
     for (int u = 0; u < K; ++u) {
       const int i = r0 + u * a.rp;
       if (on && i < live) {
-        g[u] = load_piece<T>(dy + (int64_t)i * a.dyr, nv);
-        x[u].load(a, b, i, c0, nv);
+        g[u] = cut.load(dy + (int64_t)i * a.dyr);
+        x[u].load(a, b, i, c0, cut);
       }
     }
     float mean[E], rstd[E];
@@ -80,6 +84,8 @@ __global__ __launch_bounds__(NT) void norm_bwd_resident_kernel(NormArgs a) {
     for (int u = 0; u < K; ++u)
       if (on && r0 + u * a.rp < live) {
         float h[V], s[V];
+        cut.cut(g[u]);
+        x[u].cut(cut);
 #pragma unroll
         for (int v = 0; v < V; ++v) h[v] = (x[u].at(v) - mean[IN ? 0 : v]) * rstd[IN ? 0 : v];
         act_slopes<V>(a.act, h, w, bias, s);
@@ -167,7 +173,8 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_sums_kernel(NormArgs a) {
   for (int v = 0; v < V; ++v) s1[v] = s2[v] = 0.0f;
   if (p.on && p.nv > 0) {
     const Scale<V, sizeof(T) == 2 && ACT != GVAE_ACT_RELU> k(a, p.b, p.c0, p.nv);
-    const T *dy = (const T *)a.dy + p.b * a.dyb + p.c0;
+    const T *dy = (const T *)a.dy + p.b * a.dyb;
+    const Cut<T> cut(p.c0, p.nv, a.C);
     for (int i0 = p.chunk * a.chunk_rows + p.r; i0 < p.row_end; i0 += kAhead * a.rp) {
       typename Piece<T>::raw g[kAhead];
       XPiece<T, KEPT> x[kAhead];
@@ -175,12 +182,14 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_sums_kernel(NormArgs a) {
       for (int u = 0; u < kAhead; ++u) {
         const int i = i0 + u * a.rp;
         if (i >= p.row_end) break;
-        g[u] = load_piece<T>(dy + (int64_t)i * a.dyr, p.nv);
-        x[u].load(a, p.b, i, p.c0, p.nv);
+        g[u] = cut.load(dy + (int64_t)i * a.dyr);
+        x[u].load(a, p.b, i, p.c0, cut);
       }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         if (i0 + u * a.rp >= p.row_end) break;
+        cut.cut(g[u]);
+        x[u].cut(cut);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const float h = k.h(v, x[u].at(v));
@@ -283,7 +292,8 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_apply_kernel(NormArgs a) {
     a2[v] = a.A[2 * q + 1] * k.rstd[v];
     wr[v] = k.w[v] * k.rstd[v];
   }
-  const T *dy = (const T *)a.dy + p.b * a.dyb + p.c0;
+  const T *dy = (const T *)a.dy + p.b * a.dyb;
+  const Cut<T> cut(p.c0, p.nv, a.C);
   for (int i0 = p.chunk * a.chunk_rows + p.r; i0 < p.row_end; i0 += kAhead * a.rp) {
     typename Piece<T>::raw g[kAhead];
     XPiece<T, KEPT> x[kAhead];
@@ -291,8 +301,8 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_apply_kernel(NormArgs a) {
     for (int u = 0; u < kAhead; ++u) {
       const int i = i0 + u * a.rp;
       if (i >= p.row_end || i >= live) break;
-      g[u] = load_piece<T>(dy + (int64_t)i * a.dyr, p.nv);
-      x[u].load(a, p.b, i, p.c0, p.nv);
+      g[u] = cut.load(dy + (int64_t)i * a.dyr);
+      x[u].load(a, p.b, i, p.c0, cut);
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
@@ -301,13 +311,16 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_apply_kernel(NormArgs a) {
       float dx[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) dx[v] = 0.0f;
-      if (i < live)
+      if (i < live) {
+        cut.cut(g[u]);
+        x[u].cut(cut);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const float h = k.h(v, x[u].at(v));
           const float dz = (float)g[u][v] * act_slope<ACT>(pre_act<ACT>(h, k.w[v], k.b[v]));
           dx[v] = __fmaf_rn(dz, wr[v], -__fmaf_rn(h, a2[v], a1[v]));
         }
+      }
       store_piece<PAST, T>((T *)a.out + ((int64_t)p.b * a.N + i) * a.C + p.c0, dx, p.nv);
     }
   }

@@ -20,13 +20,14 @@ __global__ __launch_bounds__(NT) void norm_resident_kernel(NormArgs a) {
   const int c0 = s0 + col * V, nv = s1 - c0 < V ? s1 - c0 : V;
   const bool on = r0 < a.rp && nv > 0;
   const int live = live_rows(a, b), ng = (s1 - s0) / a.cpg, g0 = s0 / a.cpg;
-  const T *x = (const T *)a.x + b * a.xb + c0;
+  const T *x = (const T *)a.x + b * a.xb;
+  const Cut<T> cut(c0, nv, a.C);
   typename Piece<T>::raw k[K];
 #pragma unroll
   for (int u = 0; u < K; ++u) {
     const int i = r0 + u * a.rp;
     k[u] = typename Piece<T>::raw{};
-    if (on && i < live) k[u] = load_piece<T>(x + (int64_t)i * a.xr, nv);
+    if (on && i < live) k[u] = cut.load(x + (int64_t)i * a.xr);
   }
   float w[V], bias[V];
   load_params<V>(a.w, c0, nv, 1.0f, w);
@@ -41,9 +42,11 @@ __global__ __launch_bounds__(NT) void norm_resident_kernel(NormArgs a) {
 #pragma unroll
     for (int e = 0; e < E; ++e) s[e] = 0.0f;
 #pragma unroll
-    for (int u = 0; u < K; ++u)
+    for (int u = 0; u < K; ++u) {
+      if (on) cut.cut(k[u]);
 #pragma unroll
       for (int v = 0; v < V; ++v) s[IN ? 0 : v] += (float)k[u][v];
+    }
     if (mine >= 0)
 #pragma unroll
       for (int e = 0; e < E; ++e) ent[0][mine + e] = s[e];
@@ -53,12 +56,12 @@ __global__ __launch_bounds__(NT) void norm_resident_kernel(NormArgs a) {
   __syncthreads();
   join_groups<1, NT * E, NT * E>(ent, a.lanes * E, ge, ng, a.rp, a.join, NT, grp);
   __syncthreads();
-  auto group_of = [&](int e) {
-    const int c = c0 + e < s1 ? c0 + e : s1 - 1;
-    return (c - s0) / a.cpg;
-  };
+  int group[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) mean[e] = grp[0][group_of(e)] * inv;
+  for (int e = 0; e < E; ++e)
+    group[e] = e == 0 ? (c0 < s1 ? c0 - s0 : 0) / a.cpg : group_after(group[e - 1], c0 + e - s0, a.cpg, ng);
+#pragma unroll
+  for (int e = 0; e < E; ++e) mean[e] = grp[0][group[e]] * inv;
   {
     float s[E];
 #pragma unroll
@@ -81,7 +84,7 @@ __global__ __launch_bounds__(NT) void norm_resident_kernel(NormArgs a) {
   join_groups<1, NT * E, NT * E>(ent, a.lanes * E, ge, ng, a.rp, a.join, NT, grp + 1);
   __syncthreads();
 #pragma unroll
-  for (int e = 0; e < E; ++e) rstd[e] = 1.0f / sqrtf(grp[1][group_of(e)] * inv + a.eps);
+  for (int e = 0; e < E; ++e) rstd[e] = 1.0f / sqrtf(grp[1][group[e]] * inv + a.eps);
   for (int g = threadIdx.x; g < ng; g += NT) {
     const int64_t q = (int64_t)b * a.G + g0 + g;
     a.mean[q] = grp[0][g] * inv;
@@ -127,17 +130,21 @@ __global__ __launch_bounds__(kThreads) void norm_stats_kernel(NormArgs a) {
 #pragma unroll
   for (int v = 0; v < V; ++v) mean[v] = m2[v] = 0.0f;
   if (p.on && p.nv > 0) {
-    const T *x = (const T *)a.x + p.b * a.xb + p.c0;
+    const T *x = (const T *)a.x + p.b * a.xb;
+    const Cut<T> cut(p.c0, p.nv, a.C);
     typename Piece<T>::raw k[kBatch], ahead[kBatch];
     auto request = [&](int i, typename Piece<T>::raw *to) {
 #pragma unroll
       for (int u = 0; u < kBatch; ++u)
-        if (i + u * a.rp < p.row_end) to[u] = load_piece<T>(x + (int64_t)(i + u * a.rp) * a.xr, p.nv);
+        if (i + u * a.rp < p.row_end) to[u] = cut.load(x + (int64_t)(i + u * a.rp) * a.xr);
     };
     request(row0 + p.r, ahead);
     for (int i = row0 + p.r; i < p.row_end; i += kBatch * a.rp) {
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) k[u] = ahead[u];
+      for (int u = 0; u < kBatch; ++u) {
+        k[u] = ahead[u];
+        cut.cut(k[u]);
+      }
       request(i + kBatch * a.rp, ahead);
       const int left = (p.row_end - i + a.rp - 1) / a.rp, cnt = left < kBatch ? left : kBatch;
       const float inv = 1.0f / (float)cnt;
@@ -252,14 +259,15 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(NormArgs a) {
   if (!p.on) return;
   const int live = live_rows(a, p.b);
   const Scale<V, sizeof(T) == 2 && ACT != GVAE_ACT_RELU> k(a, p.b, p.c0, p.nv);
-  const T *x = (const T *)a.x + p.b * a.xb + p.c0;
+  const T *x = (const T *)a.x + p.b * a.xb;
+  const Cut<T> cut(p.c0, p.nv, a.C);
   for (int i0 = p.chunk * a.chunk_rows + p.r; i0 < p.row_end; i0 += kAhead * a.rp) {
     typename Piece<T>::raw r[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int i = i0 + u * a.rp;
       r[u] = typename Piece<T>::raw{};
-      if (i < p.row_end && i < live && p.nv > 0) r[u] = load_piece<T>(x + (int64_t)i * a.xr, p.nv);
+      if (i < p.row_end && i < live && p.nv > 0) r[u] = cut.load(x + (int64_t)i * a.xr);
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
@@ -268,6 +276,7 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(NormArgs a) {
       float xf[V], y[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) xf[v] = y[v] = 0.0f;
+      if (p.nv > 0) cut.cut(r[u]);
       if (i < live) {    // (channels behind the last: weight and bias 0, and every activation of 0 is 0)
 #pragma unroll
         for (int v = 0; v < V; ++v) {

@@ -131,8 +131,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad8_kernel(WgradArgs a) {
 #pragma unroll
     for (int j = 0; j < S::NA; ++j) {
       ra[j] = typename Piece<T>::raw{};
-      if (ka + j * (NT / CA) < left && nva > 0)
-        ra[j] = load_piece<T>(dy + ((int64_t)step * KT + j * (NT / CA)) * a.ldy + va, nva);
+      if (ka + j * (NT / CA) < left && nva > 0) {
+        const Cut<T> cut(cola, nva, a.O);
+        ra[j] = cut.load(dy + ((int64_t)step * KT + j * (NT / CA) + ka) * a.ldy);
+        cut.cut(ra[j]);
+      }
     }
 #pragma unroll
     for (int j = 0; j < S::NB; ++j) {
