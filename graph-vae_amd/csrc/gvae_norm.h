@@ -13,15 +13,16 @@
 // off by 2^-24 |mean r|, where a 16-bit x is itself off by 2^-9 or 2^-12 |x|.
 //
 // The split kernels come near the rate of the vector units before that of memory: a SiLU's slope is 13
-// instructions a value, two of them at a quarter of the rate (backward sums of 16 graphs of 16384 rows, 512
-// channels, bf16: 20 instructions a value and 82 % of the issue slots before the two forms above).
+// instructions a value, two of them at a quarter of the rate.  Backward sums of 16 graphs of 16384 rows, 512
+// channels, bf16, from the checkpoint: 14 instructions a value and 87 us for 406 MB with the two forms
+// above, 20 instructions and 82 % of the issue slots without.
 //
 // All of it is bound by memory.  Two forms each:
 //   resident   a work-group holds a graph's live rows of a run of groups (a slab) in registers: one
 //              read, the sums through LDS, one write.  The slab is as narrow as fills the chip, but
 //              no row segment is under 64 bytes.
 //   split      a group too long for that is summed in chunks of rows by as many work-groups, joined
-//              by one wavefront per group, and read again to be written.
+//              by one wavefront (few chunks) or work-group (many) per group, and read again to be written.
 #pragma once
 #include "gvae_ckpt8.h"
 

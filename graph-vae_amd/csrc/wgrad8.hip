@@ -12,6 +12,11 @@
 // of one column each).  Those 4 rows are brought to different banks by XORing the 64-byte piece of a
 // row with bits of its row number.
 //
+// 65536 rows, 2048 x 2048, bf16: 470 to 500 us, 1100 to 1170 TFLOP/s.  The products and their reads from
+// LDS alone take 390 us of it on random numbers (less on zeros: the clock gives way to the power drawn),
+// conversions and stores to LDS the rest.  Half and float pay for each piece of a gradient with a whole
+// product: 50001 rows, 515 x 387, half 86 us in 128 x 256 tiles that cover 1.65 times dW.
+//
 // A work-group owns a tile of dW and a range of rows; the parts are summed in their order by a second
 // launch.  Column sums of dY ride along: among the work-groups that share a dY tile, each adds up its
 // share of the row steps.
