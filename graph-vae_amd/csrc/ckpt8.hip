@@ -70,6 +70,7 @@ static int ckpt8_args(const char *who, void *x, int dtype, int64_t rows, int C, 
   GVAE_REQUIRE(dtype_known(dtype), GVAE_EINVAL, "%s: unknown element type %d", who, dtype);
   GVAE_REQUIRE(rows > 0 && C > 0 && ld >= C, GVAE_EINVAL, "%s: bad sizes (rows=%lld channels=%d stride=%lld)", who,
                (long long)rows, C, (long long)ld);
+  GVAE_REQUIRE(aligned16(codes), GVAE_EINVAL, "%s: codes are not 16-byte aligned", who);
   GVAE_REQUIRE(C <= (1 << 24), GVAE_ELIMIT, "%s: %d channels", who, C);
   a->x = x; a->codes = codes; a->scales = scales; a->rows = rows; a->ld = ld;
   a->C = C; a->ld8 = ckpt8_ld(C); a->nb8 = ckpt8_blocks(C); a->lanes = a->nb8 * (kBlock8 * dtype_bytes(dtype) / 16);

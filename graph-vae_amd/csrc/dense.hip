@@ -457,7 +457,7 @@ __global__ __launch_bounds__(256) void gcn_adjacency_kernel(const float *__restr
                                                             float *__restrict__ Ahat) {
   __shared__ double dinv[1024];
   const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
-  const int nx = n_x[g], R = Rarr[g];
+  const int nx = n_x[g], R = Rarr[g] < N ? Rarr[g] : N;
   const float *A = adj + (int64_t)g * N * N;
   for (int i = tid >> 6; i < N; i += 4) {       // a wavefront per row
     int cnt = 0;
@@ -488,7 +488,7 @@ __global__ __launch_bounds__(256) void pool_fwd_kernel(const float *__restrict__
                                                        float *__restrict__ gvec) {
   __shared__ double sh[4][64];
   const int cl = threadIdx.x & 63, rl = threadIdx.x >> 6, c = blockIdx.x * 64 + cl, g = blockIdx.y;
-  const int nx = n_x[g];
+  const int nx = n_x[g] < N ? n_x[g] : N;
   double s = 0.0;
   if (c < H)
     for (int i = rl; i < nx; i += 4) s += act[((int64_t)g * N + i) * H + c];

@@ -16,6 +16,7 @@
 namespace gvae {
 
 constexpr int kBlock8 = 32;
+inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 inline int ckpt8_ld(int C) { return (C + 15) / 16 * 16; }
 inline int ckpt8_blocks(int C) { return (C + kBlock8 - 1) / kBlock8; }
 

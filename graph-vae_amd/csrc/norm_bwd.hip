@@ -395,8 +395,11 @@ int gvae_group_norm_bwd(const void *d_dy, int dtype, int64_t dy_batch_stride, in
   GVAE_REQUIRE(!d_dweight == !d_dbias, GVAE_EINVAL, "group_norm_bwd: weight and bias gradients come together");
   GVAE_REQUIRE(!d_x == (d_x8 && d_x8_scales) && !d_x8 == !d_x8_scales, GVAE_EINVAL,
                "group_norm_bwd: give either the input or its checkpoint (codes and scales)");
+  GVAE_REQUIRE(aligned16(d_x8) && aligned16(d_ws), GVAE_EINVAL,
+               "group_norm_bwd: codes or workspace not 16-byte aligned");
   if (int rc = norm_check("group_norm_bwd", dtype, B, N, C, G, act, dy_row_stride)) return rc;
-  GVAE_REQUIRE(dy_batch_stride >= 0 && batch_stride >= 0 && row_stride >= 0, GVAE_EINVAL, "group_norm_bwd: negative stride");
+  GVAE_REQUIRE(dy_batch_stride >= 0 && batch_stride >= 0 && row_stride >= 0, GVAE_EINVAL,
+               "group_norm_bwd: negative stride");
   NormArgs a{};
   a.dy = d_dy; a.dyb = dy_batch_stride; a.dyr = dy_row_stride;
   a.x = d_x; a.xb = batch_stride; a.xr = row_stride; a.codes = d_x8; a.scales = d_x8_scales; a.rows = d_rows;

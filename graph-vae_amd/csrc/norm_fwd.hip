@@ -369,6 +369,8 @@ int gvae_group_norm_fwd(const void *d_x, int dtype, int64_t batch_stride, int64_
   GVAE_REQUIRE(d_x && d_y && d_mean && d_rstd, GVAE_EINVAL, "group_norm_fwd: null pointer");
   GVAE_REQUIRE(!d_x8 == !d_x8_scales && !d_y8 == !d_y8_scales, GVAE_EINVAL,
                "group_norm_fwd: a checkpoint needs both its codes and its scales");
+  GVAE_REQUIRE(aligned16(d_x8) && aligned16(d_y8) && aligned16(d_ws), GVAE_EINVAL,
+               "group_norm_fwd: codes or workspace not 16-byte aligned");
   GVAE_REQUIRE(eps > 0.0f && std::isfinite(eps), GVAE_EINVAL, "group_norm_fwd: eps must be positive");
   if (int rc = norm_check("group_norm_fwd", dtype, B, N, C, G, act, row_stride)) return rc;
   GVAE_REQUIRE(batch_stride >= 0, GVAE_EINVAL, "group_norm_fwd: negative stride");

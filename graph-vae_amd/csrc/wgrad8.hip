@@ -438,6 +438,8 @@ int64_t gvae_linear_wgrad8_ws_bytes(int64_t rows, int O, int I) {
 int gvae_linear_wgrad8(const void *d_dy, int dtype, int64_t row_stride, const int8_t *d_codes, const uint8_t *d_scales,
                        int64_t rows, int O, int I, void *d_dw, void *d_db, void *d_ws, void *stream) {
   GVAE_REQUIRE(d_dy && d_codes && d_scales && d_dw && d_ws, GVAE_EINVAL, "linear_wgrad8: null pointer");
+  GVAE_REQUIRE(aligned16(d_codes) && aligned16(d_ws), GVAE_EINVAL,
+               "linear_wgrad8: codes or workspace not 16-byte aligned");
   GVAE_REQUIRE(dtype_known(dtype), GVAE_EINVAL, "linear_wgrad8: unknown element type %d", dtype);
   GVAE_REQUIRE(rows > 0 && O > 0 && I > 0 && row_stride >= O, GVAE_EINVAL,
                "linear_wgrad8: bad sizes (rows=%lld out=%d in=%d stride=%lld)", (long long)rows, O, I,

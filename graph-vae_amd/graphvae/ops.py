@@ -115,6 +115,12 @@ def _graph_strides(t: torch.Tensor) -> tuple[int, int]:
     return (t.stride(0) if B > 1 else 0), (t.stride(1) if N > 1 else C)
 
 
+def _sizes(what: str, *sizes: int) -> None:
+    """Refuses sizes that the C entry points' 32-bit arguments cannot hold."""
+    if max(sizes) > 0x7fffffff:
+        raise _hip.GvaeHipError(f"{what}: sizes {sizes} pass 2^31 - 1")
+
+
 _NONE = (None, None)
 
 
@@ -194,8 +200,9 @@ class Checkpoint8:
         if code is None:
             raise _hip.GvaeHipError(f"Checkpoint8.read: cannot be read as {dtype}")
         index = self._check("Checkpoint8.read")
-        out = _empty(self.shape, dtype=dtype, device=self.device)
         C = self.shape[-1]
+        _sizes("Checkpoint8.read", C)
+        out = _empty(self.shape, dtype=dtype, device=self.device)
         rc = (_bound or _bind()).gvae_ckpt8_read(self._at[0], self._at[1], out.numel() // C, C, out.data_ptr(), code, C,
                                                  _raw_stream(index))
         if rc:
@@ -210,6 +217,7 @@ def checkpoint8(x: torch.Tensor) -> Checkpoint8:
     code = _activation(x, "checkpoint8")
     rows, ld = _rows_of(x, "checkpoint8")
     C = x.shape[-1]
+    _sizes("checkpoint8", C)
     c = Checkpoint8._new(x.shape, rows, C, x.device, x.dtype)
     rc = (_bound or _bind()).gvae_ckpt8_write(x.data_ptr(), code, rows, C, ld, c._at[0], c._at[1], _raw_stream(index))
     if rc:
@@ -229,6 +237,7 @@ def _norm_sizes(x_shape, groups: int, what: str):
     if len(x_shape) != 3:
         raise _hip.GvaeHipError(f"{what}: expected (graphs, rows, channels), got shape {tuple(x_shape)}")
     B, N, C = x_shape
+    _sizes(what, B, N, C, groups)
     if groups < 1 or C % groups:
         raise ValueError(f"{what}: {C} channels do not divide into {groups} groups")
     return B, N, C
@@ -335,6 +344,7 @@ def linear_wgrad8(dy: torch.Tensor, x8: Checkpoint8) -> tuple[torch.Tensor, torc
                                 "rows")
     rows, ld = _rows_of(dy, what)
     O, I = dy.shape[-1], x8.shape[-1]
+    _sizes(what, O, I)
     L, dev = _bound or _bind(), dy.device
     dw = _empty((O, I), dtype=dy.dtype, device=dev)
     db = _empty((O,), dtype=dy.dtype, device=dev)

@@ -387,7 +387,7 @@ int gvae_sample_decode(const gvae_dims *d, const float *d_params, const float *d
  * The value of channel c is code[c] * 2^(scale[c/32] - 127).  When written, a block's power of two
  * is the least one (at least 2^-126) of which 127 reach the block's largest magnitude, and codes
  * are rounded to nearest, ties to even; a block with an infinity or a NaN gets the scale byte 255
- * and reads as NaN.  d_codes must be 16-byte aligned. */
+ * and reads as NaN.  Codes and workspaces must be 16-byte aligned. */
 int gvae_ckpt8_row_bytes(int C);
 int gvae_ckpt8_row_scales(int C);
 /* d_x: (rows, C) with unit channel stride and row_stride elements between rows. */

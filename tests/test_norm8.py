@@ -83,7 +83,7 @@ def _norm_fwd(L, x=16, dtype=0, bs=8, rs=8, B=1, N=1, C=8, G=2, act=1, eps=1e-5,
 @pytest.mark.parametrize("bad", [dict(x=None), dict(y=None), dict(ws=None, N=100000), dict(mean=None), dict(dtype=3),
                                  dict(dtype=-1), dict(B=0), dict(N=0), dict(C=0), dict(G=0), dict(G=3), dict(act=4),
                                  dict(act=-1), dict(rs=-8), dict(bs=-8), dict(eps=0.0), dict(eps=float("nan")),
-                                 dict(eps=float("inf")), dict(x8=16), dict(x8s=16), dict(y8=16), dict(y8s=16)])
+                                 dict(eps=float("inf")), dict(ws=8), dict(x8=24, x8s=16), dict(y8=8, y8s=16), dict(x8=16), dict(x8s=16), dict(y8=16), dict(y8s=16)])
 def test_norm_forward_refusals(bad):
     L = _lib()
     assert _norm_fwd(L, **bad) == -1
@@ -100,7 +100,8 @@ def test_norm_limits():
 @pytest.mark.parametrize("bad", [dict(dy=None), dict(dx=None), dict(x=None), dict(x8=16, x8s=16), dict(x8=16),
                                  dict(x=None, x8=16), dict(x=None, x8s=16), dict(dw=None), dict(db=None),
                                  dict(mean=None), dict(rstd=None), dict(ws=None), dict(dtype=9), dict(G=3), dict(C=0),
-                                 dict(rs=-1), dict(drs=-4), dict(bs=-1), dict(dbs=-1), dict(act=7)])
+                                 dict(rs=-1), dict(drs=-4), dict(bs=-1), dict(dbs=-1), dict(act=7), dict(ws=8),
+                                 dict(x=None, x8=8, x8s=16)])
 def test_norm_backward_refusals(bad):
     L = _lib()
     k = dict(dy=16, dtype=0, dbs=8, drs=8, x=16, bs=8, rs=8, x8=None, x8s=None, B=1, N=1, C=8, G=2, mean=16, rstd=16,
@@ -125,7 +126,8 @@ def test_checkpoint_and_wgrad_refusals():
               (16, 0, 7, 16, 16, 4, 8, 8, 16, 16, 16), (16, 0, 8, None, 16, 4, 8, 8, 16, 16, 16),
               (16, 0, 8, 16, None, 4, 8, 8, 16, 16, 16), (16, 0, 8, 16, 16, 0, 8, 8, 16, 16, 16),
               (16, 0, 8, 16, 16, 4, 0, 8, 16, 16, 16), (16, 0, 8, 16, 16, 4, 8, 0, 16, 16, 16),
-              (16, 0, 8, 16, 16, 4, 8, 8, None, 16, 16), (16, 0, 8, 16, 16, 4, 8, 8, 16, 16, None)]:
+              (16, 0, 8, 16, 16, 4, 8, 8, None, 16, 16), (16, 0, 8, 16, 16, 4, 8, 8, 16, 16, None),
+              (16, 0, 8, 8, 16, 4, 8, 8, 16, 16, 16), (16, 0, 8, 16, 16, 4, 8, 8, 16, 16, 8)]:
         assert L.gvae_linear_wgrad8(*a, None) == -1, a
         assert b"linear_wgrad8" in L.gvae_last_error()
     for dy_ld, rows, O, I in [(1 << 21, 4, 1 << 21, 8), (1 << 16, 4, 1 << 16, 1 << 16), (1 << 26, 4, 8, 8)]:
@@ -870,3 +872,28 @@ def test_checkpoint_copies_and_views():
     assert torch.equal(d.read(), want) and not c.read().any() and d.shape == x.shape and d.dtype == x.dtype
     e = ops.Checkpoint8(d.codes[1:3], d.scales[1:3], 70, torch.float32)
     assert torch.equal(e.read(), want[1:3])
+
+
+@gpu
+def test_sizes_past_32_bits_are_refused():
+    from graphvae import _hip, ops
+    E, dev = _hip.GvaeHipError, "cuda"
+    big = 2 ** 32 + 32      # (the C entry points would see 32)
+    one = torch.zeros(1, 1, 1, device=dev)
+    for shape in [(1, big, 1), (big, 1, 1)]:
+        with pytest.raises(E):
+            ops.group_norm_act(one.expand(shape), None, None, 1)
+        with pytest.raises(E):
+            st = torch.zeros(1, 1, device=dev)
+            ops.group_norm_act_backward(one.expand(shape), one.expand(shape), None, None, st, st, 1)
+    x = torch.empty(1, big, dtype=torch.float16, device=dev)
+    with pytest.raises(E):
+        ops.checkpoint8(x)
+    c = ops.Checkpoint8(torch.empty(1, 16, dtype=torch.int8, device=dev), torch.empty(1, 1, dtype=torch.uint8, device=dev), 8)
+    with pytest.raises(E):
+        ops.linear_wgrad8(x, c)
+    del x
+    c = ops.Checkpoint8(torch.empty(1, big, dtype=torch.int8, device=dev),
+                        torch.empty(1, big // 32, dtype=torch.uint8, device=dev), big)
+    with pytest.raises(E):
+        c.read()
