@@ -318,8 +318,8 @@ inline SplitShape split_shape(int B, int N, int C, int V, bool whole_blocks) {
 // memory transaction (4 of 16 bytes; 8 where checkpoints are written, whose segments are half as long; 1
 // where everything is a few MB and stays in the caches: there a slab may end inside its one piece);
 // `threads` and `held`: the largest work-group and the pieces a thread holds in it.  The slab is the
-// widest that leaves 1024 work-groups and has at most 2048 pieces, so that several work-groups share a CU
-// and one's loads run beside another's sums; the narrowest may have 4096.  false: no slab of whole
+// widest that leaves 1024 work-groups and has at most `most` pieces, so that several work-groups share a CU
+// and one's loads run beside another's sums; the narrowest may have `last_most`.  false: no slab of whole
 // groups is that small, or the batch would leave most of the chip idle that the split form fills.
 // Measured, forward, bf16, SiLU, 512 channels: 256 graphs of 250 rows 34 us (42 with slabs of up to 4096
 // pieces, 53 split); 192 graphs of 1000 rows 107 us (127 split), but 180 (162 split) with checkpoints
@@ -327,8 +327,8 @@ inline SplitShape split_shape(int B, int N, int C, int V, bool whole_blocks) {
 struct ResidentShape {
   int slab, nslab, lanes;
 };
-inline bool resident_shape(int B, int N, int C, int cpg, int V, int align, int least, int threads, int held,
-                           ResidentShape *s) {
+inline bool resident_shape(int B, int N, int C, int cpg, int V, int align, int least, int threads, int held, int most,
+                           int last_most, ResidentShape *s) {
   int64_t unit = cpg;
   while (unit % align && unit < C) unit += cpg;
   if (unit > C) unit = C;
@@ -342,7 +342,7 @@ inline bool resident_shape(int B, int N, int C, int cpg, int V, int align, int l
     const int lanes = lanes_of(slab);
     const int64_t pieces = (int64_t)N * lanes;
     const bool last = units <= fewest || units <= 1;
-    if (pieces <= (last ? 4096 : 2048) && lanes <= threads && (int64_t)(threads / lanes) * held >= N) {
+    if (pieces <= (last ? last_most : most) && lanes <= threads && (int64_t)(threads / lanes) * held >= N) {
       s->slab = (int)slab; s->lanes = lanes; s->nslab = ceil_div(C, (int)slab);
       return (int64_t)B * s->nslab >= 128 || pieces <= 2048;
     }
@@ -369,8 +369,15 @@ inline NormPlan norm_plan(bool backward, int dtype, int B, int N, int C, int G, 
   NormPlan p{};
   const int V = dtype == GVAE_F32 ? 4 : 8, cpg = C / G;
   const int least = (int64_t)B * N * C * (16 / V) <= (8 << 20) ? 1 : 4;
-  p.resident = backward ? resident_shape(B, N, C, cpg, V, checkpoints ? V : 1, least, 512, 4, &p.rs)
-                        : resident_shape(B, N, C, cpg, V, checkpoints ? kBlock8 : 1, checkpoints ? 8 : least, 1024, 8, &p.rs);
+  // The backward holds two to three times the registers a piece, hence smaller work-groups.  Measured, SiLU,
+  // bf16, slabs of up to 512 / 2048 pieces: 256 graphs of 250 rows, 512 channels 56 / 64 us, from the
+  // checkpoint 54 / 68; 512 graphs of 128 rows, 128 channels, float 25 / 36.  Split / narrowest slab: 192
+  // graphs of 500 rows, 512 channels (2000 pieces) 99 / 107, of 400 rows 85 / 79; 300 graphs of 300 rows,
+  // 320 channels in groups of ten (1500) 80 / 88.
+  p.resident = backward ? resident_shape(B, N, C, cpg, V, checkpoints ? V : 1, least, 512, 4, 512,
+                                         cpg % V == 0 ? 1600 : 1024, &p.rs)
+                        : resident_shape(B, N, C, cpg, V, checkpoints ? kBlock8 : 1, checkpoints ? 8 : least, 1024, 8,
+                                         2048, 4096, &p.rs);
   if (p.resident) {
     // about 1024 work-groups walk the graphs of the backward
     p.graph_step = p.rs.nslab >= 1024 ? 1 : 1024 / p.rs.nslab;

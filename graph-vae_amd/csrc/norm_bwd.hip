@@ -1,6 +1,6 @@
 // Group norm with an activation: gradients (gvae_norm.h has the mathematics and the two forms).
 //
-// Measured.  Resident: 256 graphs of 250 rows, 512 channels, bf16, SiLU 68 us (197 MB, 2.9 TB/s: loads, sums
+// Measured.  Resident: 256 graphs of 250 rows, 512 channels, bf16, SiLU 56 us (197 MB, 3.5 TB/s: loads, sums
 // and writes of a slab follow one another, and registers leave few work-groups to a CU); 64 ragged graphs of
 // at most 126 rows, 128 channels, float, from the checkpoint 7.2 us and 2.9 for dw and db.  Split: 16
 // graphs of 16384 rows, 512 channels, bf16, SiLU, from the checkpoint: sums 87 us (406 MB, bound by
