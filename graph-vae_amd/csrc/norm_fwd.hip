@@ -7,7 +7,7 @@
 // MB the latency of one work-group remains: 256 graphs of 32 rows, 128 channels, float, with both
 // checkpoints 8.9 us, a graph of 20 rows 5.1.  Split: 4 graphs of 65536 rows, 320 channels: sums 35 us
 // (4.8 TB/s), join 6, second pass 57 (336 MB, 5.9 TB/s); 192 ragged graphs of 1000 rows, 512 channels, with
-// both checkpoints: 28 + 6 + 114.
+// both checkpoints: 28 + 6 + 101.
 #include "gvae_norm.h"
 
 namespace gvae {
@@ -117,8 +117,14 @@ __global__ __launch_bounds__(NT) void norm_resident_kernel(NormArgs a) {
     // (the lanes of a block share a row: with checkpoints kept, `lanes` is a whole number of blocks)
     const int nc = a.ld8 - c0;
     const bool first = c0 % kBlock8 == 0 && nv > 0;
-    if (a.x8) emit8<PAST, V>(xf, a.x8 + row * a.ld8 + c0, nc, a.x8s + row * a.nb8 + c0 / kBlock8, first);
-    if (a.y8) emit8<PAST, V>(rounded<T>(y), a.y8 + row * a.ld8 + c0, nc, a.y8s + row * a.nb8 + c0 / kBlock8, first);
+    auto leave = [&](const float *f, int8_t *codes, uint8_t *scales) {
+      codes += row * a.ld8 + c0;
+      scales += row * a.nb8 + c0 / kBlock8;
+      if (i < live) emit8<PAST, V>(f, codes, nc, scales, first);
+      else emit8_zeros<PAST, V>(codes, nc, scales, first);
+    };
+    if (a.x8) leave(xf, a.x8, a.x8s);
+    if (a.y8) leave(rounded<T>(y), a.y8, a.y8s);
   }
 }
 
@@ -295,8 +301,14 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(NormArgs a) {
       // (the lanes of a block share a row: with checkpoints kept, `lanes` is a whole number of blocks)
       const int nc = a.ld8 - p.c0;
       const bool first = p.c0 % kBlock8 == 0 && p.nv > 0;
-      if (a.x8) emit8<PAST, V>(xf, a.x8 + row * a.ld8 + p.c0, nc, a.x8s + row * a.nb8 + p.c0 / kBlock8, first);
-      if (a.y8) emit8<PAST, V>(rounded<T>(y), a.y8 + row * a.ld8 + p.c0, nc, a.y8s + row * a.nb8 + p.c0 / kBlock8, first);
+      auto leave = [&](const float *f, int8_t *codes, uint8_t *scales) {
+        codes += row * a.ld8 + p.c0;
+        scales += row * a.nb8 + p.c0 / kBlock8;
+        if (i < live) emit8<PAST, V>(f, codes, nc, scales, first);
+        else emit8_zeros<PAST, V>(codes, nc, scales, first);
+      };
+      if (a.x8) leave(xf, a.x8, a.x8s);
+      if (a.y8) leave(rounded<T>(y), a.y8, a.y8s);
     }
   }
 }

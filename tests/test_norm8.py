@@ -784,7 +784,8 @@ def test_wgrad_large_tiles_and_many_parts(dtype, shape):
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape", [(200, 400, 64, 4), (40, 1000, 96, 6), (2, 70000, 32, 4), (1200, 9, 40, 8),
-                                   (1100, 3, 5, 5), (9, 4000, 45, 9), (130, 600, 33, 1)])
+                                   (1100, 3, 5, 5), (9, 4000, 45, 9), (130, 600, 33, 1), (4, 1200, 16, 2),
+                                   (40, 300, 512, 16), (130, 200, 60, 6)])
 def test_group_norm_forms(dtype, shape):
     """Sizes around the resident and the split form's borders, forward and backward, from the tensor and
     from its checkpoint."""
