@@ -44,19 +44,22 @@ template <> struct Pieces<bf16_t> { static constexpr int P = 1; };
 template <> struct Pieces<f16_t> { static constexpr int P = 2; };
 template <> struct Pieces<float> { static constexpr int P = 3; };
 
-// a finite value into P bf16 pieces that add up to it; what is not finite stays whole in the first
+// A finite value into P > 1 bf16 pieces that add up to it, each the upper half of a float.  An infinity stays
+// in the first; a NaN may lie in the second alone (the first is then an infinity).
 template <int P>
-__device__ __forceinline__ void cut(float x, uint16_t *out) {
-  const uint32_t b = __float_as_uint(x);
-  const bool finite = (b & 0x7f800000u) != 0x7f800000u;
-  out[0] = (uint16_t)((b >> 16) | (x != x ? 0x40u : 0u));
-  float r = finite ? x - __uint_as_float(b & 0xffff0000u) : 0.0f;
+__device__ __forceinline__ void cut(float x, uint32_t *out) {
+  out[0] = __float_as_uint(x);
+  float r = x - __uint_as_float(out[0] & 0xffff0000u);
+  r = fabsf(x) == __builtin_inff() ? 0.0f : r;
 #pragma unroll
   for (int p = 1; p < P; ++p) {
-    const uint32_t c = __float_as_uint(r);
-    out[p] = (uint16_t)(c >> 16);
-    r -= __uint_as_float(c & 0xffff0000u);
+    out[p] = __float_as_uint(r);
+    r -= __uint_as_float(out[p] & 0xffff0000u);
   }
+}
+// the upper halves of two floats
+__device__ __forceinline__ uint32_t upper_halves(uint32_t lo, uint32_t hi) {
+  return __builtin_amdgcn_perm(hi, lo, 0x07060302u);
 }
 
 // What the 64-byte piece of a row is XORed with in a tile of W columns: four rows that are read together
@@ -159,14 +162,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad8_kernel(WgradArgs a) {
     if constexpr (P == 1) {
       *reinterpret_cast<typename Piece<T>::raw *>(dst) = ra[j];
     } else {
-      uint16_t out[V][P];
+      uint32_t out[V][P];
 #pragma unroll
       for (int v = 0; v < V; ++v) cut<P>((float)ra[j][v], out[v]);
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         uint32_t w[V / 2];
 #pragma unroll
-        for (int v = 0; v < V / 2; ++v) w[v] = out[2 * v][p] | ((uint32_t)out[2 * v + 1][p] << 16);
+        for (int v = 0; v < V / 2; ++v) w[v] = upper_halves(out[2 * v][p], out[2 * v + 1][p]);
         if constexpr (V == 8) *reinterpret_cast<uint4 *>(dst + p * S::kBytesA) = make_uint4(w[0], w[1], w[2], w[3]);
         else *reinterpret_cast<uint2 *>(dst + p * S::kBytesA) = make_uint2(w[0], w[1]);
       }
@@ -185,7 +188,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad8_kernel(WgradArgs a) {
         // (exact in bf16: the upper half of the float is all of it)
         const uint32_t c = src[2 * h + (v >> 1)] >> (16 * (v & 1));
         const uint32_t lo = __float_as_uint((float)(int8_t)c * p), hi = __float_as_uint((float)(int8_t)(c >> 8) * p);
-        w[v] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+        w[v] = upper_halves(lo, hi);
       }
       *reinterpret_cast<uint4 *>(bb + tile_at<TN>(k, cb + 8 * h)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
