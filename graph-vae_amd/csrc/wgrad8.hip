@@ -15,7 +15,7 @@
 // 65536 rows, 2048 x 2048, bf16: 470 to 500 us, 1100 to 1170 TFLOP/s.  The products and their reads from
 // LDS alone take 390 us of it on random numbers (less on zeros: the clock gives way to the power drawn),
 // conversions and stores to LDS the rest.  Half and float pay for each piece of a gradient with a whole
-// product: 50001 rows, 515 x 387, half 86 us in 128 x 256 tiles that cover 1.65 times dW.
+// product: 50001 rows, 515 x 387, half 73 us (and 9 for its sums) in 128 x 256 tiles that cover 1.65 times dW.
 //
 // A work-group owns a tile of dW and a range of rows; the parts are summed in their order by a second
 // launch.  Column sums of dY ride along: among the work-groups that share a dY tile, each adds up its
@@ -371,13 +371,13 @@ struct WgradShape {
   int64_t split_rows;
 };
 // Larger tiles need fewer bytes and conversions per product, smaller ones fill the chip sooner.  Measured
-// (us, tiles of 64 / 128 / 256): 8192 rows of 256 x 256 float 18 / 23 / 29; 4096 x 1024 x 1024 bf16
-// 31 / 28 / 34; 50001 x 515 x 387 half 124 / 107 / 98; 65536 x 1024 x 1024 bf16 277 / 170 / 142; 100000 x
-// 64 x 64 float 18 / 28 / 46.  So: 256 from 200000 rows times tiles on, 64 below 100000 or where a side has
-// no more than 64.  Where tiles of 128 x 256 cover dW with 10 % less, they are taken in place of 256 x 256:
-// 50001 x 515 x 387 half 95 / 107, 100000 x 640 x 640 half 211 / 237 (fewer work-groups share a tile of x, so
-// with no less to cover they are slower: 65536 x 1024 x 1024 bf16 162 / 138).  Rows are split until there is a work-group for each CU (two of the smaller ones; one
-// range where that makes half of them already), no range shorter than 128 rows.
+// (us, tiles of 64 x 64 / 128 x 128 / 128 x 256 / 256 x 256): 8192 rows of 256 x 256 float 18 / 23 / 26 / 30;
+// 100000 x 64 x 64 float 19 / 27 / 35 / 44; 4096 x 1024 x 1024 bf16 38 / 30 / 36 / 35; 50001 x 515 x 387 half
+// 108 / 92 / 82 / 87; 100000 x 640 x 640 half 310 / 201 / 193 / 211; 65536 x 1024 x 1024 bf16 473 / 180 / 175
+// / 140.  So: 256 x 256 from 200000 rows times tiles on, or 128 x 256 where that covers dW with 10 % less;
+// 64 x 64 below 100000 or where a side has no more than 64.  Rows are split until there is a work-group
+// for each CU (two of the smaller ones; one range where that makes half of them already), no range shorter
+// than 128 rows.
 static WgradShape wgrad_shape(int64_t rows, int O, int I) {
   WgradShape s;
   auto tiles_of = [&](int tm, int tn) { return (int64_t)ceil_div(I, tn) * ceil_div(O, tm); };
