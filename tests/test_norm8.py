@@ -898,3 +898,30 @@ def test_sizes_past_32_bits_are_refused():
                         torch.empty(1, big // 32, dtype=torch.uint8, device=dev), big)
     with pytest.raises(E):
         c.read()
+
+
+@gpu
+def test_two_graphs_and_two_streams_at_once():
+    """Two captured layers replayed on two streams beside each other, and eager layers on both: as each alone."""
+    from graphvae import ops
+    sets = [_layer_inputs(torch.bfloat16, 11, B=40, N=150, I=64, O=192), _layer_inputs(torch.float32, 12)]
+    alone = [_layer(ops, *s) for s in sets]
+    graphs, outs = [], []
+    for s in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(_layer(ops, *s))
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(3):
+        for t in [t for out in outs for t in out]:
+            t.zero_()
+        torch.cuda.synchronize()
+        eager = []
+        for _ in range(4):
+            for graph, stream, s in zip(graphs, streams, sets):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+                    eager.append(_layer(ops, *s))
+        torch.cuda.synchronize()
+        for k, want in enumerate(alone):
+            assert all(torch.equal(p, q) for got in [outs[k], *eager[k::2]] for p, q in zip(got, want))
