@@ -925,3 +925,55 @@ def test_two_graphs_and_two_streams_at_once():
         torch.cuda.synchronize()
         for k, want in enumerate(alone):
             assert all(torch.equal(p, q) for got in [outs[k], *eager[k::2]] for p, q in zip(got, want))
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(2, 2 ** 21, 520, 4), (70000, 64, 512, 4)])
+def test_group_norm_past_32_bit_offsets(shape):
+    """A graph of rows that repeat a pattern has the pattern's statistics, values and dx: the last rows of more
+    than 2^31 values against the pattern alone, within its rounding and that of the sums' other order."""
+    from graphvae import ops
+    B, N, C, G = shape
+    n = min(N, 1024)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    base, dbase = (torch.randn(n, C, generator=g, device="cuda").half() for _ in range(2))
+    w, b = torch.randn(C, generator=g, device="cuda"), torch.randn(C, generator=g, device="cuda")
+    x, dy = (t.expand(B, N // n, n, C).reshape(B, N, C).contiguous() for t in (base, dbase))
+    assert x.numel() > 2 ** 31
+    one, done = base[None], dbase[None]
+    r, e = (ops.group_norm_act(t, w, b, G, act="silu") for t in (x, one))
+    # (values of a few units: two of their last places of half, and 2^-16 for sums of up to 2^28 values)
+    assert ((r.mean - e.mean).abs() <= 2.0 ** -16).all() and ((r.rstd / e.rstd - 1).abs() <= 2.0 ** -16).all()
+    for got in (r.y[-1, -n:], r.y[0, :n]):
+        assert ((got.float() - e.y[0].float()).abs() <= 2.0 ** -10 * (e.y[0].float().abs() + 2.0 ** -4)).all()
+    keep = ops.checkpoint8(x)
+    del r
+    for src, osrc in ((x, one), (keep, ops.checkpoint8(one))):
+        d = ops.group_norm_act_backward(dy, src, w, b, e.mean.expand(B, G).contiguous(),
+                                        e.rstd.expand(B, G).contiguous(), G, act="silu")
+        f = ops.group_norm_act_backward(done, osrc, w, b, e.mean, e.rstd, G, act="silu")
+        for got in (d[0][-1, -n:], d[0][0, :n]):
+            assert ((got.float() - f[0][0].float()).abs() <= 2.0 ** -10 * (f[0][0].float().abs() + 2.0 ** -4)).all()
+        for k in (1, 2):
+            want = f[k].double() * (B * (N // n))
+            assert ((d[k].double() - want).abs() <= 2.0 ** -12 * want.abs().max()).all()
+        del d
+
+
+@gpu
+def test_wgrad_past_32_bit_offsets():
+    """More than 2^31 gradients and codes; all but the last rows of the gradient are 0: exact."""
+    from graphvae import ops
+    M, O, I = 2 ** 21 + 77, 1030, 1040
+    g = torch.Generator(device="cuda").manual_seed(6)
+    dy = torch.zeros(M, O, dtype=torch.float16, device="cuda")
+    codes = torch.zeros(M, I, dtype=torch.int8, device="cuda")
+    codes[-300:] = torch.randint(-127, 128, (300, I), generator=g, device="cuda").to(torch.int8)
+    codes[:300] = 1
+    dy[-300:] = torch.randint(-1, 2, (300, O), generator=g, device="cuda").half()
+    assert dy.numel() > 2 ** 31 and codes.numel() > 2 ** 31
+    c = ops.Checkpoint8(codes, torch.full((M, -(-I // 32)), 127, dtype=torch.uint8, device="cuda"), I)
+    dw, db = ops.linear_wgrad8(dy, c)
+    # (sums of 300 products of at most 127: integers under 2^16, exact in fp32; half rounds them once)
+    want = (dy[-300:].double().t() @ codes[-300:].double()).float().half()
+    assert torch.equal(dw, want) and torch.equal(db, dy[-300:].double().sum(0).float().half())
