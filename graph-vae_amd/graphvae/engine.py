@@ -150,7 +150,7 @@ class _Slot:
 
     def __init__(self, device) -> None:
         self.ws = None
-        self.ws_graphs = 0
+        self.ws_bytes = 0
         self.out4 = torch.zeros(4, dtype=torch.float32, device=device)
         self.perm = None
         self.iters_done = None
@@ -171,7 +171,7 @@ class StepEngine:
     current slot.  The similarity-tensor buffer is shared: matchings run one after the other."""
 
     _ws = _slot_attr("ws")
-    _ws_graphs = _slot_attr("ws_graphs")
+    _ws_bytes = _slot_attr("ws_bytes")
     out4 = _slot_attr("out4")
     perm = _slot_attr("perm")
     iters_done = _slot_attr("iters_done")
@@ -194,6 +194,7 @@ class StepEngine:
         self.matching = matching
         self.mpm_iters, self.tol, self.early_stop = int(mpm_iters), float(tol), bool(early_stop)
         self._slots = [_Slot(self.device)]
+        self._ws_need = {}
         self._cur = 0
         # the streamed matching keeps the similarity tensor of as many graphs as fit this many
         # bytes and walks the batch in chunks (default: a third of the device's memory)
@@ -216,12 +217,17 @@ class StepEngine:
 
     # ------------------------------------------------------------------ helpers
     def _ensure(self, B: int) -> None:
-        if self._ws is None or B > self._ws_graphs:
+        # (bytes per batch size: with group norm 512 graphs can need more than 513, whose rows are cut into
+        # fewer ranges)
+        need = self._ws_need.get(B)
+        if need is None:
             need = (self.L.gvae_step_ws_bytes(ctypes.byref(self.dims), B) if self.gn is None else
                     self.L.gvae_step_gn_ws_bytes(ctypes.byref(self.dims), ctypes.byref(self.gn), B))
+            self._ws_need[B] = need
+        if self._ws is None or need > self._ws_bytes:
             # (zeroed once: the streamed matching's statistics words in it are only ever added to)
             self._ws = torch.zeros(need, dtype=torch.uint8, device=self.device)
-            self._ws_graphs = B
+            self._ws_bytes = need
         if self.perm is None or self.perm.shape[0] != B:
             self.perm = torch.empty(B, self.N, dtype=torch.int64, device=self.device)
             self.iters_done = torch.empty(B, dtype=torch.int32, device=self.device)

@@ -444,6 +444,8 @@ typedef struct gvae_gn_opts {
   float eps;
 } gvae_gn_opts;
 
+/* Bytes of scratch for n_graphs graphs.  Fewer graphs may need MORE (their rows can be cut into more
+ * ranges): a workspace used for several batch sizes takes the largest of their sizes. */
 int64_t gvae_step_gn_ws_bytes(const gvae_dims *d, const gvae_gn_opts *gn, int n_graphs);
 
 /* gvae_step_forward_model with group norm (no statistics to update, hence no mode argument).  The

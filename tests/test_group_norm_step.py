@@ -279,3 +279,29 @@ def test_single_node_graphs_and_equal_nodes():
         nodes.backward()
         g = torch.cat([p.grad.reshape(-1) for p in model.parameters() if p.grad is not None])
         assert torch.isfinite(g).all() and torch.isfinite(out["kl"])
+
+
+def _host_engine(F_, H, Z, N, **norm):
+    """The engine's workspace bookkeeping on host memory (nothing is launched)."""
+    from graphvae import engine
+    eng = object.__new__(engine.StepEngine)
+    eng.gn = engine.norm_options(norm.get("norm", "batch"), norm.get("norm_groups", 8), norm.get("act_bits", 32), H)
+    eng.L, eng.dims, eng.N, eng.device = engine._bind(), engine.Dims(F_, H, Z, N), N, torch.device("cpu")
+    eng._slots, eng._cur, eng._ws_need = [engine._Slot(eng.device)], 0, {}
+    return eng
+
+
+@pytest.mark.parametrize("N,H,sizes", [(32, 128, (513, 512, 513, 100, 512)), (126, 64, (521, 520)), (8, 256, (513, 512)),
+                                       (16, 128, (1025, 1024, 1, 1024))])
+def test_workspace_holds_every_batch_size(N, H, sizes):
+    """A smaller batch can need more scratch than a larger one before it (its rows are cut into more ranges);
+    the workspace always holds what the batch at hand needs."""
+    import ctypes
+    from graphvae import engine
+    for kw in ({}, {"norm": "group"}, {"norm": "group", "act_bits": 8}):
+        eng = _host_engine(1, H, 64, N, **kw)
+        for B in sizes:
+            eng._ensure(B)
+            need = (eng.L.gvae_step_ws_bytes(ctypes.byref(eng.dims), B) if eng.gn is None else
+                    eng.L.gvae_step_gn_ws_bytes(ctypes.byref(eng.dims), ctypes.byref(eng.gn), B))
+            assert eng._ws.numel() >= need > 0, (kw, B)
