@@ -66,8 +66,10 @@ __global__ __launch_bounds__(NT) void norm_resident_kernel(NormArgs a) {
 #pragma unroll
   for (int e = 0; e < E; ++e)
     group[e] = e == 0 ? (c0 < s1 ? c0 - s0 : 0) / a.cpg : group_after(group[e - 1], c0 + e - s0, a.cpg, ng);
+  // (0 behind the slab's last channel, as rstd below: what a lane there adds to a block's checkpoint must not
+  // come from another group, whose mean may be large or not finite)
 #pragma unroll
-  for (int e = 0; e < E; ++e) mean[e] = grp[0][group[e]] * inv;
+  for (int e = 0; e < E; ++e) mean[e] = c0 + e < s1 ? grp[0][group[e]] * inv : 0.0f;
   {
     float s[E];
 #pragma unroll
@@ -90,7 +92,7 @@ __global__ __launch_bounds__(NT) void norm_resident_kernel(NormArgs a) {
   join_groups<1, NT * E, NT * E>(ent, a.lanes * E, ge, ng, a.rp, a.join, NT, grp + 1);
   __syncthreads();
 #pragma unroll
-  for (int e = 0; e < E; ++e) rstd[e] = 1.0f / sqrtf(grp[1][group[e]] * inv + a.eps);
+  for (int e = 0; e < E; ++e) rstd[e] = c0 + e < s1 ? 1.0f / sqrtf(grp[1][group[e]] * inv + a.eps) : 0.0f;
   for (int g = threadIdx.x; g < ng; g += NT) {
     const int64_t q = (int64_t)b * a.G + g0 + g;
     a.mean[q] = grp[0][g] * inv;

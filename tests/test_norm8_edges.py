@@ -1,0 +1,55 @@
+"""Group norm, 8-bit checkpoints and weight gradients where values, sizes or callers are at an edge: what is
+not finite stays where it belongs, extreme but finite values, the precision of the activations.  Bounds as
+in test_norm8.py: u = 2^-24 for every fp32 operation, half a step of the type for the result."""
+import pytest
+import torch
+
+from test_norm8 import ACTS, DTYPES, make_x
+
+gpu = pytest.mark.gpu
+
+# (rows, channels, groups): a last block of 32 channels that is not full, in the resident form (a slab of the whole row,
+# lanes behind the last channel) and in the split form
+RAGGED_BLOCKS = [(10, 40, 5), (20, 40, 2), (20, 45, 9), (20, 48, 8), (10, 100, 5), (7, 33, 3), (6000, 40, 5), (9000, 45, 9)]
+
+
+# ------------------------------------------------------------------ what is not finite
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", RAGGED_BLOCKS)
+def test_output_checkpoint_beside_a_group_that_is_not_finite(dtype, shape):
+    """An infinity or a NaN in the first group reaches the blocks of that group's channels and no other: the
+    output's checkpoint is the one that checkpoint8 makes of the output, in the row's last block too."""
+    from graphvae import ops
+    N, C, G = shape
+    x, w, b, _, _ = make_x(2, N, C, dtype, 21)
+    first, blocks = C // G, -(-C // 32)
+    touched = -(-first // 32)
+    for k, act in enumerate(ACTS):
+        bad = x.clone()
+        bad[1, N // 2, first // 2] = (float("nan"), float("inf"), float("-inf"), float("nan"))[k]
+        r = ops.group_norm_act(bad.cuda(), w.cuda(), b.cuda(), G, act=act, keep_x=True, keep_y=True)
+        assert r.y[1, :, first:].isfinite().all() and r.y[0].isfinite().all()
+        for got, src in ((r.y8, r.y), (r.x8, bad.cuda())):
+            want = ops.checkpoint8(src)
+            assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales), act
+        assert (r.y8.scales[1, :, :touched] == 255).all() or act != "none"
+        assert (r.y8.scales[1, :, touched:blocks] != 255).all() and (r.y8.scales[0] != 255).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("C,G,which", [(40, 5, 0), (42, 21, 0), (42, 21, 20), (33, 33, 32)])
+def test_output_checkpoint_beside_a_large_constant_group(dtype, C, G, which):
+    """A group of equal values of 2^120: its mean is exact (8 rows and a power of two of channels), its
+    variance 0, its output act(bias), and the output's checkpoint is that of the output."""
+    from graphvae import ops
+    x, w, b, _, _ = make_x(2, 8, C, dtype, 22)
+    n = C // G
+    x[1, :, which * n:(which + 1) * n] = 2.0 ** 120
+    for act in ACTS:
+        r = ops.group_norm_act(x.cuda(), w.cuda(), b.cuda(), G, act=act, keep_y=True)
+        assert r.mean[1, which].item() == 2.0 ** 120 and r.y.isfinite().all()
+        want = ops.checkpoint8(r.y)
+        assert torch.equal(r.y8.codes, want.codes) and torch.equal(r.y8.scales, want.scales), act
+        assert (r.y8.scales != 255).all()
