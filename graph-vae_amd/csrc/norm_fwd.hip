@@ -178,7 +178,7 @@ __global__ __launch_bounds__(kThreads) void norm_stats_kernel(NormArgs a) {
           }
           const float d = mb - mean[v];
           mean[v] = __fmaf_rn(d, share, mean[v]);
-          m2[v] += __fmaf_rn(d * d, cross, q);
+          m2[v] += __fmaf_rn(d * cross, d, q);   // (first batch: cross is 0, and d * d alone may overflow)
         }
       };
       if (cnt == kBatch) batch(std::true_type{});

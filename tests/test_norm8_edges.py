@@ -4,7 +4,7 @@ in test_norm8.py: u = 2^-24 for every fp32 operation, half a step of the type fo
 import pytest
 import torch
 
-from test_norm8 import ACTS, DTYPES, make_x
+from test_norm8 import ACTS, DTYPES, U32, half_step, make_x, norm_ref, subnormal
 
 gpu = pytest.mark.gpu
 
@@ -53,3 +53,25 @@ def test_output_checkpoint_beside_a_large_constant_group(dtype, C, G, which):
         want = ops.checkpoint8(r.y)
         assert torch.equal(r.y8.codes, want.codes) and torch.equal(r.y8.scales, want.scales), act
         assert (r.y8.scales != 255).all()
+
+
+# ------------------------------------------------------------------ extreme but finite values
+@gpu
+@pytest.mark.parametrize("dtype,spread", [(torch.float32, 1e17), (torch.bfloat16, 3e17)])
+@pytest.mark.parametrize("shape", [(2, 3000, 32, 2), (1, 20000, 24, 3), (2, 5000, 33, 11)])
+def test_split_statistics_of_means_whose_squares_overflow(dtype, spread, shape):
+    """Means of 4e19 (squared: over the largest fp32) with deviations whose squares are not: finite, and within
+    the bounds of any other mean."""
+    from graphvae import ops
+    B, N, C, G = shape
+    g = torch.Generator().manual_seed(23)
+    sign = 1.0 - 2.0 * (torch.arange(C) // (C // G) % 2)
+    x = (4e19 * sign + spread * torch.randn(B, N, C, generator=g)).to(dtype)
+    _, w, b, rows, _ = make_x(B, N, C, dtype, 23)
+    rows[0] = N
+    x = torch.where(torch.arange(N)[None, :, None] < rows[:, None, None], x, torch.zeros_like(x))
+    r = ops.group_norm_act(x.cuda(), w.cuda(), b.cuda(), G, act="none", rows=rows.cuda())
+    y, mean, rstd, tol, dmean, drel = norm_ref(x, w, b, G, "none", 1e-5, rows)
+    assert ((r.mean.cpu().double() - mean).abs() <= dmean + 2 * U32 * mean.abs()).all()
+    assert ((r.rstd.cpu().double() / rstd - 1).abs() <= drel + 4 * U32).all()
+    assert ((r.y.cpu().double() - y).abs() <= half_step(dtype) * y.abs() + 1.01 * tol + subnormal(dtype)).all()
