@@ -9,13 +9,11 @@
 //
 // For a ReLU z is formed by a subtraction, two products and a sum, each rounded, in the forward and in the
 // backward alike: its branch is the same in both.  The other activations add b in the same step as the
-// product (one rounding less); for 16-bit types the split form also takes h = x r - (mean r) in one step:
-// off by 2^-24 |mean r|, where a 16-bit x is itself off by 2^-9 or 2^-12 |x|.
+// product (one rounding less); for 16-bit types the split form also centres and scales in one step, by a power
+// of two (`Scale`: as exact, an instruction less).
 //
 // The split kernels come near the rate of the vector units before that of memory: a SiLU's slope is 13
-// instructions a value, two of them at a quarter of the rate.  Backward sums of 16 graphs of 16384 rows, 512
-// channels, bf16, from the checkpoint: 14 instructions a value and 87 us for 406 MB with the two forms
-// above, 20 instructions and 82 % of the issue slots without.
+// instructions a value, two of them at a quarter of the rate.
 //
 // All of it is bound by memory.  Two forms each:
 //   resident   a work-group holds a graph's live rows of a run of groups (a slab) in registers: one
@@ -196,21 +194,53 @@ __device__ __forceinline__ void load_params(const float *p, int c0, int nv, floa
   for (int v = 0; v < V; ++v) f[v] = v < nv ? (p ? p[c0 + v] : none) : 0.0f;
 }
 
-// What the channels of a piece are scaled and shifted by.  FOLD: `mean` holds -mean * rstd.
-template <int V, bool FOLD>
+// What the channels of a piece are scaled and shifted by: centred(x) * unit is h, and pre<ACT>(centred(x)) the
+// value before the activation.
+//   POW2: centred(x) = x p - mean p in one step, p the power of two at or under rstd, at most 1: both products
+//         are exact, so it is (x - mean) p rounded once; unit = rstd / p is left in the weight.
+//   else: centred(x) = (x - mean) rstd, unit = 1.
+template <int V, bool POW2>
 struct Scale {
-  float mean[V], rstd[V], w[V], b[V];
-  __device__ __forceinline__ float h(int v, float x) const {
-    return FOLD ? __fmaf_rn(x, rstd[v], mean[v]) : (x - mean[v]) * rstd[v];
+  float mean[V], rstd[V], w[V], b[V], unit[V];      // POW2: -mean p, p, w unit
+  static __device__ __forceinline__ float pow2_of(float rstd) {
+    const float p = __uint_as_float(__float_as_uint(rstd) & 0x7f800000u);
+    return fminf(fmaxf(p, 0x1p-126f), 1.0f);
   }
+  // (rstd / p by an exponent's subtraction: exact)
+  static __device__ __forceinline__ float unit_of(float rstd) {
+    return POW2 ? rstd * __uint_as_float(0x7f000000u - __float_as_uint(pow2_of(rstd))) : 1.0f;
+  }
+  __device__ __forceinline__ float centred(int v, float x) const {
+    return POW2 ? __fmaf_rn(x, rstd[v], mean[v]) : (x - mean[v]) * rstd[v];
+  }
+  template <int ACT>
+  __device__ __forceinline__ float pre(int v, float c) const { return pre_act<ACT>(c, w[v], b[v]); }
   __device__ Scale(const NormArgs &a, int g, int c0, int nv) {
     load_params<V>(a.w, c0, nv, 1.0f, w);
     load_params<V>(a.b, c0, nv, 0.0f, b);
     per_group<V>(a, a.mean, g, c0, nv, mean);
     per_group<V>(a, a.rstd, g, c0, nv, rstd);
-    if (FOLD)
 #pragma unroll
-      for (int v = 0; v < V; ++v) mean[v] = -mean[v] * rstd[v];
+    for (int v = 0; v < V; ++v) unit[v] = 1.0f;
+    if (!POW2) return;
+    auto split = [&](int from, int v) {
+      unit[v] = unit_of(rstd[from]);
+      w[v] *= unit[v];
+      mean[v] *= -pow2_of(rstd[from]);
+    };
+    if (a.cpg % V == 0) {          // (uniform: one group, as in per_group)
+      const float p = pow2_of(rstd[0]);
+#pragma unroll
+      for (int v = 0; v < V; ++v) split(0, v);
+#pragma unroll
+      for (int v = 0; v < V; ++v) rstd[v] = p;
+      return;
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      split(v, v);
+      rstd[v] = pow2_of(rstd[v]);
+    }
   }
 };
 

@@ -198,13 +198,17 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_sums_kernel(NormArgs a) {
         x[u].cut(cut);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float h = k.h(v, x[u].at(v));
-          const float dz = (float)g[u][v] * act_slope<ACT>(pre_act<ACT>(h, k.w[v], k.b[v]));
+          const float h = k.centred(v, x[u].at(v));
+          const float dz = (float)g[u][v] * act_slope<ACT>(k.template pre<ACT>(v, h));
           s1[v] += dz;
           s2[v] = __fmaf_rn(dz, h, s2[v]);
         }
       }
     }
+    float rstd[V];
+    per_group<V>(a, a.rstd, p.b, p.c0, p.nv, rstd);
+#pragma unroll
+    for (int v = 0; v < V; ++v) s2[v] *= k.unit_of(rstd[v]);
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -294,8 +298,9 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_apply_kernel(NormArgs a) {
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int64_t q = (int64_t)p.b * a.G + (p.c0 + (v < p.nv ? v : 0)) / a.cpg;
-    a1[v] = a.A[2 * q] * k.rstd[v];
-    a2[v] = a.A[2 * q + 1] * k.rstd[v];
+    const float r = k.rstd[v] * k.unit[v];
+    a1[v] = a.A[2 * q] * r;
+    a2[v] = a.A[2 * q + 1] * r * k.unit[v];
     wr[v] = k.w[v] * k.rstd[v];
   }
   const T *dy = (const T *)a.dy + p.b * a.dyb;
@@ -322,8 +327,8 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_apply_kernel(NormArgs a) {
         x[u].cut(cut);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float h = k.h(v, x[u].at(v));
-          const float dz = (float)g[u][v] * act_slope<ACT>(pre_act<ACT>(h, k.w[v], k.b[v]));
+          const float h = k.centred(v, x[u].at(v));
+          const float dz = (float)g[u][v] * act_slope<ACT>(k.template pre<ACT>(v, h));
           dx[v] = __fmaf_rn(dz, wr[v], -__fmaf_rn(h, a2[v], a1[v]));
         }
       }

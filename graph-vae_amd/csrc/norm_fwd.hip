@@ -295,7 +295,7 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(NormArgs a) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           xf[v] = (float)r[u][v];
-          y[v] = act_value<ACT>(pre_act<ACT>(k.h(v, xf[v]), k.w[v], k.b[v]));
+          y[v] = act_value<ACT>(k.template pre<ACT>(v, k.centred(v, xf[v])));
         }
       }
       const int64_t row = (int64_t)p.b * a.N + i;

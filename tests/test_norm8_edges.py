@@ -4,7 +4,7 @@ in test_norm8.py: u = 2^-24 for every fp32 operation, half a step of the type fo
 import pytest
 import torch
 
-from test_norm8 import ACTS, DTYPES, U32, half_step, make_x, norm_ref, subnormal
+from test_norm8 import ACTS, DEPTH, DTYPES, U32, act_ref, half_step, make_x, norm_ref, per_channel, slope_ref, subnormal
 
 gpu = pytest.mark.gpu
 
@@ -75,3 +75,56 @@ def test_split_statistics_of_means_whose_squares_overflow(dtype, spread, shape):
     assert ((r.mean.cpu().double() - mean).abs() <= dmean + 2 * U32 * mean.abs()).all()
     assert ((r.rstd.cpu().double() / rstd - 1).abs() <= drel + 4 * U32).all()
     assert ((r.y.cpu().double() - y).abs() <= half_step(dtype) * y.abs() + 1.01 * tol + subnormal(dtype)).all()
+
+
+def _far(B, N, C, dtype):
+    """Values of 1024 and, one in a hundred, the next one of the type up to 1032: about 10^3 to 10^5 deviations from 0."""
+    g = torch.Generator().manual_seed(24)
+    step = {torch.float32: 1.0, torch.bfloat16: 8.0, torch.float16: 1.0}[dtype]
+    x = (1024.0 + step * (torch.rand(B, N, C, generator=g) < 0.01)).to(dtype)
+    w, b = 1 + 0.3 * torch.randn(C, generator=g), 0.3 * torch.randn(C, generator=g)
+    dy = (0.5 + torch.rand(B, N, C, generator=g)).to(dtype)
+    return x, w, b, dy
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(3, 40, 48, 6), (2, 4000, 48, 6), (2, 6000, 45, 9)])
+@pytest.mark.parametrize("act", ["none", "silu", "gelu"])
+def test_values_far_from_zero_keep_their_bits(dtype, shape, act):
+    """With the mean and rstd that are used (fp32), x - mean is off by u of itself only, however far from zero
+    both lie, in the resident and in the split form alike."""
+    from graphvae import ops
+    B, N, C, G = shape
+    x, w, b, dy = _far(B, N, C, dtype)
+    r = ops.group_norm_act(x.cuda(), w.cuda(), b.cuda(), G, act=act)
+    m, rs = (per_channel(t.cpu().double(), C) for t in (r.mean, r.rstd))
+    h = (x.double() - m) * rs
+    z = h * w.double() + b.double()
+    # x - mean, its product with rstd (or rstd's with w) and that with w: u each; the sum: u of it
+    ez = 3 * U32 * (h * w).abs() + U32 * z.abs()
+    ry = act_ref(z, act)
+    tol = 1.13 * ez + (12 * U32 * z.abs() if act != "none" else 0.0)
+    err = (r.y.cpu().double() - ry).abs()
+    assert (err <= half_step(dtype) * ry.abs() + 1.01 * tol + subnormal(dtype)).all()
+    _, dw, db = ops.group_norm_act_backward(dy.cuda(), x.cuda(), w.cuda(), b.cuda(), r.mean, r.rstd, G, act=act)
+    dz = dy.double() * slope_ref(z, act)
+    edz = dy.double() * (1.2 * ez + 16 * U32) if act != "none" else 0.0 * dz
+    # two roundings of h and DEPTH of the sums (with 80 more over graphs and chunks)
+    edw = (edz * h.abs() + (3 + DEPTH + 80) * U32 * (dz * h).abs()).sum((0, 1))
+    edb = (edz + (DEPTH + 80) * U32 * dz.abs()).sum((0, 1))
+    assert ((dw.cpu().double() - (dz * h).sum((0, 1))).abs() <= 1.01 * edw).all()
+    assert ((db.cpu().double() - dz.sum((0, 1))).abs() <= 1.01 * edb).all()
+
+
+@gpu
+def test_large_constant_rows_in_both_forms():
+    """bf16 rows of one value whose product with 1 / sqrt(eps) is over the largest fp32 (sums of it are not, and
+    with powers of two all round): the norm's value is 0, y the bias."""
+    from graphvae import ops
+    for N in (8, 16384):
+        x = torch.full((1, N, 8), 2.0 ** 100, dtype=torch.bfloat16, device="cuda")
+        x[:, :, 4:] = -2.0 ** 105
+        b = torch.arange(8, dtype=torch.float32, device="cuda")
+        r = ops.group_norm_act(x, None, b, 2, act="none", eps=1e-24)
+        assert torch.equal(r.y.float(), b.expand(1, N, 8))
