@@ -72,30 +72,34 @@ __device__ __forceinline__ int live_rows(const NormArgs &a, int b) {
 __device__ __forceinline__ float sigmoid_fast(float z) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
 }
-// Phi(z) = (1 + erf(z / sqrt 2)) / 2 and *e = exp(-z^2 / 2), by formula 7.1.26 of Abramowitz and
-// Stegun (Hastings): 1 - erf(x) = (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 + p x), |error| <= 1.5e-7
+// Phi(z) = (1 + erf(z / sqrt 2)) / 2 and *e = exp(-z^2 / 2).  FULL (fp32 tensors): with erff.  Else by
+// formula 7.1.26 of Abramowitz and Stegun (Hastings): 1 - erf(x) = (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 + p x),
+// |error| <= 1.5e-7, in half the instructions: under the rounding of 16-bit values, over that of fp32 (GELU of
+// normal values off by 5.6e-8 rms, 2.4e-8 with erff).
+template <bool FULL>
 __device__ __forceinline__ float normal_cdf(float z, float *e) {
+  *e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
+  if (FULL) return __fmaf_rn(0.5f, erff(z * 0.70710678118654752f), 0.5f);
   const float x = fabsf(z) * 0.70710678118654752f;
   const float t = __builtin_amdgcn_rcpf(__fmaf_rn(0.3275911f, x, 1.0f));
   float p = __fmaf_rn(1.061405429f, t, -1.453152027f);
   p = __fmaf_rn(p, t, 1.421413741f);
   p = __fmaf_rn(p, t, -0.284496736f);
   p = __fmaf_rn(p, t, 0.254829592f);
-  *e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
   const float tail = 0.5f * p * t * *e;                  // 1 - Phi(|z|)
   return z < 0.0f ? tail : 1.0f - tail;
 }
-template <int ACT>
+template <int ACT, bool FULL>
 __device__ __forceinline__ float act_value(float z) {
   if (ACT == GVAE_ACT_RELU) return z < 0.0f ? 0.0f : z;   // (keeps a NaN)
   if (ACT == GVAE_ACT_SILU) return z * sigmoid_fast(z);
   if (ACT == GVAE_ACT_GELU) {
     float e;
-    return z * normal_cdf(z, &e);
+    return z * normal_cdf<FULL>(z, &e);
   }
   return z;
 }
-template <int ACT>
+template <int ACT, bool FULL>
 __device__ __forceinline__ float act_slope(float z) {
   if (ACT == GVAE_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
   if (ACT == GVAE_ACT_SILU) {
@@ -104,7 +108,7 @@ __device__ __forceinline__ float act_slope(float z) {
   }
   if (ACT == GVAE_ACT_GELU) {
     float e;
-    const float c = normal_cdf(z, &e);
+    const float c = normal_cdf<FULL>(z, &e);
     return __fmaf_rn(z * 0.39894228040143268f, e, c);
   }
   return 1.0f;
@@ -114,12 +118,12 @@ __device__ __forceinline__ float pre_act(float h, float w, float b) {
   return ACT == GVAE_ACT_RELU ? h * w + b : __fmaf_rn(h, w, b);
 }
 // the same for a piece, with the activation chosen at run time (uniform over the launch)
-template <int V>
+template <int V, bool FULL>
 __device__ __forceinline__ void act_values(int act, const float *h, const float *w, const float *b, float *y) {
   auto all = [&](auto tag) {
     constexpr int ACT = decltype(tag)::value;
 #pragma unroll
-    for (int v = 0; v < V; ++v) y[v] = act_value<ACT>(pre_act<ACT>(h[v], w[v], b[v]));
+    for (int v = 0; v < V; ++v) y[v] = act_value<ACT, FULL>(pre_act<ACT>(h[v], w[v], b[v]));
   };
   switch (act) {
     case GVAE_ACT_RELU: all(std::integral_constant<int, GVAE_ACT_RELU>{}); break;
@@ -128,12 +132,12 @@ __device__ __forceinline__ void act_values(int act, const float *h, const float 
     default: all(std::integral_constant<int, GVAE_ACT_NONE>{}); break;
   }
 }
-template <int V>
+template <int V, bool FULL>
 __device__ __forceinline__ void act_slopes(int act, const float *h, const float *w, const float *b, float *s) {
   auto all = [&](auto tag) {
     constexpr int ACT = decltype(tag)::value;
 #pragma unroll
-    for (int v = 0; v < V; ++v) s[v] = act_slope<ACT>(pre_act<ACT>(h[v], w[v], b[v]));
+    for (int v = 0; v < V; ++v) s[v] = act_slope<ACT, FULL>(pre_act<ACT>(h[v], w[v], b[v]));
   };
   switch (act) {
     case GVAE_ACT_RELU: all(std::integral_constant<int, GVAE_ACT_RELU>{}); break;

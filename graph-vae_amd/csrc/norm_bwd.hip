@@ -94,7 +94,7 @@ __global__ __launch_bounds__(NT) void norm_bwd_resident_kernel(NormArgs a) {
         x[u].cut(cut);
 #pragma unroll
         for (int v = 0; v < V; ++v) h[v] = (x[u].at(v) - mean[IN ? 0 : v]) * rstd[IN ? 0 : v];
-        act_slopes<V>(a.act, h, w, bias, s);
+        act_slopes<V, sizeof(T) == 4>(a.act, h, w, bias, s);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           dz[u][v] = (float)g[u][v] * s[v];
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_sums_kernel(NormArgs a) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const float h = k.centred(v, x[u].at(v));
-          const float dz = (float)g[u][v] * act_slope<ACT>(k.template pre<ACT>(v, h));
+          const float dz = (float)g[u][v] * act_slope<ACT, sizeof(T) == 4>(k.template pre<ACT>(v, h));
           s1[v] += dz;
           s2[v] = __fmaf_rn(dz, h, s2[v]);
         }
@@ -328,7 +328,7 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_apply_kernel(NormArgs a) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const float h = k.centred(v, x[u].at(v));
-          const float dz = (float)g[u][v] * act_slope<ACT>(k.template pre<ACT>(v, h));
+          const float dz = (float)g[u][v] * act_slope<ACT, sizeof(T) == 4>(k.template pre<ACT>(v, h));
           dx[v] = __fmaf_rn(dz, wr[v], -__fmaf_rn(h, a2[v], a1[v]));
         }
       }

@@ -112,7 +112,7 @@ __global__ __launch_bounds__(NT) void norm_resident_kernel(NormArgs a) {
         xf[v] = (float)k[u][v];
         y[v] = (xf[v] - mean[IN ? 0 : v]) * rstd[IN ? 0 : v];
       }
-      act_values<V>(a.act, y, w, bias, y);
+      act_values<V, sizeof(T) == 4>(a.act, y, w, bias, y);
     }
     const int64_t row = (int64_t)b * a.N + i;
     if (nv > 0) store_piece<PAST, T>((T *)a.out + row * a.C + c0, y, nv);
@@ -295,7 +295,7 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(NormArgs a) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           xf[v] = (float)r[u][v];
-          y[v] = act_value<ACT>(k.template pre<ACT>(v, k.centred(v, xf[v])));
+          y[v] = act_value<ACT, sizeof(T) == 4>(k.template pre<ACT>(v, k.centred(v, xf[v])));
         }
       }
       const int64_t row = (int64_t)p.b * a.N + i;
