@@ -8,8 +8,10 @@ stream of the current device (libgvae_hip.so; there is no CPU fallback):
   checkpoint8               an activation into an 8-bit checkpoint; Checkpoint8.read() brings it back
   linear_wgrad8             weight and bias gradient of a linear layer from its input's checkpoint
 
-They are plain calls: nothing here is recorded by autograd.  `GraphVAE(norm="group")` builds its
-encoder from the same kernels, and its backward from the gradients here.
+They are plain calls: nothing here is recorded by autograd, and a tensor that requires grad is refused while
+grad mode is on (a graph would end there without a word).  Call them under `torch.no_grad()` or from the
+forward and backward of a `torch.autograd.Function`.  `GraphVAE(norm="group")` builds its encoder from the same
+kernels, and its backward from the gradients here.
 """
 from __future__ import annotations
 
@@ -56,6 +58,17 @@ _empty = torch.empty
 def _empty_as(t: torch.Tensor) -> torch.Tensor:
     """A contiguous tensor of t's shape, type and device (empty_like is half a microsecond less than empty)."""
     return torch.empty_like(t) if t.is_contiguous() else _empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+_grad_mode = torch.is_grad_enabled
+
+
+def _unrecorded(what: str, *tensors) -> None:
+    """Refuses tensors whose gradient would be dropped (called with grad mode on)."""
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and t.requires_grad:
+            raise _hip.GvaeHipError(f"{what}: an input requires grad, and the operators here are not recorded by "
+                                    "autograd: call it under torch.no_grad() or from a torch.autograd.Function")
 
 
 def _act_code(act: str) -> int:
@@ -213,6 +226,8 @@ class Checkpoint8:
 def checkpoint8(x: torch.Tensor) -> Checkpoint8:
     """8-bit checkpoint of x (..., C) float32 / bfloat16 / float16: contiguous, or a matrix with any
     row stride.  A block of 32 channels that holds an infinity or a NaN reads back as NaN."""
+    if _grad_mode():
+        _unrecorded("checkpoint8", x)
     index = _on_device(x, "checkpoint8")
     code = _activation(x, "checkpoint8")
     rows, ld = _rows_of(x, "checkpoint8")
@@ -255,6 +270,8 @@ def group_norm_act(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Ten
     and come out 0, a graph without any has mean 0 and variance 0.  keep_x / keep_y: also return 8-bit
     checkpoints of x (dead rows as 0) and of y, the same as `checkpoint8` of them."""
     what = "group_norm_act"
+    if _grad_mode():
+        _unrecorded(what, x, weight, bias)
     B, N, C = _norm_sizes(x.shape, groups, what)
     act_code = _act_code(act)
     index = _on_device(x, what)
@@ -292,6 +309,8 @@ def group_norm_act_backward(dy: torch.Tensor, x, weight: torch.Tensor | None, bi
     rows is 0."""
     what = "group_norm_act_backward"
     kept = isinstance(x, Checkpoint8)
+    if _grad_mode():
+        _unrecorded(what, dy, x, weight, bias)
     B, N, C = _norm_sizes(dy.shape, groups, what)
     act_code = _act_code(act)
     index = _on_device(dy, what)
@@ -334,6 +353,8 @@ def linear_wgrad8(dy: torch.Tensor, x8: Checkpoint8) -> tuple[torch.Tensor, torc
     gradient dy (..., O) and the checkpoint of its input (..., I).  dy: contiguous, or a matrix with any
     row stride.  Every product is exact, sums are float32 in a fixed order, rounded once."""
     what = "linear_wgrad8"
+    if _grad_mode():
+        _unrecorded(what, dy)
     if not isinstance(x8, Checkpoint8):
         raise _hip.GvaeHipError(f"{what}: the input must be a Checkpoint8")
     x8._check(what)

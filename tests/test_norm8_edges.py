@@ -152,3 +152,63 @@ def test_gelu_in_fp32_has_the_precision_of_its_plain_form(N, lo, hi):
     for got, form, want in zip((r.y[0, 0], db), plain, (act_ref(z.double(), "gelu"), slope_ref(z.double(), "gelu"))):
         rms = [float((t.cpu().double() - want).square().mean().sqrt()) for t in (got, form)]
         assert 0.0 < rms[0] <= 1.5 * rms[1], rms
+
+
+# ------------------------------------------------------------------ autograd
+def test_inputs_that_require_grad_are_refused():
+    """While grad mode is on; with it off the same calls get as far as asking for a device."""
+    from graphvae import _hip, ops
+    x, g, w = torch.zeros(2, 4, 32), torch.zeros(2, 4, 32), torch.ones(32)
+    st = torch.zeros(2, 4)
+    c = ops.Checkpoint8(torch.zeros(2, 4, 32, dtype=torch.int8), torch.zeros(2, 4, 1, dtype=torch.uint8), 32)
+
+    def calls(x, g, w, b):
+        return [lambda: ops.group_norm_act(x, w, b, 4), lambda: ops.group_norm_act_backward(g, x, w, b, st, st, 4)]
+
+    for k in range(4):
+        args = [x, g, w, w.clone()]
+        args[k] = args[k].clone().requires_grad_()
+        for n, call in enumerate(calls(*args)):
+            with pytest.raises(_hip.GvaeHipError, match="expected a device tensor" if (n, k) == (0, 1) else "requires grad"):
+                call()
+            with torch.no_grad(), pytest.raises(_hip.GvaeHipError, match="expected a device tensor"):
+                call()
+    lone = [lambda t: ops.checkpoint8(t), lambda t: ops.linear_wgrad8(t, c),
+            lambda t: ops.group_norm_act_backward(t, c, w, None, st, st, 4)]
+    for call in lone:
+        with pytest.raises(_hip.GvaeHipError, match="requires grad"):
+            call(x.clone().requires_grad_())
+        with torch.no_grad(), pytest.raises(_hip.GvaeHipError, match="expected a device tensor"):
+            call(x.clone().requires_grad_())
+        with pytest.raises(_hip.GvaeHipError, match="expected a device tensor"):
+            call(x)
+
+
+class _NormFunction(torch.autograd.Function):
+    """The operators in an autograd node, the input kept in 8 bits."""
+
+    @staticmethod
+    def forward(ctx, x, w, b):
+        from graphvae import ops
+        r = ops.group_norm_act(x, w, b, 4, act="silu", keep_x=True)
+        ctx.kept, ctx.args = r.x8, (w, b, r.mean, r.rstd)
+        return r.y
+
+    @staticmethod
+    def backward(ctx, dy):
+        from graphvae import ops
+        return ops.group_norm_act_backward(dy, ctx.kept, *ctx.args, 4, act="silu")
+
+
+@gpu
+def test_operators_in_an_autograd_function():
+    """Leaves that require grad, through a Function: the gradients of the plain calls, bit for bit."""
+    from graphvae import ops
+    g = torch.Generator(device="cuda").manual_seed(27)
+    leaves = [torch.randn(s, generator=g, device="cuda").requires_grad_() for s in ((3, 20, 48), (48,), (48,))]
+    y = _NormFunction.apply(*leaves)
+    y.sum().backward()
+    x, w, b = (t.detach() for t in leaves)
+    r = ops.group_norm_act(x, w, b, 4, act="silu", keep_x=True)
+    want = ops.group_norm_act_backward(torch.ones_like(x), r.x8, w, b, r.mean, r.rstd, 4, act="silu")
+    assert torch.equal(y.detach(), r.y) and all(torch.equal(t.grad, e) for t, e in zip(leaves, want))
