@@ -34,7 +34,10 @@ def load_model(run_dir: Path, device) -> tuple[GraphVAE, dict]:
     in_dim = cfg.get("in_dim") or state["conv1.lin.weight"].shape[1]
     pairs = cfg.get("off_diag") or state["dec_edge.2.weight"].size(0)
     max_nodes = cfg.get("max_nodes") or int((1 + math.isqrt(1 + 8 * pairs)) // 2)
-    model = GraphVAE(in_dim, cfg["hid_dim"], cfg["z_dim"], max_nodes, pool=cfg.get("pool", "sum"))
+    # (the state dict has the same keys for either norm; runs without these entries were trained with BatchNorm)
+    model = GraphVAE(in_dim, cfg["hid_dim"], cfg["z_dim"], max_nodes, pool=cfg.get("pool", "sum"),
+                     norm=cfg.get("norm") or "batch", norm_groups=cfg.get("norm_groups") or 8,
+                     act_bits=cfg.get("act_bits") or 32)
     model.load_state_dict(state, strict=True)
     return model.to(device).eval(), cfg
 

@@ -305,3 +305,44 @@ def test_workspace_holds_every_batch_size(N, H, sizes):
             need = (eng.L.gvae_step_ws_bytes(ctypes.byref(eng.dims), B) if eng.gn is None else
                     eng.L.gvae_step_gn_ws_bytes(ctypes.byref(eng.dims), ctypes.byref(eng.gn), B))
             assert eng._ws.numel() >= need > 0, (kw, B)
+
+
+def _load_model(run, device):
+    sys.path.insert(0, str(ROOT / "graph-vae_amd" / "experiments"))
+    from sample import load_model
+    return load_model(run, device)[0]
+
+
+@pytest.mark.parametrize("entries,want", [({}, ("batch", 8, 32)), ({"norm": None}, ("batch", 8, 32)),
+                                          ({"norm": "batch", "norm_groups": 8, "act_bits": 32}, ("batch", 8, 32)),
+                                          ({"norm": "group", "norm_groups": 4, "act_bits": 8}, ("group", 4, 8)),
+                                          ({"norm": "group", "norm_groups": 2, "act_bits": 32}, ("group", 2, 32))])
+def test_a_run_is_loaded_with_its_norm(tmp_path, entries, want):
+    import yaml
+    from graphvae.models import GraphVAE
+    torch.save(GraphVAE(1, 16, 4, 6).state_dict(), tmp_path / "graphvae_ddp.pt")
+    (tmp_path / "params.yaml").write_text(yaml.safe_dump({"hid_dim": 16, "z_dim": 4, **entries}))
+    model = _load_model(tmp_path, "cpu")
+    assert (model.norm, model.norm_groups, model.act_bits) == want
+
+
+@gpu
+def test_a_trained_run_evaluates_as_it_was_trained(tmp_path):
+    """A run of the trainer's command line, loaded for sampling: its forward is that of the trained model."""
+    from graphvae.data import synthetic_batch
+    from graphvae.models import GraphVAE
+    from graphvae.train import train_ddp as T
+    T.main(["--dataset", "synthetic-dense", "--feature_type", "deg", "--max_nodes", "16", "--epochs", "1", "--norm", "group",
+            "--norm_groups", "4", "--act_bits", "8", "--log_dir", str(tmp_path), "--no_wandb"])
+    loaded = _load_model(tmp_path, DEV)
+    hid, z = loaded.hid_dim, loaded.z_dim
+    built = GraphVAE(1, hid, z, 16, norm="group", norm_groups=4, act_bits=8)
+    built.load_state_dict(torch.load(tmp_path / "graphvae_ddp.pt", weights_only=True), strict=True)
+    hb = synthetic_batch("dense", 7, 16, "deg", seed=6)
+    eps = torch.randn(7, z, generator=torch.Generator().manual_seed(6)).to(DEV)
+    outs = []
+    for model in (loaded, built.to(DEV).eval()):
+        model.precompute_dataset_rho([hb])
+        with torch.no_grad():
+            outs.append(model.forward_with_eps(hb.to(DEV), eps))
+    assert all(torch.equal(outs[0][k], outs[1][k]) for k in ("rec", "kl"))
