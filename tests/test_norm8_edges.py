@@ -197,7 +197,8 @@ class _NormFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         from graphvae import ops
-        return ops.group_norm_act_backward(dy, ctx.kept, *ctx.args, 4, act="silu")
+        # (the gradient of a sum is one value expanded along all axes; channels have to be contiguous)
+        return ops.group_norm_act_backward(dy.contiguous(), ctx.kept, *ctx.args, 4, act="silu")
 
 
 @gpu
