@@ -346,3 +346,31 @@ def test_a_trained_run_evaluates_as_it_was_trained(tmp_path):
         with torch.no_grad():
             outs.append(model.forward_with_eps(hb.to(DEV), eps))
     assert all(torch.equal(outs[0][k], outs[1][k]) for k in ("rec", "kl"))
+
+
+@gpu
+@pytest.mark.parametrize("matching", ["fused", "stream"])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_steps_in_flight_equal_the_sequential_schedule(matching, bits):
+    """Eleven pipelined steps over four workspaces, batches of two sizes and their noise on the device beforehand and
+    nothing waited for or read until the last: losses, their sum and the parameters bit for bit those of
+    steps run one after the other."""
+    from graphvae.data import synthetic_batch
+    from graphvae.train.train_ddp import TrainStep
+    N, steps = 24, 11
+    host = [synthetic_batch("enzymes", b, N, "deg", seed=b) for b in (40, 57, 41)]
+    order = [host[s % 3] for s in range(steps)]
+    gen = torch.Generator().manual_seed(9)
+    noise = [torch.randn(hb.num_graphs, 32, generator=gen).to(DEV) for hb in order]
+    batches = {id(hb): hb.to(DEV) for hb in host}
+    runs = []
+    for overlap, pipeline in ((False, False), (True, True)):
+        model, _ = _model(1, 64, 32, N, 8, bits, host[0], matching)
+        model = model.to(DEV).train()
+        step = TrainStep(model, 1e-2, 1e-4, 5.0, overlap_matching=overlap, pipeline=pipeline, slots=4)
+        torch.cuda.synchronize()
+        outs = [step(batches[id(hb)], 0.5, 1.0, eps=e) for hb, e in zip(order, noise)]
+        step.wait()
+        runs.append([torch.stack(outs).cpu(), step.pop_loss_sum().cpu(), model.flat_parameters().detach().cpu().clone()])
+        model._engine.check_matching()
+    assert torch.isfinite(runs[0][2]).all() and all(torch.equal(a, b) for a, b in zip(*runs))
