@@ -213,3 +213,33 @@ def test_operators_in_an_autograd_function():
     r = ops.group_norm_act(x, w, b, 4, act="silu", keep_x=True)
     want = ops.group_norm_act_backward(torch.ones_like(x), r.x8, w, b, r.mean, r.rstd, 4, act="silu")
     assert torch.equal(y.detach(), r.y) and all(torch.equal(t.grad, e) for t, e in zip(leaves, want))
+
+
+# ------------------------------------------------------------------ weight gradients of the smallest gradients
+@gpu
+@pytest.mark.parametrize("dtype,exponent", [(torch.float32, -110), (torch.float32, -103), (torch.bfloat16, -133),
+                                            (torch.bfloat16, -126), (torch.float16, -24), (torch.float16, -15)])
+def test_wgrad_of_small_gradients(dtype, exponent):
+    """One row, one power of two as input: dW is the gradient times it, exactly, down to where the last piece
+    of a gradient is the smallest bf16 number, 2^-133: |dy| >= 2^-110 in fp32, every value of bf16 and half."""
+    from graphvae import ops
+    g = torch.Generator().manual_seed(28)
+    dy = (2.0 ** exponent * (1 + torch.rand(1, 200, generator=g, dtype=torch.float64))).to(dtype)
+    dy[0, ::3] *= -1
+    up = 60 if dtype != torch.float16 else 8
+    c = ops.checkpoint8(torch.full((1, 40), 2.0 ** up).cuda())
+    dw, db = ops.linear_wgrad8(dy.cuda(), c)
+    want = (dy.double() * 2.0 ** up).t().expand(200, 40).to(dtype)
+    assert torch.equal(dw.cpu(), want) and torch.equal(db.cpu(), dy[0]) and dy.all()
+
+
+@gpu
+def test_wgrad_below_the_smallest_piece():
+    """fp32 gradients under 2^-110: what lies below 2^-133 is dropped, and no more."""
+    from graphvae import ops
+    g = torch.Generator().manual_seed(29)
+    dy = (torch.randn(1, 300, generator=g) * torch.exp2(-torch.randint(110, 136, (1, 300), generator=g).float())).float()
+    c = ops.checkpoint8(torch.full((1, 40), 2.0 ** 60).cuda())
+    dw, db = ops.linear_wgrad8(dy.cuda(), c)
+    want = (dy.double() * 2.0 ** 60).t().expand(300, 40)
+    assert ((dw.cpu().double() - want).abs() < 2.0 ** (60 - 133)).all() and torch.equal(db.cpu(), dy[0])
