@@ -198,10 +198,10 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_sums_kernel(NormArgs a) {
         x[u].cut(cut);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float h = k.centred(v, x[u].at(v));
-          const float dz = (float)g[u][v] * act_slope<ACT, sizeof(T) == 4>(k.template pre<ACT>(v, h));
+          const float c = k.centred(v, x[u].at(v));
+          const float dz = (float)g[u][v] * act_slope<ACT, sizeof(T) == 4>(k.template pre<ACT>(v, c));
           s1[v] += dz;
-          s2[v] = __fmaf_rn(dz, h, s2[v]);
+          s2[v] = __fmaf_rn(dz, c, s2[v]);
         }
       }
     }
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_apply_kernel(NormArgs a) {
     const int64_t q = (int64_t)p.b * a.G + (p.c0 + (v < p.nv ? v : 0)) / a.cpg;
     const float r = k.rstd[v] * k.unit[v];
     a1[v] = a.A[2 * q] * r;
-    a2[v] = a.A[2 * q + 1] * r * k.unit[v];
+    a2[v] = a.A[2 * q + 1] * r;
     wr[v] = k.w[v] * k.rstd[v];
   }
   const T *dy = (const T *)a.dy + p.b * a.dyb;
@@ -327,9 +327,9 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_apply_kernel(NormArgs a) {
         x[u].cut(cut);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float h = k.centred(v, x[u].at(v));
-          const float dz = (float)g[u][v] * act_slope<ACT, sizeof(T) == 4>(k.template pre<ACT>(v, h));
-          dx[v] = __fmaf_rn(dz, wr[v], -__fmaf_rn(h, a2[v], a1[v]));
+          const float c = k.centred(v, x[u].at(v));
+          const float dz = (float)g[u][v] * act_slope<ACT, sizeof(T) == 4>(k.template pre<ACT>(v, c));
+          dx[v] = __fmaf_rn(dz, wr[v], -__fmaf_rn(c * k.unit[v], a2[v], a1[v]));
         }
       }
       store_piece<PAST, T>((T *)a.out + ((int64_t)p.b * a.N + i) * a.C + p.c0, dx, p.nv);

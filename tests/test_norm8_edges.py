@@ -4,7 +4,7 @@ in test_norm8.py: u = 2^-24 for every fp32 operation, half a step of the type fo
 import pytest
 import torch
 
-from test_norm8 import ACTS, DEPTH, DTYPES, U32, act_ref, half_step, make_x, norm_ref, per_channel, slope_ref, subnormal
+from test_norm8 import ACTS, DEPTH, DTYPES, U32, act_ref, bwd_ref, half_step, make_x, norm_ref, per_channel, slope_ref, subnormal
 
 gpu = pytest.mark.gpu
 
@@ -128,6 +128,28 @@ def test_large_constant_rows_in_both_forms():
         b = torch.arange(8, dtype=torch.float32, device="cuda")
         r = ops.group_norm_act(x, None, b, 2, act="none", eps=1e-24)
         assert torch.equal(r.y.float(), b.expand(1, N, 8))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(3, 40, 48, 6), (2, 4000, 48, 6), (2, 6000, 45, 9)])
+@pytest.mark.parametrize("scale", [2.0 ** -62, 2.0 ** 60])
+def test_gradients_of_very_small_and_very_large_values(dtype, shape, scale):
+    """The norm does not depend on the scale of its input: with mean and rstd to match, gradients times 2^12 of
+    values of 2^-62 and 2^60 stay within the bounds of ordinary ones."""
+    from graphvae import ops
+    B, N, C, G = shape
+    x, w, b, rows, dy = make_x(B, N, C, dtype, 31)
+    x, dy = x * scale, dy * 2.0 ** 12
+    x = torch.where(torch.arange(N)[None, :, None] < rows[:, None, None], x, torch.zeros_like(x))
+    g = torch.Generator().manual_seed(32)
+    mean, rstd = 0.3 * torch.randn(B, G, generator=g) * scale, (0.5 + torch.rand(B, G, generator=g)) / scale
+    for act in ("none", "silu"):
+        got = ops.group_norm_act_backward(dy.cuda(), x.cuda(), w.cuda(), b.cuda(), mean.cuda(), rstd.cuda(), G, act=act,
+                                          rows=rows.cuda())
+        dx, dw, db, edx, edw, edb = bwd_ref(dy, x, w, b, mean, rstd, G, act, rows)
+        assert ((got[0].cpu().double() - dx).abs() <= half_step(dtype) * dx.abs() + 1.01 * edx + subnormal(dtype)).all()
+        assert ((got[1].cpu().double() - dw).abs() <= 2 * edw).all() and ((got[2].cpu().double() - db).abs() <= 2 * edb).all()
 
 
 # ------------------------------------------------------------------ activations
