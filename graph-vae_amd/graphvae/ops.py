@@ -60,15 +60,14 @@ def _empty_as(t: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(t) if t.is_contiguous() else _empty(t.shape, dtype=t.dtype, device=t.device)
 
 
-_grad_mode = torch.is_grad_enabled
+_any_requires_grad = torch._C._any_requires_grad
 
 
-def _unrecorded(what: str, *tensors) -> None:
-    """Refuses tensors whose gradient would be dropped (called with grad mode on)."""
-    for t in tensors:
-        if isinstance(t, torch.Tensor) and t.requires_grad:
-            raise _hip.GvaeHipError(f"{what}: an input requires grad, and the operators here are not recorded by "
-                                    "autograd: call it under torch.no_grad() or from a torch.autograd.Function")
+def _refuse_recorded(what: str) -> None:
+    """Refuses inputs that require grad, whose gradient would be dropped, unless grad mode is off."""
+    if torch.is_grad_enabled():
+        raise _hip.GvaeHipError(f"{what}: an input requires grad, and the operators here are not recorded by "
+                                "autograd: call it under torch.no_grad() or from a torch.autograd.Function")
 
 
 def _act_code(act: str) -> int:
@@ -226,8 +225,8 @@ class Checkpoint8:
 def checkpoint8(x: torch.Tensor) -> Checkpoint8:
     """8-bit checkpoint of x (..., C) float32 / bfloat16 / float16: contiguous, or a matrix with any
     row stride.  A block of 32 channels that holds an infinity or a NaN reads back as NaN."""
-    if _grad_mode():
-        _unrecorded("checkpoint8", x)
+    if _any_requires_grad(x):
+        _refuse_recorded("checkpoint8")
     index = _on_device(x, "checkpoint8")
     code = _activation(x, "checkpoint8")
     rows, ld = _rows_of(x, "checkpoint8")
@@ -270,8 +269,8 @@ def group_norm_act(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Ten
     and come out 0, a graph without any has mean 0 and variance 0.  keep_x / keep_y: also return 8-bit
     checkpoints of x (dead rows as 0) and of y, the same as `checkpoint8` of them."""
     what = "group_norm_act"
-    if _grad_mode():
-        _unrecorded(what, x, weight, bias)
+    if _any_requires_grad(x, weight, bias):
+        _refuse_recorded(what)
     B, N, C = _norm_sizes(x.shape, groups, what)
     act_code = _act_code(act)
     index = _on_device(x, what)
@@ -309,8 +308,8 @@ def group_norm_act_backward(dy: torch.Tensor, x, weight: torch.Tensor | None, bi
     rows is 0."""
     what = "group_norm_act_backward"
     kept = isinstance(x, Checkpoint8)
-    if _grad_mode():
-        _unrecorded(what, dy, x, weight, bias)
+    if _any_requires_grad(dy, x, weight, bias):
+        _refuse_recorded(what)
     B, N, C = _norm_sizes(dy.shape, groups, what)
     act_code = _act_code(act)
     index = _on_device(dy, what)
@@ -353,8 +352,8 @@ def linear_wgrad8(dy: torch.Tensor, x8: Checkpoint8) -> tuple[torch.Tensor, torc
     gradient dy (..., O) and the checkpoint of its input (..., I).  dy: contiguous, or a matrix with any
     row stride.  Every product is exact, sums are float32 in a fixed order, rounded once."""
     what = "linear_wgrad8"
-    if _grad_mode():
-        _unrecorded(what, dy)
+    if _any_requires_grad(dy):
+        _refuse_recorded(what)
     if not isinstance(x8, Checkpoint8):
         raise _hip.GvaeHipError(f"{what}: the input must be a Checkpoint8")
     x8._check(what)
