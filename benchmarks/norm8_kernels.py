@@ -1,4 +1,5 @@
-"""Run the cases of perf/operators.py on graphvae.ops, 20 calls each, for a kernel trace:
+"""Run the cases of perf/operators.py on graphvae.ops, 400 calls each (the clocks settle after some tens), for a
+kernel trace:
 rocprofv3 --kernel-trace --stats --output-format csv -d OUT -- python3 benchmarks/norm8_kernels.py [case,case]"""
 import sys
 from pathlib import Path
@@ -14,7 +15,7 @@ for case in cases.listed():
     if only and case["name"] not in only:
         continue
     state = cases.prepare(dict(case), 1)
-    for _ in range(20):
+    for _ in range(400):
         cases.run(state)
     torch.cuda.synchronize()
     print(case["name"], flush=True)

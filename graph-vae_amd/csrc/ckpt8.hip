@@ -1,8 +1,8 @@
 // Activations into 8-bit checkpoints and back (the format: gvae_ckpt8.h).  Bound by memory: a value
 // is read once and a byte written, or the other way round.  A lane holds 16 bytes of a row, four (16-bit
 // types) or eight neighbouring lanes a block; the block's largest magnitude is an integer maximum of
-// bit patterns over its lanes.  262144 rows of 1024, bf16 (537 MB and 277 MB): written in 155 us, read
-// in 132 (5.3 and 6.2 TB/s); four pieces of a lane in flight instead of one were slower.
+// bit patterns over its lanes.  262144 rows of 1024, bf16 (537 MB and 277 MB): written in 145 us, read
+// in 137 (5.6 and 5.9 TB/s; medians of 400 calls); four pieces of a lane in flight instead of one were slower.
 #include "gvae_ckpt8.h"
 
 #include <type_traits>

@@ -4,10 +4,11 @@
 // Checkpoint format.  A row of C values is cut into blocks of 32 consecutive channels.  A block
 // holds one byte s and a signed code per value, value = code * 2^(s - 127), where e = s - 127 is the
 // least integer >= -126 with max|x| <= 127 * 2^e and code = x / 2^e rounded to nearest, ties to
-// even: off by at most 2^(e-1) <= max|x| / 127.  A power of two as the scale keeps every step
-// exact: x / 2^e is an exponent shift, and code * 2^e has at most 7 significant bits and is a
-// value of bfloat16, of float and (inside its range) of half.  A block with an infinity or a NaN
-// has s = 255 and codes 0 and reads as NaN throughout.
+// even: off by at most 2^(e-1), which is under max|x| / 127 unless e = -126.  At e = 122 (max|x| over
+// 127 * 2^121, within 1 % of the largest float) codes end at 63, since 64 * 2^122 is no float: off by at most
+// 2^122.  A power of two as the scale keeps every step exact: x / 2^e is an exponent shift, and code * 2^e
+// has at most 7 significant bits and is a value of bfloat16, of float and (inside its range) of half.  A block
+// with an infinity or a NaN has s = 255 and codes 0 and reads as NaN throughout; s = 0, never written, reads as 0.
 // Codes of a row take ld = 16 * ceil(C / 16) bytes (the tail is zero) so that every row can be read
 // in 16-byte pieces; scales take ceil(C / 32) bytes.
 #pragma once
@@ -165,7 +166,7 @@ __device__ __forceinline__ void emit8(const float *f, int8_t *codes, int nc, uin
   m = lanes_max<kBlock8 / V>(m);
   const uint32_t s = scale_byte(m);
   // Adding 1.5 * 2^23 rounds to an integer, ties to even, whose low byte is the code's; the product before it
-  // is exact.  (|x| / 2^e is at most 127; at 2^122 a largest value that rounds up to 2^128 is kept below it)
+  // is exact.  (|x| / 2^e is at most 127; at 2^122, where 64 steps are no float any more, at most 63)
   constexpr float kShift = 12582912.0f;
   const float lim = s == 249u ? 63.0f : 127.0f;
   const float inv = s == 255u ? 0.0f : pow2_field(254u - s);

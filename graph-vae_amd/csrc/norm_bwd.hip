@@ -1,10 +1,10 @@
 // Group norm with an activation: gradients (gvae_norm.h has the mathematics and the two forms).
 //
-// Measured.  Resident: 256 graphs of 250 rows, 512 channels, bf16, SiLU 56 us (197 MB, 3.5 TB/s: loads, sums
-// and writes of a slab follow one another, and registers leave few work-groups to a CU); 64 ragged graphs of
-// at most 126 rows, 128 channels, float, from the checkpoint 7.2 us and 2.9 for dw and db.  Split: 16
-// graphs of 16384 rows, 512 channels, bf16, SiLU, from the checkpoint: sums 87 us (406 MB, bound by
-// the vector units), join 6, second pass 120 (675 MB, 5.6 TB/s).
+// Measured (medians of 400 calls).  Resident: 256 graphs of 250 rows, 512 channels, bf16, SiLU 51 us and 5 for
+// dw and db (197 MB, 3.9 TB/s: loads, sums and writes of a slab follow one another, and registers leave few
+// work-groups to a CU); 64 ragged graphs of at most 126 rows, 128 channels, float, from the checkpoint 7.2 us
+// and 2.9.  Split: 16 graphs of 16384 rows, 512 channels, bf16, SiLU, from the checkpoint: sums 80 to 82 us
+// (406 MB, 5 TB/s, bound by the vector units as much), join 6, second pass 120 (675 MB, 5.6 TB/s).
 #include "gvae_norm.h"
 
 namespace gvae {

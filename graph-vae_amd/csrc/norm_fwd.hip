@@ -3,11 +3,11 @@
 // Split form: what a chunk leaves is one (mean, M2) pair per channel, combined as n, mean, M2 with
 // M2 = M2a + M2b + d^2 na nb / n, so no square of an uncentred value is ever summed.
 //
-// Measured (bf16, SiLU).  Resident: 256 graphs of 250 rows, 512 channels 33 us (131 MB, 4.0 TB/s); in a few
-// MB the latency of one work-group remains: 256 graphs of 32 rows, 128 channels, float, with both
-// checkpoints 8.9 us, a graph of 20 rows 5.1.  Split: 4 graphs of 65536 rows, 320 channels: sums 35 us
-// (4.8 TB/s), join 6, second pass 57 (336 MB, 5.9 TB/s); 192 ragged graphs of 1000 rows, 512 channels, with
-// both checkpoints: 28 + 6 + 101.
+// Measured (bf16, SiLU; medians of 400 calls).  Resident: 256 graphs of 250 rows, 512 channels 32 us (131 MB,
+// 4.1 TB/s); in a few MB the latency of one work-group remains: 256 graphs of 32 rows, 128 channels, float,
+// with both checkpoints 9.0 us, a graph of 20 rows 5.3.  Split: 4 graphs of 65536 rows, 320 channels: sums 33 us
+// (5.1 TB/s), join 6, second pass 57 (336 MB, 5.9 TB/s); 192 ragged graphs of 1000 rows, 512 channels, with
+// both checkpoints: 25 + 6 + 93.
 #include "gvae_norm.h"
 
 namespace gvae {

@@ -2,9 +2,10 @@
 //   dW[o,i] = sum_t dY[t,o] * code[t,i] * 2^(s[t,i/32] - 127),   db[o] = sum_t dY[t,o]
 //
 // On the matrix cores in bf16 without a rounding of either factor: code * 2^e has 7 significant bits
-// and is a bf16 value as it stands; a gradient is cut into bf16 pieces that add up to it exactly, one
-// for bf16 (8 significant bits), two for half (11), three for float (24), each multiplied in turn.
-// Sums are fp32 (v_mfma_f32_32x32x16_bf16).
+// and is a bf16 value as it stands; a gradient is cut into bf16 pieces that add up to it, one for bf16 (8
+// significant bits), two for half (11), three for float (24), each multiplied in turn.  The matrix cores keep
+// subnormal pieces, so that bf16 and half enter exactly throughout and float from 2^-110 on; of a smaller
+// float what lies below 2^-133, the least bf16 number, is dropped.  Sums are fp32 (v_mfma_f32_32x32x16_bf16).
 //
 // Both factors lie with the summed axis outermost in memory, so a lane's eight consecutive rows of
 // one column are a column of the tile: tiles are staged row by row in LDS and read through
@@ -12,10 +13,11 @@
 // of one column each).  Those 4 rows are brought to different banks by XORing the 64-byte piece of a
 // row with bits of its row number.
 //
-// 65536 rows, 2048 x 2048, bf16: 470 to 500 us, 1100 to 1170 TFLOP/s.  The products and their reads from
-// LDS alone take 390 us of it on random numbers (less on zeros: the clock gives way to the power drawn),
-// conversions and stores to LDS the rest.  Half and float pay for each piece of a gradient with a whole
-// product: 50001 rows, 515 x 387, half 73 us (and 9 for its sums) in 128 x 256 tiles that cover 1.65 times dW.
+// 65536 rows, 2048 x 2048, bf16: 468 us on one card, 498 on another (medians of 400 calls) and 13 for the sums
+// of its parts, 1080 to 1140 TFLOP/s.  The products and their reads from LDS alone take 390 us of it on random
+// numbers (less on zeros: the clock gives way to the power drawn), conversions and stores to LDS the rest.
+// Half and float pay for each piece of a gradient with a whole product: 50001 rows, 515 x 387, half 75 us (and
+// 10 for its sums) in 128 x 256 tiles that cover 1.64 times dW.
 //
 // A work-group owns a tile of dW and a range of rows; the parts are summed in their order by a second
 // launch.  Column sums of dY ride along: among the work-groups that share a dY tile, each adds up its
@@ -44,8 +46,8 @@ template <> struct Pieces<bf16_t> { static constexpr int P = 1; };
 template <> struct Pieces<f16_t> { static constexpr int P = 2; };
 template <> struct Pieces<float> { static constexpr int P = 3; };
 
-// A finite value into P > 1 bf16 pieces that add up to it, each the upper half of a float.  An infinity stays
-// in the first; a NaN may lie in the second alone (the first is then an infinity).
+// A finite value into P > 1 bf16 pieces that add up to it (to its multiple of 2^-133), each the upper half of a
+// float.  An infinity stays in the first; a NaN may lie in the second alone (the first is then an infinity).
 template <int P>
 __device__ __forceinline__ void cut(float x, uint32_t *out) {
   out[0] = __float_as_uint(x);

@@ -168,7 +168,7 @@ class GraphVAE(nn.Module):
         `bn{1,2}.weight` / `.bias`; the running statistics stay as they are.  `act_bits` (norm="group"):
         the encoder's activations are kept for the backward in 32 bits or as 8-bit checkpoints, which
         leaves the forward as it is (up to the order of its sums) and gives the gradients the checkpoints'
-        rounding."""
+        rounding.  With "group" the encoder runs in fp32 (with "batch" its forward is evaluated in fp64)."""
         super().__init__()
         norm_options(norm, norm_groups, act_bits, int(hid_dim))
         self.norm, self.norm_groups, self.act_bits = norm, int(norm_groups), int(act_bits)

@@ -139,7 +139,9 @@ _NONE = (None, None)
 class Checkpoint8:
     """An activation kept in 8 bits: `codes` (..., 16*ceil(C/16)) int8 and `scales` (..., ceil(C/32))
     uint8, value = code * 2^(scale - 127) with one scale per 32 consecutive channels of a row (each
-    value off by at most 1/127 of its block's largest).  `channels` is C; `dtype` what `read` returns.
+    value off by at most 1/127 of its block's largest; in a block whose largest is under 2^-119 by at most
+    2^-127, in one within 1 % of the largest float by at most 1/63).  `channels` is C; `dtype` what
+    `read` returns.
 
     Checkpoint8(codes, scales, channels, dtype) wraps existing tensors, which it keeps."""
 
@@ -224,7 +226,7 @@ class Checkpoint8:
 
 def checkpoint8(x: torch.Tensor) -> Checkpoint8:
     """8-bit checkpoint of x (..., C) float32 / bfloat16 / float16: contiguous, or a matrix with any
-    row stride.  A block of 32 channels that holds an infinity or a NaN reads back as NaN."""
+    row stride of at least C.  A block of 32 channels that holds an infinity or a NaN reads back as NaN."""
     if _any_requires_grad(x):
         _refuse_recorded("checkpoint8")
     index = _on_device(x, "checkpoint8")
@@ -304,8 +306,8 @@ def group_norm_act_backward(dy: torch.Tensor, x, weight: torch.Tensor | None, bi
     """Gradients of `group_norm_act`: (dx, dweight, dbias), dx of dy's type, the others float32 (summed
     over graphs and rows in a fixed order).  x: the forward's input, of dy's type, or its Checkpoint8;
     mean, rstd: as the forward returned them; weight, bias, groups, act, rows: as given to it.  dy: like x
-    of any row and batch strides (a gradient expanded over graphs or rows is read in place).  dx of dead
-    rows is 0."""
+    of any row and batch strides (a gradient expanded over graphs or rows is read in place; one expanded over
+    channels is refused).  dx of dead rows is 0."""
     what = "group_norm_act_backward"
     kept = isinstance(x, Checkpoint8)
     if _any_requires_grad(dy, x, weight, bias):
@@ -350,7 +352,8 @@ def group_norm_act_backward(dy: torch.Tensor, x, weight: torch.Tensor | None, bi
 def linear_wgrad8(dy: torch.Tensor, x8: Checkpoint8) -> tuple[torch.Tensor, torch.Tensor]:
     """(dweight (O, I), dbias (O)) of a linear layer y = x W^T + b, in dy's type, from its output's
     gradient dy (..., O) and the checkpoint of its input (..., I).  dy: contiguous, or a matrix with any
-    row stride.  Every product is exact, sums are float32 in a fixed order, rounded once."""
+    row stride of at least O.  Every product is exact (of float32 gradients under 2^-110 what lies below 2^-133
+    is dropped), sums are float32 in a fixed order, rounded once."""
     what = "linear_wgrad8"
     if _any_requires_grad(dy):
         _refuse_recorded(what)

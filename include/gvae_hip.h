@@ -386,8 +386,11 @@ int gvae_sample_decode(const gvae_dims *d, const float *d_params, const float *d
  * (16 * ceil(C/16), zero behind the C-th) and gvae_ckpt8_row_scales(C) = ceil(C/32) scale bytes.
  * The value of channel c is code[c] * 2^(scale[c/32] - 127).  When written, a block's power of two
  * is the least one (at least 2^-126) of which 127 reach the block's largest magnitude, and codes
- * are rounded to nearest, ties to even; a block with an infinity or a NaN gets the scale byte 255
- * and reads as NaN.  Codes and workspaces must be 16-byte aligned. */
+ * are rounded to nearest, ties to even: off by half the power of two at most, which is under 1/127 of the
+ * largest magnitude unless the power is 2^-126.  At 2^122 (a largest magnitude over 127 * 2^121) codes end at
+ * 63 in magnitude and are off by 2^122 at most.  A block with an infinity or a NaN gets the scale byte 255 and
+ * reads as NaN; a scale byte of 0, which is never written, reads as 0.  Codes and workspaces must be
+ * 16-byte aligned. */
 int gvae_ckpt8_row_bytes(int C);
 int gvae_ckpt8_row_scales(int C);
 /* d_x: (rows, C) with unit channel stride and row_stride elements between rows. */
@@ -428,8 +431,8 @@ int gvae_group_norm_bwd(const void *d_dy, int dtype, int64_t dy_batch_stride, in
 
 /* Weight and bias gradient of a linear layer whose input (rows, I) was kept as a checkpoint:
  * d_dw (O, I) = dY^T x, d_db (O) = column sums of dY (may be NULL), both contiguous and of dY's type.
- * Every product of a gradient and a checkpointed value enters the sums exactly; sums are fp32, in a
- * fixed order.  d_ws: gvae_linear_wgrad8_ws_bytes(rows, O, I) bytes. */
+ * Every product of a gradient and a checkpointed value enters the sums exactly (of fp32 gradients under
+ * 2^-110 what lies below 2^-133 is dropped); sums are fp32, in a fixed order.  d_ws: gvae_linear_wgrad8_ws_bytes(rows, O, I) bytes. */
 int64_t gvae_linear_wgrad8_ws_bytes(int64_t rows, int O, int I);
 int gvae_linear_wgrad8(const void *d_dy, int dtype, int64_t row_stride, const int8_t *d_codes,
                        const uint8_t *d_scales, int64_t rows, int O, int I, void *d_dw, void *d_db, void *d_ws,
@@ -449,9 +452,9 @@ typedef struct gvae_gn_opts {
 int64_t gvae_step_gn_ws_bytes(const gvae_dims *d, const gvae_gn_opts *gn, int n_graphs);
 
 /* gvae_step_forward_model with group norm (no statistics to update, hence no mode argument).  The
- * workspace (gvae_step_gn_ws_bytes) then takes gvae_step_forward_match_loss as it does after
- * gvae_step_forward_model, and gvae_step_gn_backward with the same options.  gvae_step_read_debug
- * knows the buffers 0-8, 13, 16 and 17 in it. */
+ * encoder is evaluated in fp32.  The workspace (gvae_step_gn_ws_bytes) then takes
+ * gvae_step_forward_match_loss as it does after gvae_step_forward_model, and gvae_step_gn_backward with
+ * the same options.  gvae_step_read_debug knows the buffers 0-8, 13, 16 and 17 in it. */
 int gvae_step_gn_forward_model(const gvae_dims *d, const gvae_gn_opts *gn, const float *d_params, const float *d_x,
                                const float *d_adj, const int32_t *d_n_x, const int32_t *d_R, int n_graphs,
                                const float *d_eps, void *d_ws, void *stream);
