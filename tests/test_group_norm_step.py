@@ -332,8 +332,8 @@ def test_a_trained_run_evaluates_as_it_was_trained(tmp_path):
     from graphvae.data import synthetic_batch
     from graphvae.models import GraphVAE
     from graphvae.train import train_ddp as T
-    T.main(["--dataset", "synthetic-dense", "--feature_type", "deg", "--max_nodes", "16", "--epochs", "1", "--norm", "group",
-            "--norm_groups", "4", "--act_bits", "8", "--log_dir", str(tmp_path), "--no_wandb"])
+    T.main(["--dataset", "synthetic-dense", "--feature_type", "deg", "--max_nodes", "16", "--epochs", "1", "--norm",
+            "group", "--norm_groups", "4", "--act_bits", "8", "--log_dir", str(tmp_path), "--no_wandb"])
     loaded = _load_model(tmp_path, DEV)
     hid, z = loaded.hid_dim, loaded.z_dim
     built = GraphVAE(1, hid, z, 16, norm="group", norm_groups=4, act_bits=8)
@@ -374,3 +374,24 @@ def test_steps_in_flight_equal_the_sequential_schedule(matching, bits):
         runs.append([torch.stack(outs).cpu(), step.pop_loss_sum().cpu(), model.flat_parameters().detach().cpu().clone()])
         model._engine.check_matching()
     assert torch.isfinite(runs[0][2]).all() and all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_smaller_batch_behind_a_larger_one(bits):
+    """512 graphs behind 513, whose workspace is smaller: losses and gradients are those of a model that has seen the
+    512 alone."""
+    from graphvae.data import synthetic_batch
+    hb = synthetic_batch("dense", 513, 32, "deg", seed=8)
+    large, small = hb.to(DEV), hb.index(range(512)).to(DEV)
+    eps = torch.randn(513, 16, generator=torch.Generator().manual_seed(8)).to(DEV)
+    runs = []
+    for batches in ((small,), (large, small)):
+        model, _ = _model(1, 128, 16, 32, 8, bits, hb, matching="none")
+        model = model.to(DEV).train()
+        for b in batches:
+            model.zero_grad(set_to_none=True)
+            out = model.forward_with_eps(b, eps[:b.num_graphs].contiguous())
+            (out["rec"] + out["kl"]).backward()
+        runs.append([out["rec"].detach(), out["kl"].detach(), *(p.grad for p in model.parameters() if p.grad is not None)])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
